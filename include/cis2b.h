@@ -258,6 +258,128 @@ int cis2b_op_sample_gumbel(int32_t device, const float *logits, int32_t n, float
 int cis2b_op_sample_static(int32_t device, const float *d_logits, int32_t n, float temperature, float top_p,
                            uint64_t seed, uint64_t position, uint32_t *d_out_index, void *stream);
 
+/* ---- 4-bit key/value cache ----------------------------------------------
+ * No counterpart in the reference.  A paged cache that holds keys and values
+ * in 4 bits, for callers that run their own layers: the step's block tables
+ * and slot maps built on the GPU, rows quantised into the cache and read
+ * back, and causal attention over it with an optional sliding window and
+ * sinks.  Results are approximate (4 bits) and outside the witness; every
+ * call is deterministic: the same inputs give the same bits.
+ *
+ * These entry points take DEVICE pointers, run asynchronously on `stream`
+ * (NULL: the legacy default stream), allocate nothing and can be captured in
+ * a CUDA graph.  They make the cache's device current on the calling thread.
+ *
+ * Format.  A group is one token's head_dim elements of one KV head:
+ *   base = min(x) rounded down to bfloat16
+ *   step = (max(x) - base) / 15 rounded up to bfloat16, 0 if below 2^-100
+ *   code = rint((x - base) * (1 / step)) clamped to 0..15, 0 if step is 0
+ * each operation rounded to fp32; a code stands for base + step * code.  A
+ * group with a NaN or an infinity, or whose range passes fp32's, reads back
+ * as NaN.  Per page and KV head the pool holds page_size / 16 records of 16
+ * tokens: 16 x head_dim/2 bytes of key codes (byte b: element 2b in the low
+ * four bits, 2b + 1 in the high), the same of value codes, then 16 x {key
+ * step, key base, value step, value base} as bfloat16. */
+#define CIS2B_F32 0
+#define CIS2B_F16 1
+#define CIS2B_BF16 2
+
+typedef struct {
+  int32_t device;
+  int32_t pages;     /* >= 1; pages * page_size < 2^31 */
+  int32_t page_size; /* tokens: 16, 32, 64, 128 or 256 */
+  int32_t kv_heads;  /* >= 1 */
+  int32_t head_dim;  /* 64 or 128 */
+  int32_t reserved;  /* must be zero */
+  void *pool;        /* cis2b_kv4_bytes() bytes, 16-byte aligned */
+  int32_t *status;   /* one word or NULL: bits OR-ed in by the kernels, CIS2B_KV4_BAD_* */
+} cis2b_kv4_cache;
+
+#define CIS2B_KV4_BAD_SLOT 1 /* a slot >= pages * page_size; the row was skipped */
+#define CIS2B_KV4_BAD_PAGE 2 /* a visible key on a page that is not in the pool; it was not seen */
+
+/* Bytes of the pool: pages * kv_heads * page_size * (head_dim + 8). */
+int cis2b_kv4_bytes(const cis2b_kv4_cache *c, uint64_t *out_bytes);
+
+/* Plans one step of a batch: request r holds cached[r] tokens and adds
+ * new_tokens[r] (0 or more).  Its rows are row_start[r] .. row_start[r+1]-1
+ * of the step's tensors, in request order.  Pages that it needs beyond
+ * ceil(cached / page_size) are taken from free_pages in request order and
+ * entered in its row of `table`; other entries are left as they are.
+ *   length     [requests]      cached + new_tokens
+ *   row_start  [requests + 1]  prefix sums of new_tokens
+ *   slot, position, request [rows]  of each row: page * page_size + offset in
+ *              the cache, position in the request, request; -1 in the rows
+ *              past row_start[requests]
+ *   counts     [4]  rows in use, pages needed, CIS2B_KV4_PLAN_* bits, 0
+ * A row whose page is missing (bits FREE, WIDTH) has slot -1.  At most 16384
+ * requests.  Work that a later call must see goes on the same stream. */
+#define CIS2B_KV4_PLAN_FREE 1     /* more pages needed than free_count */
+#define CIS2B_KV4_PLAN_WIDTH 2    /* a request longer than width * page_size */
+#define CIS2B_KV4_PLAN_ROWS 4     /* more new tokens than `rows` */
+#define CIS2B_KV4_PLAN_NEGATIVE 8 /* a negative cached or new_tokens; taken as 0 */
+typedef struct {
+  int32_t device;
+  int32_t requests;   /* 1 .. 16384 */
+  int32_t rows;       /* capacity of slot, position and request; >= 0 */
+  int32_t width;      /* entries per row of table */
+  int32_t page_size;  /* 16, 32, 64, 128 or 256 */
+  int32_t free_count; /* entries of free_pages */
+  const int32_t *cached, *new_tokens; /* [requests] */
+  const int32_t *free_pages;          /* [free_count]; may be NULL if 0 */
+  int32_t *table;                     /* [requests][width] */
+  int32_t *length, *row_start;
+  int32_t *slot, *position, *request; /* may be NULL if rows is 0 */
+  int32_t *counts;
+} cis2b_kv4_step;
+int cis2b_kv4_plan(const cis2b_kv4_step *s, void *stream);
+
+/* Quantises rows k, v [rows][kv_heads][head_dim] (elements of a head
+ * contiguous; row and head strides in elements) into their slots.  A
+ * negative slot skips its row.  Slots in one call must differ. */
+int cis2b_kv4_append(const cis2b_kv4_cache *c, int32_t dtype, const void *k, const void *v,
+                     int64_t k_row_stride, int64_t k_head_stride, int64_t v_row_stride, int64_t v_head_stride,
+                     const int32_t *slot, int32_t rows, void *stream);
+/* Reads the rows of `slot` back as the values that their codes stand for,
+ * into contiguous k, v [rows][kv_heads][head_dim]; zeros for negative slots
+ * and slots out of range. */
+int cis2b_kv4_gather(const cis2b_kv4_cache *c, int32_t dtype, void *k, void *v, const int32_t *slot, int32_t rows,
+                     void *stream);
+
+/* Causal attention of the step's rows over the cache (their own keys and
+ * values appended before).  Row i of request r stands at position
+ * p = length[r] - (row_start[r+1] - row_start[r]) + i - row_start[r] and sees
+ * keys j <= p with, if window > 0, j > p - window or j < sinks.  Query head h
+ * reads KV head h / (heads / kv_heads).  Rows that see nothing, and rows past
+ * row_start[requests], are zero.
+ *   max_new    the most rows of any one request, or a bound (chooses the
+ *              kernel; a request with more is still computed)
+ *   scale      factor of the scores (1 / sqrt(head_dim) in most models)
+ *   work       cis2b_kv4_workspace() bytes, zeroed once before the first
+ *              call; calls that may overlap on the GPU need one each
+ * Softmax statistics and sums are held in fp32; fp32 rows keep 22 bits of
+ * every product's operands, 16-bit rows at least 11. */
+typedef struct {
+  int32_t dtype;    /* CIS2B_F32, _F16 or _BF16: q and out */
+  int32_t heads;    /* a multiple of kv_heads, at most 32 times as many */
+  int32_t requests; /* >= 1 */
+  int32_t rows;     /* rows of q and out */
+  int32_t width;    /* entries per row of table */
+  int32_t max_new;  /* >= 1 */
+  int32_t window;   /* 0: none */
+  int32_t sinks;    /* >= 0 */
+  float scale;
+  int32_t reserved; /* must be zero */
+  const void *q;
+  void *out;        /* [rows][heads][head_dim]; strides in elements, heads' elements contiguous */
+  int64_t q_row_stride, q_head_stride, out_row_stride, out_head_stride;
+  const int32_t *table, *length, *row_start;
+  void *work;       /* 16-byte aligned */
+  uint64_t work_bytes;
+} cis2b_kv4_attn;
+int cis2b_kv4_workspace(const cis2b_kv4_cache *c, const cis2b_kv4_attn *a, uint64_t *out_bytes);
+int cis2b_kv4_attention(const cis2b_kv4_cache *c, const cis2b_kv4_attn *a, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
