@@ -75,6 +75,41 @@ __device__ __forceinline__ void load8(const void *base, int64_t at, bool wide, f
   }
 }
 
+// N consecutive query elements as float32, zeros where `on` is not set: fp32,
+// or 16-bit elements of a type known at run time.  All loads are issued before
+// anything is done with them.
+template <bool F32, int N>
+__device__ __forceinline__ void load_query(const void *base, bool bf16, int64_t at, bool wide, bool on, float (&x)[N]) {
+  constexpr int WORDS = F32 ? N : N / 2;
+  uint32_t w[WORDS];
+#pragma unroll
+  for (int i = 0; i < WORDS; ++i) w[i] = 0;
+  const uint8_t *p = static_cast<const uint8_t *>(base) + at * (F32 ? 4 : 2);
+  if (on && wide) {
+#pragma unroll
+    for (int i = 0; i < WORDS; i += 4) {
+      const uint4 a = __ldg(reinterpret_cast<const uint4 *>(p) + i / 4);
+      w[i] = a.x, w[i + 1] = a.y, w[i + 2] = a.z, w[i + 3] = a.w;
+    }
+  } else if (on) {
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) {
+      if constexpr (F32) w[i] = __ldg(reinterpret_cast<const uint32_t *>(p) + i);
+      else w[i] = __ldg(reinterpret_cast<const uint16_t *>(p) + 2 * i) |
+                  (uint32_t)__ldg(reinterpret_cast<const uint16_t *>(p) + 2 * i + 1) << 16;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if constexpr (F32) {
+      x[i] = __uint_as_float(w[i]);
+    } else {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i / 2]));
+      x[i] = (i & 1) ? (bf16 ? bf16_hi(w[i / 2]) : f.y) : (bf16 ? bf16_lo(w[i / 2]) : f.x);
+    }
+  }
+}
+
 __device__ __forceinline__ uint32_t pack_half(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t *>(&h);
@@ -108,6 +143,21 @@ __device__ __forceinline__ void store8(void *base, int dt, int64_t at, bool wide
 #pragma unroll
     for (int i = 0; i < 4; ++i) p[2 * i] = (uint16_t)w[i], p[2 * i + 1] = (uint16_t)(w[i] >> 16);
   }
+}
+
+// Four, where an aligned address is one of 8 or 16 bytes.
+__device__ __forceinline__ void store4(void *base, int dt, int64_t at, bool wide, float4 x) {
+  if (dt == KV4_F32) {
+    float *p = static_cast<float *>(base) + at;
+    if (wide) *reinterpret_cast<float4 *>(p) = x;
+    else p[0] = x.x, p[1] = x.y, p[2] = x.z, p[3] = x.w;
+    return;
+  }
+  const uint32_t a = dt == KV4_F16 ? pack_half(x.x, x.y) : pack_bf16(x.x, x.y);
+  const uint32_t b = dt == KV4_F16 ? pack_half(x.z, x.w) : pack_bf16(x.z, x.w);
+  uint16_t *p = static_cast<uint16_t *>(base) + at;
+  if (wide) *reinterpret_cast<uint2 *>(p) = make_uint2(a, b);
+  else p[0] = (uint16_t)a, p[1] = (uint16_t)(a >> 16), p[2] = (uint16_t)b, p[3] = (uint16_t)(b >> 16);
 }
 
 }  // namespace cis2b

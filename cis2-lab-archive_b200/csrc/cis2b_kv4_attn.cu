@@ -19,11 +19,11 @@
 namespace cis2b {
 namespace {
 
-constexpr int ATT_WARPS = 4;
+constexpr int ATT_WARPS = 8;
 constexpr int ATT_THREADS = 32 * ATT_WARPS;
-constexpr int ATT_CHUNK = 32;       // least records (of 16 keys) per split of a request
-constexpr int ATT_MAX_SPLITS = 64;  // per (query tile, KV head)
-constexpr uint64_t ATT_PART_BYTES = 64ull << 20;  // partial results of the splits
+constexpr int ATT_LEAST = 8;   // least records (of 16 keys) that a warp is given
+constexpr int ATT_SETUP = 6;   // what an item's fixed costs come to, in records
+constexpr int ATT_MEET = 8;    // what joining the parts of several blocks comes to, in records
 
 struct AttArgs {
   const void *q;
@@ -32,17 +32,18 @@ struct AttArgs {
   const uint8_t *pool;
   int32_t *status;
   const int32_t *table, *length, *row_start;
-  float *part;        // [part_units][cols][HD + 2]
-  uint32_t *counter;  // [query tiles][kv_heads]
+  float *part;        // [10 or 18 per block][cols][HD + 2], see PART below
+  uint32_t *counter;  // [items]
   int dtype, requests, rows, width, kv_heads, group, shift, pages, window, sinks;
   int q_wide, o_wide;
   int qt;             // tokens per query tile
-  int part_units, counters;
+  int items, whole;   // a bound on the items; whole items per block
   float scale;
+  float per_warp;     // 1 / warps of the grid, rounded up
 };
 
-// What the splitting rule and the kernel must agree on: the keys that one
-// query tile sees, as 16-key records 0 .. sink_recs-1 and lo .. hi-1.
+// The keys that one query tile sees, as 16-key records 0 .. sink-1 and
+// lo .. hi-1.
 struct Span {
   int p0, p1;     // first and last position of the tile's rows (p1 < 0: none sees anything)
   int sink, lo;   // records before the gap, first record after it (0 and 0 without one)
@@ -66,14 +67,14 @@ __device__ __forceinline__ Span span_of(const AttArgs &a, int len, int n, int qt
   return s;
 }
 
-// Splits of a request: by its own length and rows alone, so that what else is
-// in the batch does not change its result (unless the partial results outgrow
-// the workspace, where `coarse` doubles the chunk).
-__device__ __forceinline__ int splits_of(const AttArgs &a, int tiles, int query_tiles, int coarse) {
-  const int most = max(1, ATT_MAX_SPLITS * 8 / max(1, query_tiles * a.kv_heads));
-  return max(1, min(min((tiles + (ATT_CHUNK << coarse) - 1) / (ATT_CHUNK << coarse), ATT_MAX_SPLITS), most));
+// A bound on span_of().tiles over the query tiles of a request: what each of
+// them counts as when the work is shared out.
+__device__ __forceinline__ int tiles_bound(const AttArgs &a, int len) {
+  const int all = (len + 15) >> 4;
+  if (!a.window) return max(all, 1);
+  const int some = ((min(a.sinks, len) + 15) >> 4) + ((min(a.window, len) + a.qt - 2) >> 4) + 2;
+  return max(min(all, some), 1);
 }
-
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                          uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -85,8 +86,35 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src));
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool on) {
+  asm volatile("{.reg .pred p; setp.ne.b32 p, %2, 0; @p cp.async.cg.shared.global [%0], [%1], 16;}" ::"r"(dst), "l"(src),
+               "r"((int)on));
+}
+// Four 8 x 8 matrices of 16-bit units, transposed: lane (g, t) gets units
+// (2t, g) and (2t + 1, g) of each; lane l gives row l % 8 of matrix l / 8.
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+// Pairs of fp32 numbers in one instruction.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{.reg .b64 x, y, z; mov.b64 x, {%2,%3}; mov.b64 y, {%4,%5}; mul.rn.f32x2 z, x, y; mov.b64 {%0,%1}, z;}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{.reg .b64 x, y, z; mov.b64 x, {%2,%3}; mov.b64 y, {%4,%5}; add.rn.f32x2 z, x, y; mov.b64 {%0,%1}, z;}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{.reg .b64 x, y, z, w; mov.b64 x, {%2,%3}; mov.b64 y, {%4,%5}; mov.b64 z, {%6,%7}; fma.rn.f32x2 w, x, y, z; "
+      "mov.b64 {%0,%1}, w;}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;"); }
 template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N)); }
@@ -99,6 +127,53 @@ __device__ __forceinline__ float lg2(float x) {
   float y;
   asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// Four elements of a column's result: numerators over the denominator (zero
+// where nothing was seen).
+__device__ __forceinline__ void emit(const AttArgs &a, int row0, int head, int col, int d, float4 x, float den) {
+  const float f = den > 0.0f || den != den ? 1.0f / den : 0.0f;
+  const int tok = col / a.group;
+  const int64_t row = (int64_t)row0 + tok;
+  if (row >= 0 && row < a.rows)
+    store4(a.out, a.dtype, row * a.o_row + (int64_t)(head * a.group + col - tok * a.group) * a.o_head + d, a.o_wide,
+           make_float4(x.x * f, x.y * f, x.z * f, x.w * f));
+}
+
+// Parts of a column joined, four elements of it: n parts `stride` floats apart,
+// then one more at `extra` (unless NULL).  col_at and ml_at are the places of
+// the elements and of (maximum, denominator) in a part.
+struct Joined {
+  float4 x;
+  float m, den;
+};
+__device__ __forceinline__ Joined join_parts(const float *p, int64_t stride, int n, const float *extra, int col_at, int ml_at) {
+  Joined s = {make_float4(0, 0, 0, 0), -1e30f, 0.0f};
+  const int all = n + (extra != nullptr);
+  constexpr int AT_ONCE = 4;
+  for (int k = 0; k < all; k += AT_ONCE) {
+    float4 y[AT_ONCE];
+    float2 ml[AT_ONCE];
+    float top = s.m;
+#pragma unroll
+    for (int e = 0; e < AT_ONCE; ++e) {
+      const float *q = k + e < n ? p + (k + e) * stride : extra;
+      ml[e] = make_float2(-1e30f, 0.0f), y[e] = make_float4(0, 0, 0, 0);
+      if (k + e < all) ml[e] = *reinterpret_cast<const float2 *>(q + ml_at), y[e] = *reinterpret_cast<const float4 *>(q + col_at);
+    }
+#pragma unroll
+    for (int e = 0; e < AT_ONCE; ++e) top = fmaxf(top, ml[e].x);
+    const float keep = ex2(s.m - top);
+    s.m = top, s.den *= keep, s.x.x *= keep, s.x.y *= keep, s.x.z *= keep, s.x.w *= keep;
+#pragma unroll
+    for (int e = 0; e < AT_ONCE; ++e) {
+      const float f = ex2(ml[e].x - top);
+      s.den = fmaf(f, ml[e].y, s.den);
+      s.x.x = fmaf(f, y[e].x, s.x.x), s.x.y = fmaf(f, y[e].y, s.x.y);
+      s.x.z = fmaf(f, y[e].z, s.x.z), s.x.w = fmaf(f, y[e].w, s.x.w);
+    }
+  }
+  return s;
 }
 
 // Codes of a 16-bit half each, as half-precision operands.  EXACT: the normal
@@ -118,18 +193,35 @@ template <bool EXACT> __device__ __forceinline__ uint32_t codes_high(uint32_t x)
   return *reinterpret_cast<const uint32_t *>(&h);
 }
 
-template <int HD, int NT, int LIMBS> __host__ __device__ constexpr int att_stages() { return HD == 64 ? 6 : 4; }
-template <int HD, int NT, int LIMBS> __host__ __device__ constexpr int att_ring_bytes() {
-  const int ring = ATT_WARPS * att_stages<HD, NT, LIMBS>() * kv4_rec_bytes(HD);
-  const int merge = 2 * 8 * NT * HD * 4;  // two warps' sums, reusing the ring
-  return ring > merge ? ring : merge;
+// Records that a warp takes per iteration (one where 32 columns fill the
+// registers), iterations in its ring, and the shared memory of a block: its
+// warps' rings, then their query operands.
+__host__ __device__ constexpr int att_pair(int nt) { return nt < 4 ? 2 : 1; }
+__host__ __device__ constexpr int att_stages(int hd, int nt) { return nt < 4 ? (hd == 64 ? 4 : 3) : (hd == 64 ? 6 : 4); }
+__host__ __device__ constexpr int att_ring_bytes(int hd, int nt) {
+  return ATT_WARPS * att_stages(hd, nt) * att_pair(nt) * kv4_rec_bytes(hd);
 }
-template <int HD, int NT, int LIMBS> __host__ __device__ constexpr int att_smem_bytes() {
-  return att_ring_bytes<HD, NT, LIMBS>() + NT * LIMBS * (HD / 32) * 512;
+__host__ __device__ constexpr int att_smem_bytes(int hd, int nt, int limbs) {
+  return att_ring_bytes(hd, nt) + (nt > 1 ? ATT_WARPS * nt * limbs * (hd / 32) * 512 : 0);
 }
 
-// One block takes units (request, query tile, split, KV head) in turn; its
-// four warps take the unit's records in turn and meet at the end.
+__host__ __device__ constexpr bool att_on_shared(int hd, int nt) {
+  return 8 * nt * (hd + 2) * 4 <= att_stages(hd, nt) * att_pair(nt) * kv4_rec_bytes(hd);
+}
+__host__ __device__ constexpr int att_parts(int hd, int nt) { return ATT_WARPS + 2 + (att_on_shared(hd, nt) ? 0 : ATT_WARPS); }
+
+// An item is a query tile of one request and one KV head.  The records of all
+// items stand in one row, (request, query tile, KV head, record), with a gap
+// of ATT_SETUP before each item for its fixed costs, and every warp of the
+// grid takes an equal stretch of it: each has the same work, whatever the
+// requests' lengths, and none waits for another on the way.  Items that are
+// cut are put together at the end: the parts of a block's eight warps in
+// shared memory, the parts of several blocks through the workspace by the
+// last block to arrive.  Both join parts in the order of their records, so
+// the result does not depend on which block that is.  Where items are short,
+// and with CIS2B_KV4_WHOLE, a block takes whole items in turn, an eighth per
+// warp, and nothing is left for other blocks; a row's result then does not
+// depend on the rest of the batch.
 //
 // The codes reach the tensor pipe without being converted: a code in bits
 // 0-3 of a 16-bit word IS the half-precision number c * 2^-24 (a subnormal),
@@ -154,105 +246,175 @@ template <int HD, int NT, int LIMBS> __host__ __device__ constexpr int att_smem_
 // rounding's effect: directly for fp32 rows, by the sum of the rounded
 // weights (a product with ones) for 16-bit rows.
 template <int HD, int NT, int LIMBS>
-__global__ __launch_bounds__(ATT_THREADS) void k_kv4_attention(AttArgs a) {
-  constexpr int REC = kv4_rec_bytes(HD), ST = att_stages<HD, NT, LIMBS>();
+__global__ __launch_bounds__(ATT_THREADS, NT == 1 ? 2 : 1) void k_kv4_attention(AttArgs a) {
+  constexpr int REC = kv4_rec_bytes(HD), ST = att_stages(HD, NT), RP = att_pair(NT);
   constexpr int KS = HD / 16;            // k-steps of the first product, row tiles of the second
   constexpr int W = HD / 32;             // 32-bit words of a key row per lane
   constexpr int COLS = 8 * NT;
   constexpr bool EXACT = LIMBS == 2;
+  // Parts that a block has in the workspace: items that end in each warp, the
+  // block's first and last item, and, where a ring cannot hold one, items
+  // that go on after each warp.
+  constexpr bool ON_SHARED = att_on_shared(HD, NT);
+  constexpr int PARTS = att_parts(HD, NT);
   constexpr float UNIT = EXACT ? 1.0f : 16777216.0f;  // what a code's operand is divided by
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ int scan_u[ATT_THREADS + 1], scan_q[ATT_THREADS + 1], warp_u[ATT_WARPS], warp_q[ATT_WARPS];
-  __shared__ float red[ATT_WARPS][3][COLS];  // M, l and the base sum of each warp
-  __shared__ int last;
+  __shared__ int scan_t[ATT_THREADS], scan_q[ATT_THREADS], warp_t[ATT_WARPS], warp_q[ATT_WARPS], warp_top[ATT_WARPS];
+  __shared__ int req_len[ATT_THREADS], req_row[ATT_THREADS], req_n[ATT_THREADS];  // of up to as many requests
+  // Each warp's cut items: one that ends in it, one that goes on after it.
+  struct Cut {
+    int item, row0, head, ncol, begin, size;  // begin and size: its stretch of the row
+  };
+  __shared__ Cut cut_end[ATT_WARPS], cut_on[ATT_WARPS];
+  __shared__ int has_end[ATT_WARPS], on_kind[ATT_WARPS];  // on: 0 none, 1 the item begins here, 2 it began before
+  struct Run {  // the parts of one item within the block: `on` of warps w .., then the one that ends it
+    int on, end, side;  // end: its warp or -1; side: 0 began before the block, 1 goes on after it, 2 done here, -1 no run
+  };
+  __shared__ Run run[ATT_WARPS + 1];  // by the warp it begins in; the last: what began before the block
+  __shared__ Cut edge[2];       // the block's items that began before it and that go on after it
+  __shared__ int edge_last[2];  // 0: no such item, 1: left to another block, 2: to be joined here
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-  uint8_t *ring = smem + warp * ST * REC;
-  uint4 *qfrag = reinterpret_cast<uint4 *>(smem + att_ring_bytes<HD, NT, LIMBS>());
+  uint8_t *ring = smem + warp * ST * RP * REC;
+  uint4 *qfrag = reinterpret_cast<uint4 *>(smem + att_ring_bytes(HD, NT)) + warp * (NT * LIMBS * W * 32);
 
-  // Rows past the last request are zero.
-  {
-    const int used = max(0, min(__ldg(a.row_start + a.requests), a.rows));
-    const float zero[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    const int64_t per = (int64_t)a.kv_heads * a.group * (HD / 8);
-    for (int64_t i = (int64_t)blockIdx.x * ATT_THREADS + tid; i < (a.rows - used) * per; i += gridDim.x * ATT_THREADS) {
-      const int64_t row = used + i / per;
-      const int h = (int)(i % per) / (HD / 8), d = (int)(i % (HD / 8)) * 8;
-      store8(a.out, a.dtype, row * a.o_row + h * a.o_head + d, a.o_wide, zero);
-    }
-  }
-
-  // Units before each request: thread i sums requests i * per .. of its own.
+  // Records (with the gaps) and items before each request: thread i sums
+  // requests i * per .. of its own.
   const int per = (a.requests + ATT_THREADS - 1) / ATT_THREADS;
-  int coarse = 0, total = 0;
-  for (;; ++coarse) {
-    int64_t units = 0;
-    int tiles_q = 0;
-    int64_t split_units = 0;
-    for (int i = 0; i < per; ++i) {
-      const int r = tid * per + i;
-      if (r >= a.requests) break;
-      const int len = __ldg(a.length + r), n = __ldg(a.row_start + r + 1) - __ldg(a.row_start + r);
+  int all_tiles = 0, all_q = 0, top_tiles = 1;
+  {
+    int st = 0, sq = 0, top = 1;
+    for (int r = tid * per; r < min(tid * per + per, a.requests); ++r) {
+      const int row = __ldg(a.row_start + r), n = __ldg(a.row_start + r + 1) - row, len = __ldg(a.length + r);
+      if (per == 1) req_len[r] = len, req_row[r] = row, req_n[r] = n;
       if (n <= 0) continue;
-      const int nq = (n + a.qt - 1) / a.qt;
-      const int sp = splits_of(a, span_of(a, len, n, nq - 1).tiles, nq, coarse);
-      units += (int64_t)nq * sp;
-      tiles_q += nq;
-      if (sp > 1) split_units += (int64_t)nq * sp;
+      const int nq = n <= a.qt ? 1 : (n + a.qt - 1) / a.qt;
+      const int vt = tiles_bound(a, len);
+      st += nq * (vt + ATT_SETUP), sq += nq, top = max(top, vt);
     }
-    int u = (int)min(units, (int64_t)INT_MAX / 1024), sq = tiles_q;
-    const int own_u = u, own_q = sq;
+    const int own_t = st, own_q = sq;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-      const int x = __shfl_up_sync(0xffffffffu, u, d), y = __shfl_up_sync(0xffffffffu, sq, d);
-      if (lane >= d) u += x, sq += y;
+      const int x = __shfl_up_sync(0xffffffffu, st, d), y = __shfl_up_sync(0xffffffffu, sq, d);
+      if (lane >= d) st += x, sq += y;
     }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (lane == 31) warp_t[warp] = st, warp_q[warp] = sq, warp_top[warp] = top;
     __syncthreads();
-    if (lane == 31) warp_u[warp] = u, warp_q[warp] = sq;
-    __syncthreads();
-    int before_u = 0, before_q = 0;
-    total = 0;
+    int before_t = 0, before_q = 0;
 #pragma unroll
     for (int w = 0; w < ATT_WARPS; ++w) {
-      if (w < warp) before_u += warp_u[w], before_q += warp_q[w];
-      total += warp_u[w];
+      if (w < warp) before_t += warp_t[w], before_q += warp_q[w];
+      all_tiles += warp_t[w], all_q += warp_q[w], top_tiles = max(top_tiles, warp_top[w]);
     }
-    scan_u[tid] = before_u + u - own_u;
-    scan_q[tid] = before_q + sq - own_q;
-    if (tid == ATT_THREADS - 1) scan_u[ATT_THREADS] = before_u + u, scan_q[ATT_THREADS] = before_q + sq;
-    // Partial results are kept by unit: enough room, or a coarser chunk (at
-    // last one split, which needs none).
-    const bool fits = (int64_t)total * a.kv_heads <= a.part_units;
-    const int any = __syncthreads_or(split_units > 0);
-    if (fits || !any) break;
+    scan_t[tid] = (before_t + st - own_t) * a.kv_heads;
+    scan_q[tid] = (before_q + sq - own_q) * a.kv_heads;
+    __syncthreads();
   }
-  const int64_t all_units = (int64_t)total * a.kv_heads;
+  all_tiles *= a.kv_heads;
+  const int items = all_q * a.kv_heads;
+  // A range's records: an equal share, but not so few that the joins outweigh them.
+  const int range = (int)blockIdx.x * ATT_WARPS + warp;
+  const int each = max(__float2int_ru(__fmul_ru(__int2float_ru(all_tiles), a.per_warp)), ATT_LEAST);
+  // Whole items, too, where the longest is short enough that a block's turns
+  // take no longer than an even share and joining its ends.
+  const int turns = (int)((uint32_t)(items + gridDim.x - 1) / gridDim.x);
+  const bool whole = a.whole || (turns <= 64 && turns * ((top_tiles + ATT_WARPS - 1) / ATT_WARPS + ATT_SETUP) <= each + ATT_SETUP + ATT_MEET);
+  const int *scan = whole ? scan_q : scan_t;
 
-  for (int64_t unit = blockIdx.x; unit < all_units; unit += gridDim.x) {
-    // ---- which unit
-    const int head = (int)(unit % a.kv_heads), ub = (int)(unit / a.kv_heads);
-    int seg = 0;
-    for (int step = ATT_THREADS / 2; step; step >>= 1)
-      if (scan_u[seg + step] <= ub) seg += step;
-    int u = scan_u[seg], qbase = scan_q[seg], r = seg * per, n = 0, len = 0, nq = 0, sp = 1;
-    for (;; ++r) {
-      len = __ldg(a.length + r);
-      n = __ldg(a.row_start + r + 1) - __ldg(a.row_start + r);
-      if (n <= 0) continue;
-      nq = (n + a.qt - 1) / a.qt;
-      sp = splits_of(a, span_of(a, len, n, nq - 1).tiles, nq, coarse);
-      if (ub < u + nq * sp) break;
-      u += nq * sp, qbase += nq;
+  for (int turn_at = blockIdx.x;; turn_at += gridDim.x) {  // once, or once per whole item
+  int at = whole ? turn_at : (int)min((int64_t)range * each, (int64_t)all_tiles);
+  const int end = whole ? (turn_at < items ? turn_at + 1 : turn_at) : (int)min((int64_t)at + each, (int64_t)all_tiles);
+  if (whole ? at >= end : (int64_t)blockIdx.x * ATT_WARPS * each >= all_tiles) break;  // as one block
+  if (lane == 0) has_end[warp] = on_kind[warp] = 0;
+  while (at < end) {
+    // ---- which item, and which of its records
+    int seg;
+    {
+      const uint32_t coarse = __ballot_sync(0xffffffffu, scan[lane * (ATT_THREADS / 32)] <= at);
+      seg = (31 - __clz(coarse)) * (ATT_THREADS / 32);
+      const uint32_t fine = __ballot_sync(0xffffffffu, scan[seg + (lane & (ATT_THREADS / 32 - 1))] <= at);
+      seg += 31 - __clz(fine & ((1u << (ATT_THREADS / 32)) - 1));
     }
-    const int qi = (ub - u) / sp, split = (ub - u) - qi * sp;
+    int base = scan[seg], qbase = scan_q[seg], r = seg * per, n, len, row0, nq, vt, size;
+    for (;; ++r) {
+      if (per == 1) {
+        len = req_len[r], row0 = req_row[r], n = req_n[r];
+      } else {
+        len = __ldg(a.length + r), row0 = __ldg(a.row_start + r), n = __ldg(a.row_start + r + 1) - row0;
+      }
+      if (n <= 0) continue;
+      nq = n <= a.qt ? 1 : (n + a.qt - 1) / a.qt;
+      vt = tiles_bound(a, len);
+      size = whole ? 1 : vt + ATT_SETUP;  // of one item in the row
+      const int next = base + nq * a.kv_heads * size;
+      if (at < next) break;
+      base = next, qbase += nq * a.kv_heads;
+    }
+    const int item = (int)((uint32_t)(at - base) / (uint32_t)size);
+    const int turn = nq == 1 ? 0 : (int)((uint32_t)item / (uint32_t)a.kv_heads), head = item - turn * a.kv_heads;
+    // Later query tiles see more: taken from both ends in turn, so that any
+    // stretch of them is about average.
+    const int qi = turn & 1 ? nq - 1 - turn / 2 : turn / 2;
     const Span s = span_of(a, len, n, qi);
-    const int chunk = (s.tiles + sp - 1) / sp;
-    const int t_begin = min(split * chunk, s.tiles), t_end = min(t_begin + chunk, s.tiles);
-    const int row0 = __ldg(a.row_start + r) + qi * a.qt;
+    int from, to, begin = 0;  // records of the item; where it begins in the row
+    if (whole) {
+      const int share = max((s.tiles + ATT_WARPS - 1) / ATT_WARPS, 1);
+      from = min(warp * share, s.tiles), to = min(from + share, s.tiles);
+      at = end;
+    } else {
+      begin = base + item * size + ATT_SETUP;
+      if (begin >= end) break;
+      from = max(at, begin) - begin, to = min(vt, end - begin);
+      at = begin + to;
+    }
+    const int t_begin = min(from, s.tiles), t_end = min(to, s.tiles);
+    row0 += qi * a.qt;
     const int ncol = min(a.qt, n - qi * a.qt) * a.group;
 
+    // ---- this warp's records
+    const int32_t *row_table = a.table + (int64_t)r * a.width;
+    const int recs_shift = a.shift - 4;
+    auto key_rec = [&](int tile) { return tile < s.sink ? tile : tile - s.sink + s.lo; };
+    // Records in which every row of the item sees every key: sinks 0 .. all_sink-1
+    // and all_lo .. all_hi-1.
+    const int shiftr = s.sink - s.lo;
+    const int all_hi = ((s.p0 + 1) >> 4) + shiftr;
+    const int all_lo = a.window ? max(s.sink, ((max(0, s.p1 - a.window + 1) + 15) >> 4) + shiftr) : 0;
+    const int all_sink = min(a.window ? a.sinks >> 4 : 0, min((s.p0 + 1) >> 4, s.sink));
+    // Lane i looks up record i of the next 32: its index in the pool, or NONE.
+    constexpr uint32_t NONE = 0xffffffffu;
+    auto look_up = [&](int tile) {
+      if (tile >= t_end) return NONE;
+      const int rec = key_rec(tile), p = rec >> recs_shift;
+      const int pg = p < a.width ? __ldg(row_table + p) : -1;
+      if (pg >= a.pages || pg < 0) {
+        if (a.status) atomicOr(a.status, CIS2B_KV4_BAD_PAGE);
+        return NONE;
+      }
+      return (((uint32_t)pg * a.kv_heads + head) << recs_shift) + (rec & ((1 << recs_shift) - 1));
+    };
+    uint32_t ids = look_up(t_begin + lane), ids_next = look_up(t_begin + 32 + lane);
+    int ahead = t_begin;  // next record to fetch
+    uint32_t held = 0;    // bit i: slot i of the ring holds a record of the pool
+    // 16-byte pieces move within their 128 bytes so that the operand loads
+    // below touch every bank once; the parameters' 8 pieces stay in place.
+    const uint32_t ring_base = (uint32_t)__cvta_generic_to_shared(ring), ring_at = ring_base + (lane ^ ((lane >> 3) & 3)) * 16;
+    auto fetch = [&](int slot) {
+      const int i = (ahead - t_begin) & 31;
+      if (i == 0 && ahead != t_begin) ids = ids_next, ids_next = look_up(ahead + 32 + lane);
+      const uint32_t id = __shfl_sync(0xffffffffu, ids, i);
+      const bool on = id != NONE;
+      held = (held & ~(1u << slot)) | (uint32_t)on << slot;
+      const uint8_t *src = a.pool + (uint64_t)(on ? id : 0u) * REC + lane * 16;
+      const uint32_t dst = ring_at + slot * REC;
+#pragma unroll
+      for (int k = 0; k < HD / 32; ++k) cp_async16(dst + k * 512, src + k * 512, on);
+      cp_async16(dst + HD * 16, src + HD * 16, on && lane < 8);
+      ++ahead;
+    };
     // ---- query operands: lane (g, t) holds elements t HD/4 .. of column g
     uint32_t bq[NT == 1 ? LIMBS : 1][NT == 1 ? KS : 1][2];
-    float sum_s[NT][2];  // sum(q) * scale * log2 e of this lane's two columns
+    float2 sum_s[NT];  // sum(q) * scale * log2 e of this lane's two columns
     int pos[NT][2];
     float code_scale;
     {
@@ -262,33 +424,32 @@ __global__ __launch_bounds__(ATT_THREADS) void k_kv4_attention(AttArgs a) {
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
         const int col = 8 * j + g, tok = col / a.group;
-        const int64_t row = row0 + tok;
+        const int64_t row = (int64_t)row0 + tok;
         float sum = 0.0f;
+        float e[8 * W];
+        const bool on = col < ncol && row >= 0 && row < a.rows;
+        const int64_t from_q = row * a.q_row + (int64_t)(head * a.group + col - tok * a.group) * a.q_head + t * (HD / 4);
+        load_query<LIMBS == 2, 8 * W>(a.q, a.dtype == KV4_BF16, from_q, a.q_wide, on, e);
+        if (j == 0) {  // the first records are asked for after the first queries, which would wait behind them
 #pragma unroll
-        for (int w = 0; w < W; ++w) {
-          float e[8];
-          if (col < ncol && row >= 0 && row < a.rows) {
-            const int64_t at = row * a.q_row + (int64_t)(head * a.group + col - tok * a.group) * a.q_head + t * (HD / 4) + w * 8;
-            if (a.dtype == KV4_F32) load8<KV4_F32>(a.q, at, a.q_wide, e);
-            else if (a.dtype == KV4_F16) load8<KV4_F16>(a.q, at, a.q_wide, e);
-            else load8<KV4_BF16>(a.q, at, a.q_wide, e);
-          } else {
+          for (int i = 0; i < ST - 1; ++i) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) e[i] = 0.0f;
+            for (int k = 0; k < RP; ++k) fetch(i * RP + k);
+            cp_async_commit();
           }
-#pragma unroll
-          for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(e[i])), sum += e[i];
-          // Word w's `and`s give the code pairs (0,4) (1,5) (2,6) (3,7).
-#pragma unroll
-          for (int i = 0; i < 4; ++i) x[j][4 * w + i][0] = e[i], x[j][4 * w + i][1] = e[i + 4];
         }
+#pragma unroll
+        for (int i = 0; i < 8 * W; ++i) top = fmaxf(top, fabsf(e[i])), sum += e[i];
+        // Word w's `and`s give the code pairs (0,4) (1,5) (2,6) (3,7).
+#pragma unroll
+        for (int i = 0; i < 4 * W; ++i) x[j][i][0] = e[(i & ~3) * 2 + (i & 3)], x[j][i][1] = e[(i & ~3) * 2 + (i & 3) + 4];
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
         sum *= sl;
+        sum_s[j] = make_float2(__shfl_sync(0xffffffffu, sum, 8 * t), __shfl_sync(0xffffffffu, sum, 8 * t + 4));
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           const int cc = 8 * j + 2 * t + c;
-          sum_s[j][c] = __shfl_sync(0xffffffffu, sum, (2 * t + c) * 4);
           pos[j][c] = cc < ncol ? s.p0 + cc / a.group : -1;
         }
       }
@@ -320,16 +481,16 @@ __global__ __launch_bounds__(ATT_THREADS) void k_kv4_attention(AttArgs a) {
             if constexpr (NT == 1) {
               bq[l][2 * w][0] = v[l][0], bq[l][2 * w][1] = v[l][1];
               bq[l][2 * w + 1][0] = v[l][2], bq[l][2 * w + 1][1] = v[l][3];
-            } else if (warp == (j & (ATT_WARPS - 1))) {
+            } else {
               qfrag[((j * LIMBS + l) * W + w) * 32 + lane] = make_uint4(v[l][0], v[l][1], v[l][2], v[l][3]);
             }
           }
         }
     }
-    if constexpr (NT > 1) __syncthreads();
+    if constexpr (NT > 1) __syncwarp();
 
-    // ---- the unit's records, this warp's share
-    float o[NT][KS][4], ones[NT][4], M[NT][2], l[NT][2], z[NT][2];
+    float o[NT][KS][4], ones[NT][4];
+    float2 M[NT], l[NT], z[NT];
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
 #pragma unroll
@@ -338,79 +499,46 @@ __global__ __launch_bounds__(ATT_THREADS) void k_kv4_attention(AttArgs a) {
         for (int i = 0; i < 4; ++i) o[j][m][i] = 0.0f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) ones[j][i] = 0.0f;
-#pragma unroll
-      for (int c = 0; c < 2; ++c) M[j][c] = -1e30f, l[j][c] = z[j][c] = 0.0f;
-    }
-    const int32_t *row_table = a.table + (int64_t)r * a.width;
-    const int recs_shift = a.shift - 4;
-    auto key_rec = [&](int tile) { return tile < s.sink ? tile : tile - s.sink + s.lo; };
-    auto page_of = [&](int tile) {  // page of a record, -1 if there is none
-      if (tile >= t_end) return -1;
-      const int p = key_rec(tile) >> recs_shift;
-      const int pg = p < a.width ? __ldg(row_table + p) : -1;
-      if (pg >= a.pages || pg < 0) {
-        if (a.status && lane == 0) atomicOr(a.status, CIS2B_KV4_BAD_PAGE);
-        return -1;
-      }
-      return pg;
-    };
-    uint32_t held = 0;  // bit i: stage i holds a record of the pool
-    auto issue = [&](int tile, int page, int stage) {
-      held &= ~(1u << stage);
-      if (tile < t_end && page >= 0) {
-        held |= 1u << stage;
-        const uint8_t *src = a.pool + ((((int64_t)page * a.kv_heads + head) << recs_shift) +
-                                       (key_rec(tile) & ((1 << recs_shift) - 1))) * REC;
-        const uint32_t dst = (uint32_t)__cvta_generic_to_shared(ring + stage * REC);
-#pragma unroll
-        for (int i = 0; i < (REC / 16 + 31) / 32; ++i) {
-          const int c = lane + 32 * i;
-          if (c < REC / 16) {
-            // 16-byte pieces of value rows move within their 128 bytes so
-            // that the operand loads below touch every bank once.
-            const int cv = c - HD / 2;
-            const int to = cv >= 0 && cv < HD / 2 ? HD / 2 + (cv ^ (((cv >> 3) & 3) << 1)) : c;
-            cp_async16(dst + to * 16, src + c * 16);
-          }
-        }
-      }
-      cp_async_commit();
-    };
-    const int first = t_begin + warp;
-    int next_page = page_of(first);
-#pragma unroll
-    for (int i = 0; i < ST - 1; ++i) {
-      issue(first + i * ATT_WARPS, next_page, i);
-      next_page = page_of(first + (i + 1) * ATT_WARPS);
+      M[j] = make_float2(-1e30f, -1e30f), l[j] = z[j] = make_float2(0.0f, 0.0f);
     }
     int stage = 0;
-    for (int tile = first; tile < t_end; tile += ATT_WARPS) {
+    for (int tile = t_begin; tile < t_end; tile += RP) {
       {
         const int to = stage == 0 ? ST - 1 : stage - 1;
-        issue(tile + (ST - 1) * ATT_WARPS, next_page, to);
-        next_page = page_of(tile + ST * ATT_WARPS);
+#pragma unroll
+        for (int k = 0; k < RP; ++k) fetch(to * RP + k);
+        cp_async_commit();
       }
       cp_async_wait<ST - 1>();
       __syncwarp();
-      const uint8_t *rec = ring + stage * REC;
-      const int k0 = key_rec(tile) * 16;
+      const uint32_t here = held >> (stage * RP);
+      const bool unmasked = (here & ((1u << RP) - 1)) == (1u << RP) - 1 &&
+                         ((tile >= all_lo && tile + RP <= all_hi) || tile + RP <= all_sink);
 
-      // scores: keys g and g + 8 by columns 2t, 2t + 1
-      float sc[NT][4];
+      // scores: keys g and g + 8 of each record by columns 2t, 2t + 1
+      float sc[RP][NT][4];
 #pragma unroll
-      for (int j = 0; j < NT; ++j)
+      for (int k = 0; k < RP; ++k) {
+        const uint8_t *rec = ring + (stage * RP + k) * REC;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sc[j][i] = 0.0f;
-      {
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sc[k][j][i] = 0.0f;
         uint32_t ka[W], kb[W];
         if constexpr (HD == 128) {
-          const uint4 x = *reinterpret_cast<const uint4 *>(rec + g * 64 + t * 16);
-          const uint4 y = *reinterpret_cast<const uint4 *>(rec + (g + 8) * 64 + t * 16);
+          // piece 4 key + t, moved by its line (two keys) within the record
+          const int at = (((g & 1) * 4 + t) ^ (g >> 1)) * 16 + (g >> 1) * 128;
+          const uint4 x = *reinterpret_cast<const uint4 *>(rec + at);
+          const uint4 y = *reinterpret_cast<const uint4 *>(rec + at + 512);
           ka[0] = x.x, ka[1] = x.y, ka[2] = x.z, ka[3] = x.w;
           kb[0] = y.x, kb[1] = y.y, kb[2] = y.z, kb[3] = y.w;
         } else {
-          const uint2 x = *reinterpret_cast<const uint2 *>(rec + g * 32 + t * 8);
-          const uint2 y = *reinterpret_cast<const uint2 *>(rec + (g + 8) * 32 + t * 8);
+          // lines of four keys; keys 8 .. 15 are lines 2 and 3
+          const int c = 2 * g + (t >> 1), line = c >> 3;
+          const int at = ((c & 7) ^ line) * 16 + line * 128 + (t & 1) * 8;
+          const int au = ((c & 7) ^ (line + 2)) * 16 + (line + 2) * 128 + (t & 1) * 8;
+          const uint2 x = *reinterpret_cast<const uint2 *>(rec + at);
+          const uint2 y = *reinterpret_cast<const uint2 *>(rec + au);
           ka[0] = x.x, ka[1] = x.y, kb[0] = y.x, kb[1] = y.y;
         }
 #pragma unroll
@@ -423,285 +551,308 @@ __global__ __launch_bounds__(ATT_THREADS) void k_kv4_attention(AttArgs a) {
 #pragma unroll
             for (int lm = 0; lm < LIMBS; ++lm) {
               if constexpr (NT == 1) {
-                mma16816(sc[j], a0, a1, a2, a3, bq[lm][2 * w][0], bq[lm][2 * w][1]);
-                mma16816(sc[j], c0, c1, c2, c3, bq[lm][2 * w + 1][0], bq[lm][2 * w + 1][1]);
+                mma16816(sc[k][j], a0, a1, a2, a3, bq[lm][2 * w][0], bq[lm][2 * w][1]);
+                mma16816(sc[k][j], c0, c1, c2, c3, bq[lm][2 * w + 1][0], bq[lm][2 * w + 1][1]);
               } else {
                 const uint4 f = qfrag[((j * LIMBS + lm) * W + w) * 32 + lane];
-                mma16816(sc[j], a0, a1, a2, a3, f.x, f.y);
-                mma16816(sc[j], c0, c1, c2, c3, f.z, f.w);
+                mma16816(sc[k][j], a0, a1, a2, a3, f.x, f.y);
+                mma16816(sc[k][j], c0, c1, c2, c3, f.z, f.w);
               }
             }
         }
       }
       // parameters of keys g and g + 8; a value's base is taken at code 8
-      float ks[2], kz[2], vs[2], vz[2];
+      float ks[2 * RP], kz[2 * RP], vs[2 * RP], vz[2 * RP];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const uint2 p = *reinterpret_cast<const uint2 *>(rec + 16 * HD + (g + 8 * i) * 8);
+      for (int i = 0; i < 2 * RP; ++i) {
+        const uint8_t *rec = ring + (stage * RP + (i >> 1)) * REC;
+        const uint2 p = *reinterpret_cast<const uint2 *>(rec + 16 * HD + (g + 8 * (i & 1)) * 8);
         ks[i] = bf16_lo(p.x) * code_scale;
         kz[i] = EXACT ? fmaf(8.0f, bf16_lo(p.x), bf16_hi(p.x)) : bf16_hi(p.x);
         vs[i] = bf16_lo(p.y), vz[i] = fmaf(8.0f, vs[i], bf16_hi(p.y));
       }
-      // Every column sees every key of the record: no mask.
-      const bool whole = ((held >> stage) & 1) && k0 + 15 <= s.p0 &&
-                         (a.window == 0 || k0 > s.p1 - a.window || k0 + 15 < a.sinks);
-      uint32_t bw[NT][LIMBS][2];
+      uint32_t bw[RP][NT][LIMBS][2];
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
-        float tt[4], p[4], w[4], vse[4], vze[4];
+        constexpr int E = 2 * RP;  // pair i: key g + 8 (i & 1) of record i >> 1, columns 2t and 2t + 1
+        float2 tt[E], p[E], w[E], vse[E], vze[E];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          tt[i] = fmaf(sc[j][i], ks[i >> 1], kz[i >> 1] * sum_s[j][i & 1]);
-          vse[i] = vs[i >> 1], vze[i] = vz[i >> 1];
+        for (int i = 0; i < E; ++i) {
+          const float2 raw = make_float2(sc[i >> 1][j][2 * (i & 1)], sc[i >> 1][j][2 * (i & 1) + 1]);
+          tt[i] = fma2(raw, make_float2(ks[i], ks[i]), mul2(make_float2(kz[i], kz[i]), sum_s[j]));
+          vse[i] = make_float2(vs[i], vs[i]), vze[i] = make_float2(vz[i], vz[i]);
         }
-        if (!whole) {
+        if (!unmasked) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int key = k0 + g + 8 * (i >> 1), at = pos[j][i & 1];
-            const bool see = ((held >> stage) & 1) && key <= at &&
-                             (a.window == 0 || key > at - a.window || key < a.sinks);
-            if (!see) tt[i] = -INFINITY, vse[i] = vze[i] = 0.0f;  // whatever the cache holds there
+          for (int i = 0; i < E; ++i) {
+            const int key = key_rec(tile + (i >> 1)) * 16 + g + 8 * (i & 1);
+            const bool in = (here >> (i >> 1)) & 1;
+            auto sees = [&](int at) { return in && key <= at && (a.window == 0 || key > at - a.window || key < a.sinks); };
+            // Whatever the cache holds there.
+            if (!sees(pos[j][0])) tt[i].x = -INFINITY, vse[i].x = vze[i].x = 0.0f;
+            if (!sees(pos[j][1])) tt[i].y = -INFINITY, vse[i].y = vze[i].y = 0.0f;
           }
         }
-        float chk[2];
+        const float2 minus_m = make_float2(-M[j].x, -M[j].y);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) p[i] = ex2(tt[i] - M[j][i & 1]), w[i] = p[i] * vse[i];
+        for (int i = 0; i < E; ++i) {
+          const float2 u = add2(tt[i], minus_m);
+          p[i] = make_float2(ex2(u.x), ex2(u.y));
+          w[i] = mul2(p[i], vse[i]);
+        }
+        float2 chk = w[0], big = p[0];
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
-          chk[c] = fmaxf(fmaxf(w[c], w[c + 2]), fmaxf(p[c], p[c + 2]) * 0x1p-46f);
-        if (__any_sync(0xffffffffu, fmaxf(chk[0], chk[1]) > 0x1p14f)) {
+        for (int i = 1; i < E; ++i) {
+          chk.x = fmaxf(chk.x, w[i].x), chk.y = fmaxf(chk.y, w[i].y);
+          big.x = fmaxf(big.x, p[i].x), big.y = fmaxf(big.y, p[i].y);
+        }
+        chk.x = fmaxf(chk.x, big.x * 0x1p-46f), chk.y = fmaxf(chk.y, big.y * 0x1p-46f);
+        if (__any_sync(0xffffffffu, fmaxf(chk.x, chk.y) > 0x1p14f)) {
+          float2 tw = make_float2(-INFINITY, -INFINITY), ts = tw;
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            float ck = chk[c], tw = fmaxf(tt[c] + lg2(vse[c]), tt[c + 2] + lg2(vse[c + 2])), ts = fmaxf(tt[c], tt[c + 2]);
+          for (int i = 0; i < E; ++i) {
+            tw.x = fmaxf(tw.x, tt[i].x + lg2(vse[i].x)), tw.y = fmaxf(tw.y, tt[i].y + lg2(vse[i].y));
+            ts.x = fmaxf(ts.x, tt[i].x), ts.y = fmaxf(ts.y, tt[i].y);
+          }
+          auto raise = [&](float &m, float ck, float w_top, float t_top) {  // the factor for what was summed
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) {
               ck = fmaxf(ck, __shfl_xor_sync(0xffffffffu, ck, d));
-              tw = fmaxf(tw, __shfl_xor_sync(0xffffffffu, tw, d));
-              ts = fmaxf(ts, __shfl_xor_sync(0xffffffffu, ts, d));
+              w_top = fmaxf(w_top, __shfl_xor_sync(0xffffffffu, w_top, d));
+              t_top = fmaxf(t_top, __shfl_xor_sync(0xffffffffu, t_top, d));
             }
-            if (ck > 0x1p14f) {
-              const float m = fmaxf(tw - 8.0f, ts - 54.0f), f = ex2(M[j][c] - m);
-              M[j][c] = m;
-              l[j][c] *= f, z[j][c] *= f;
-              ones[j][c] *= f, ones[j][c + 2] *= f;
+            if (!(ck > 0x1p14f)) return 1.0f;
+            const float before = m;
+            m = fmaxf(w_top - 8.0f, t_top - 54.0f);
+            return ex2(before - m);
+          };
+          const float2 f = make_float2(raise(M[j].x, chk.x, tw.x, ts.x), raise(M[j].y, chk.y, tw.y, ts.y));
+          l[j] = mul2(l[j], f), z[j] = mul2(z[j], f);
+          ones[j][0] *= f.x, ones[j][1] *= f.y;
 #pragma unroll
-              for (int k = 0; k < KS; ++k) o[j][k][c] *= f, o[j][k][c + 2] *= f;
+          for (int k = 0; k < KS; ++k) o[j][k][0] *= f.x, o[j][k][1] *= f.y, o[j][k][2] *= f.x, o[j][k][3] *= f.y;
 #pragma unroll
-              for (int i = c; i < 4; i += 2) p[i] = ex2(tt[i] - m), w[i] = p[i] * vse[i];
-            }
+          for (int i = 0; i < E; ++i) {
+            p[i] = make_float2(ex2(tt[i].x - M[j].x), ex2(tt[i].y - M[j].y));
+            w[i] = mul2(p[i], vse[i]);
           }
         }
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          l[j][c] += p[c] + p[c + 2];
-          z[j][c] = fmaf(p[c], vze[c], fmaf(p[c + 2], vze[c + 2], z[j][c]));
-        }
+        for (int i = 0; i < E; ++i) l[j] = add2(l[j], p[i]), z[j] = fma2(p[i], vze[i], z[j]);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const uint32_t h = pack_half(w[2 * i], w[2 * i + 1]);
-          bw[j][0][i] = transpose8x8(h);
+        for (int i = 0; i < E; ++i) {
+          const uint32_t h = pack_half(w[i].x, w[i].y);
+          bw[i >> 1][j][0][i & 1] = transpose8x8(h);
           if constexpr (LIMBS == 2) {
             const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h));
-            bw[j][1][i] = transpose8x8(pack_half(w[2 * i] - f.x, w[2 * i + 1] - f.y));
+            bw[i >> 1][j][1][i & 1] = transpose8x8(pack_half(w[i].x - f.x, w[i].y - f.y));
           }
         }
       }
-      // values: lane (g, t) holds elements g HD/8 .. of keys 2t, 2t+1, 2t+8, 2t+9
-      {
-        uint32_t v[4][HD / 64];
-        const uint8_t *vb = rec + 8 * HD;
+      // values: lane (g, t) holds 16-bit units (four codes) of keys 2t, 2t + 1
+      // and of 2t + 8, 2t + 9; unit g of the W pieces of 32 elements
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int key = 2 * t + (i & 1) + 8 * (i >> 1), at = key * (HD / 2) + g * (HD / 16);
-          const int c = at >> 4, to = (c ^ (((c >> 3) & 3) << 1)) * 16 + (at & 15);
-          if constexpr (HD == 128) {
-            const uint2 x = *reinterpret_cast<const uint2 *>(vb + to);
-            v[i][0] = x.x, v[i][1] = x.y;
-          } else {
-            v[i][0] = *reinterpret_cast<const uint32_t *>(vb + to);
-          }
+      for (int k = 0; k < RP; ++k) {
+        const uint32_t vb = ring_base + (stage * RP + k) * REC + 8 * HD;
+        uint32_t v[2][W];  // [key half][piece]
+#pragma unroll
+        for (int h = 0; h < W / 2; ++h) {
+          // matrices: pieces 2h and 2h + 1 of keys 0-7, then of keys 8-15
+          const int key = (lane & 7) + 8 * (lane >> 4), piece = 2 * h + ((lane >> 3) & 1);
+          const int c = key * W + piece, line = c >> 3;
+          uint32_t r4[4];
+          ldmatrix4_trans(r4, vb + line * 128 + ((c & 7) ^ (line & 3)) * 16);
+          v[0][2 * h] = r4[0], v[0][2 * h + 1] = r4[1], v[1][2 * h] = r4[2], v[1][2 * h + 1] = r4[3];
         }
 #pragma unroll
-        for (int w = 0; w < HD / 64; ++w)
+        for (int w = 0; w < W; ++w) {
+          uint32_t x = v[0][w], y = v[1][w];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {  // low and high 16 bits: codes 0-3 and 4-7 of the word
-            uint32_t x = __byte_perm(v[0][w], v[1][w], h ? 0x7632 : 0x5410);
-            uint32_t y = __byte_perm(v[2][w], v[3][w], h ? 0x7632 : 0x5410);
+          for (int q = 0; q < 2; ++q) {
+            const int m = 2 * w + q;  // rows of elements 32 w + 4 g + 2 q and the next
+            const uint32_t a0 = codes_low<EXACT>(x), a1 = codes_high<EXACT>(x), a2 = codes_low<EXACT>(y), a3 = codes_high<EXACT>(y);
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              const int m = 4 * w + 2 * h + q;  // rows of elements 2m and 2m + 1 of this lane's HD/8
-              const uint32_t a0 = codes_low<EXACT>(x), a1 = codes_high<EXACT>(x), a2 = codes_low<EXACT>(y), a3 = codes_high<EXACT>(y);
+            for (int j = 0; j < NT; ++j)
 #pragma unroll
-              for (int j = 0; j < NT; ++j)
-#pragma unroll
-                for (int lm = 0; lm < LIMBS; ++lm) mma16816(o[j][m], a0, a1, a2, a3, bw[j][lm][0], bw[j][lm][1]);
-              x >>= 8, y >>= 8;
-            }
+              for (int lm = 0; lm < LIMBS; ++lm) mma16816(o[j][m], a0, a1, a2, a3, bw[k][j][lm][0], bw[k][j][lm][1]);
+            x >>= 8, y >>= 8;
           }
+        }
 #pragma unroll
         for (int j = 0; j < NT && !EXACT; ++j)
 #pragma unroll
           for (int lm = 0; lm < LIMBS; ++lm)
-            mma16816(ones[j], 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, bw[j][lm][0], bw[j][lm][1]);
+            mma16816(ones[j], 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, bw[k][j][lm][0], bw[k][j][lm][1]);
       }
       __syncwarp();
       stage = stage + 1 == ST ? 0 : stage + 1;
     }
     cp_async_wait<0>();
 
-    // ---- the warps meet: a common M per column, then sums (0 + 2) + (1 + 3)
+    // ---- the item's numerators and denominators, or this part's
+    constexpr int PART = COLS * (HD + 2);  // numerators [col][HD], then (M, denominator) [col]
+    const bool ends = !whole && to == vt, alone = ends && from == 0;
+    float *mine = nullptr;
+    if (!alone) {
+      // The last item's part takes this warp's ring where it fits, which it no
+      // longer needs; an item that ends here and is followed by others goes
+      // to the workspace.
+      if (ends) mine = a.part + ((int64_t)blockIdx.x * PARTS + warp) * PART;
+      else if (ON_SHARED) mine = reinterpret_cast<float *>(ring);
+      else mine = a.part + ((int64_t)blockIdx.x * PARTS + ATT_WARPS + 2 + warp) * PART;
+      if (lane == 0) {
+        const Cut cut = {qbase + item, row0, head, ncol, begin, vt};
+        if (ends) cut_end[warp] = cut, has_end[warp] = 1;
+        else cut_on[warp] = cut, on_kind[warp] = whole ? (warp == 0 ? 1 : 2) : (from == 0 ? 1 : 2);
+      }
+    }
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-#pragma unroll
-        for (int d = 4; d < 32; d <<= 1) {
-          l[j][c] += __shfl_xor_sync(0xffffffffu, l[j][c], d);
-          z[j][c] += __shfl_xor_sync(0xffffffffu, z[j][c], d);
-        }
-        if (g == 0) red[warp][0][8 * j + 2 * t + c] = M[j][c];
+      for (int d = 4; d < 32; d <<= 1) {
+        l[j].x += __shfl_xor_sync(0xffffffffu, l[j].x, d), l[j].y += __shfl_xor_sync(0xffffffffu, l[j].y, d);
+        z[j].x += __shfl_xor_sync(0xffffffffu, z[j].x, d), z[j].y += __shfl_xor_sync(0xffffffffu, z[j].y, d);
       }
-    __syncthreads();  // also: every warp is done with its ring
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const int col = 8 * j + 2 * t + c;
-        float m = red[0][0][col];
+        if (col >= ncol) continue;
+        const float den = c ? l[j].y : l[j].x, zs = c ? z[j].y : z[j].x;
+        const float add = EXACT ? zs : fmaf(-8.0f, ones[j][c], zs);
 #pragma unroll
-        for (int w = 1; w < ATT_WARPS; ++w) m = fmaxf(m, red[w][0][col]);
-        const float f = ex2(M[j][c] - m);
-        M[j][c] = m;
-        l[j][c] *= f, z[j][c] *= f;
-        const float base = EXACT ? z[j][c] : z[j][c] - 8.0f * f * ones[j][c];
-#pragma unroll
-        for (int k = 0; k < KS; ++k) {
-          // each warp's numerator, the base's part included
-          o[j][k][c] = fmaf(o[j][k][c], f * UNIT, base);
-          o[j][k][c + 2] = fmaf(o[j][k][c + 2], f * (UNIT / 16.0f), base);
+        for (int k = 0; k < KS; k += 2) {
+          const float4 x = make_float4(fmaf(o[j][k][c], UNIT, add), fmaf(o[j][k][c + 2], UNIT / 16.0f, add),
+                                       fmaf(o[j][k + 1][c], UNIT, add), fmaf(o[j][k + 1][c + 2], UNIT / 16.0f, add));
+          const int d = 16 * k + 4 * g;
+          if (alone) emit(a, row0, head, col, d, x, den);
+          else *reinterpret_cast<float4 *>(mine + col * HD + d) = x;
         }
-        if (g == 0) red[warp][1][col] = l[j][c];
+        if (!alone && g == 0) *reinterpret_cast<float2 *>(mine + COLS * HD + 2 * col) = make_float2(c ? M[j].y : M[j].x, den);
       }
-    float *sum = reinterpret_cast<float *>(smem);
-    auto put = [&](int place) {
-#pragma unroll
-      for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int k = 0; k < KS; ++k)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) sum[((place * NT + j) * KS + k) * 128 + i * 32 + lane] = o[j][k][i];
-    };
-    auto add = [&](int place) {
-#pragma unroll
-      for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int k = 0; k < KS; ++k)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) o[j][k][i] += sum[((place * NT + j) * KS + k) * 128 + i * 32 + lane];
-    };
-    if (warp >= 2) put(warp - 2);
-    __syncthreads();
-    if (warp < 2) add(warp);
-    __syncthreads();
-    if (warp == 1) put(0);
-    __syncthreads();
+    __syncwarp();
+  }
 
-    const bool alone = sp == 1;
-    float *part = a.part + unit * (int64_t)(COLS * (HD + 2));
-    if (warp == 0) {
-      add(0);
-#pragma unroll
-      for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const int col = 8 * j + 2 * t + c;
-          float den = red[0][1][col];
-#pragma unroll
-          for (int w = 1; w < ATT_WARPS; ++w) den += red[w][1][col];
-          if (col >= ncol) continue;
-          const float f = !alone ? 1.0f : den > 0.0f || den != den ? 1.0f / den : 0.0f;
-          const int tok = col / a.group;
-          const int64_t row = row0 + tok;
-#pragma unroll
-          for (int k = 0; k < KS; k += 4) {
-            float x[8];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x[2 * i] = o[j][k + i][c] * f, x[2 * i + 1] = o[j][k + i][c + 2] * f;
-            const int d = g * (HD / 8) + 2 * k;
-            if (alone) {
-              if (row >= 0 && row < a.rows)
-                store8(a.out, a.dtype,
-                       row * a.o_row + (int64_t)(head * a.group + col - tok * a.group) * a.o_head + d, a.o_wide, x);
-            } else {
-              float4 *to = reinterpret_cast<float4 *>(part + col * HD + d);
-              __stcg(to, make_float4(x[0], x[1], x[2], x[3]));
-              __stcg(to + 1, make_float4(x[4], x[5], x[6], x[7]));
-            }
-          }
-          if (!alone && g == 0) __stcg(reinterpret_cast<float2 *>(part + COLS * HD) + col, make_float2(M[j][c], den));
-        }
+  // ---- parts meet within the block.  A run is an item's parts in it: it
+  // begins with the part of warp w that goes on (or, in warp 0, that began
+  // before) and takes the following warps up to the one that the item ends in.
+  constexpr int PART = COLS * (HD + 2);
+  float *block_part = a.part + (int64_t)blockIdx.x * PARTS * PART;
+  if (tid < 2) edge_last[tid] = 0;
+  __syncthreads();
+  auto on_part = [&](int w) {
+    return ON_SHARED ? reinterpret_cast<float *>(smem + w * ST * RP * REC) : block_part + (ATT_WARPS + 2 + w) * PART;
+  };
+  if (tid <= ATT_WARPS) {
+    const int w = tid < ATT_WARPS ? tid : 0;
+    const bool before = tid == ATT_WARPS;
+    Run mine = {0, -1, -1};
+    if (before ? has_end[0] : false) {
+      mine = {0, 0, 0};
+    } else if (on_kind[w] == (before ? 2 : 1)) {
+      int x = w + 1;  // the warp after the last part that goes on
+      while (x < ATT_WARPS && on_kind[x] == 2) ++x;
+      const bool ended = x < ATT_WARPS && has_end[x];
+      mine = {x - w, ended ? x : -1, before ? 0 : ended || whole ? 2 : 1};
     }
-    // ---- splits meet: the last one to finish joins them, in their order
-    if (!alone) {
-      if (warp == 0) {
-        __threadfence();
-        __syncwarp();
-        if (lane == 0) {
-          uint32_t *cnt = a.counter + (int64_t)(qbase + qi) * a.kv_heads + head;
-          last = (int64_t)(qbase + qi) * a.kv_heads + head < a.counters && atomicAdd(cnt, 1u) == (uint32_t)sp - 1;
-          if (last) *cnt = 0;  // ready for the next call
+    run[tid] = mine;
+    if (mine.side == 0 || mine.side == 1) edge[mine.side] = mine.on ? cut_on[w] : cut_end[0], edge_last[mine.side] = 1;
+  }
+  __syncthreads();
+  for (int i = 0; i <= ATT_WARPS; ++i) {
+    const Run now = run[i];
+    if (now.side < 0) continue;
+    const int w = i < ATT_WARPS ? i : 0;
+    const Cut &cut = now.on ? cut_on[w] : cut_end[0];
+    for (int q = tid; q < cut.ncol * (HD / 4); q += ATT_THREADS) {
+      const int col = q / (HD / 4), d = (q % (HD / 4)) * 4;
+      const Joined y = join_parts(on_part(w), ON_SHARED ? ST * RP * REC / 4 : PART, now.on,
+                                  now.end >= 0 ? block_part + now.end * PART : nullptr, col * HD + d, COLS * HD + 2 * col);
+      if (now.side == 2) {
+        emit(a, cut.row0, cut.head, col, d, y.x, y.den);
+      } else {
+        float *p = block_part + (ATT_WARPS + now.side) * PART;
+        *reinterpret_cast<float4 *>(p + col * HD + d) = y.x;
+        if (d == 0) *reinterpret_cast<float2 *>(p + COLS * HD + 2 * col) = make_float2(y.m, y.den);
+      }
+    }
+  }
+  __syncthreads();
+
+  // ---- parts of several blocks: the last one to arrive joins them
+  if (edge_last[0] | edge_last[1]) {
+    auto blocks_of = [&](const Cut &cut, int &first) {  // that share an item
+      first = (int)((uint32_t)cut.begin / (uint32_t)each) / ATT_WARPS;
+      return (int)((uint32_t)(cut.begin + cut.size - 1) / (uint32_t)each) / ATT_WARPS - first + 1;
+    };
+    if (tid < 2 && edge_last[tid] && edge[tid].item < a.items) {
+      int first;
+      const int parts = blocks_of(edge[tid], first);
+      // One thread's fence covers the block's writes: the barrier orders them before it.
+      asm volatile("fence.acq_rel.gpu;" ::: "memory");
+      if (atomicAdd(a.counter + edge[tid].item, 1u) == (uint32_t)parts - 1) {
+        a.counter[edge[tid].item] = 0;  // ready for the next call
+        edge_last[tid] = 2;
+      }
+      asm volatile("fence.acq_rel.gpu;" ::: "memory");
+    }
+    __syncthreads();
+    for (int side = 0; side < 2; ++side) {
+      if (edge_last[side] != 2) continue;
+      const Cut cut = edge[side];
+      int first;
+      const int parts = blocks_of(cut, first);
+      // Part 0 stands second in its block, as one that goes on; the others stand first.
+      const float *p0 = a.part + ((int64_t)first * PARTS + ATT_WARPS) * PART;
+      // Threads left over by the columns take a stretch of the other parts each.
+      const int quads = cut.ncol * (HD / 4), teams = max(1, min(ATT_THREADS / quads, (parts + 2) / 4));
+      const int stretch = (parts - 1 + teams - 1) / teams;
+      float *team_part = reinterpret_cast<float *>(smem);  // [team][quad][6]: elements, then (M, denominator)
+      for (int i = tid; i < quads * teams; i += ATT_THREADS) {
+        const int quad = i % quads, team = i / quads, col = quad / (HD / 4), d = (quad % (HD / 4)) * 4;
+        const int k0 = 1 + team * stretch, n = max(0, min(stretch, parts - k0));
+        const Joined y = join_parts(p0 + (int64_t)k0 * PARTS * PART, PARTS * PART, n, team == 0 ? p0 + PART : nullptr,
+                                    col * HD + d, COLS * HD + 2 * col);
+        if (teams > 1) {
+          *reinterpret_cast<float4 *>(team_part + i * 8) = y.x;
+          *reinterpret_cast<float2 *>(team_part + i * 8 + 4) = make_float2(y.m, y.den);
+        } else {
+          emit(a, cut.row0, cut.head, col, d, y.x, y.den);
         }
       }
-      __syncthreads();
-      if (last) {
-        __threadfence();
-        const int64_t stride = (int64_t)a.kv_heads * (COLS * (HD + 2));
-        const float *p0 = part - split * stride;
-        float *fac = reinterpret_cast<float *>(smem);  // [splits][cols], then the denominators
-        for (int col = tid; col < ncol; col += ATT_THREADS) {
-          float m = -INFINITY, den = 0.0f;
-          for (int i = 0; i < sp; ++i)
-            m = fmaxf(m, __ldcg(reinterpret_cast<const float2 *>(p0 + i * stride + COLS * HD) + col).x);
-          for (int i = 0; i < sp; ++i) {
-            const float2 ml = __ldcg(reinterpret_cast<const float2 *>(p0 + i * stride + COLS * HD) + col);
-            const float f = ex2(ml.x - m);
-            fac[i * COLS + col] = f;
-            den = fmaf(f, ml.y, den);
-          }
-          red[0][0][col] = den > 0.0f || den != den ? 1.0f / den : 0.0f;
+      if (teams > 1) {  // then quads < ATT_THREADS
+        __syncthreads();
+        if (tid < quads) {
+          const Joined y = join_parts(team_part, quads * 8, teams, nullptr, tid * 8, tid * 8 + 4);
+          emit(a, cut.row0, cut.head, tid / (HD / 4), (tid % (HD / 4)) * 4, y.x, y.den);
         }
         __syncthreads();
-        for (int i = tid; i < ncol * (HD / 8); i += ATT_THREADS) {
-          const int col = i / (HD / 8), d = (i % (HD / 8)) * 8, tok = col / a.group;
-          float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-#pragma unroll 4
-          for (int k = 0; k < sp; ++k) {
-            const float4 *from = reinterpret_cast<const float4 *>(p0 + k * stride + col * HD + d);
-            const float4 u0 = __ldcg(from), u1 = __ldcg(from + 1);
-            const float f = fac[k * COLS + col];
-            x[0] = fmaf(f, u0.x, x[0]), x[1] = fmaf(f, u0.y, x[1]), x[2] = fmaf(f, u0.z, x[2]), x[3] = fmaf(f, u0.w, x[3]);
-            x[4] = fmaf(f, u1.x, x[4]), x[5] = fmaf(f, u1.y, x[5]), x[6] = fmaf(f, u1.z, x[6]), x[7] = fmaf(f, u1.w, x[7]);
-          }
-          const float f = red[0][0][col];
-#pragma unroll
-          for (int k = 0; k < 8; ++k) x[k] *= f;
-          const int64_t row = row0 + tok;
-          if (row >= 0 && row < a.rows)
-            store8(a.out, a.dtype, row * a.o_row + (int64_t)(head * a.group + col - tok * a.group) * a.o_head + d,
-                   a.o_wide, x);
-        }
       }
     }
-    __syncthreads();  // the ring and the shared sums are free again
+  }
+  if (!whole) break;
+  __syncthreads();  // the rings and the shared words are free again
+  }
+
+  // Rows past the last request are zero.
+  const int used = max(0, min(__ldg(a.row_start + a.requests), a.rows));
+  const int64_t chunks = (int64_t)a.kv_heads * a.group * (HD / 4);
+  for (int64_t i = (int64_t)blockIdx.x * ATT_THREADS + tid; i < (a.rows - used) * chunks; i += (int64_t)gridDim.x * ATT_THREADS) {
+    const int64_t row = used + i / chunks;
+    const int rest = (int)(i % chunks);
+    store4(a.out, a.dtype, row * a.o_row + rest / (HD / 4) * a.o_head + rest % (HD / 4) * 4, a.o_wide, make_float4(0, 0, 0, 0));
   }
 }
 
 struct Shape {
-  int nt, limbs, qt, cols;
-  uint64_t part_units, counters, bytes;
+  int nt, limbs, qt, cols, blocks;
+  uint64_t items, bytes;
 };
 
-// Query columns per unit: the fewest groups of 8 that hold one request's rows,
+uint64_t round128(uint64_t x) { return (x + 127) / 128 * 128; }
+
+// Query columns per item: the fewest groups of 8 that hold one request's rows,
 // up to 32.
 Shape shape_of(const cis2b_kv4_cache *c, const cis2b_kv4_attn *a) {
   Shape s;
@@ -711,19 +862,15 @@ Shape shape_of(const cis2b_kv4_cache *c, const cis2b_kv4_attn *a) {
   s.limbs = a->dtype == CIS2B_F32 ? 2 : 1;
   s.cols = 8 * s.nt;
   s.qt = s.cols / group;
-  const uint64_t tiles = (uint64_t)a->requests + (uint64_t)a->rows / s.qt;  // query tiles at most
-  s.counters = tiles * c->kv_heads;
-  const uint64_t unit = (uint64_t)s.cols * (c->head_dim + 2) * 4;
-  const uint64_t recs = ((uint64_t)a->width * c->page_size + 15) / 16;
-  const uint64_t splits = std::min<uint64_t>((recs + ATT_CHUNK - 1) / ATT_CHUNK, ATT_MAX_SPLITS);
-  s.part_units = splits < 2 ? 0 : std::min(s.counters * splits, ATT_PART_BYTES / unit);
-  s.bytes = (s.counters * 4 + 127) / 128 * 128 + s.part_units * unit;
+  s.blocks = s.nt == 1 ? 320 : 160;  // at most: two or one for each of 148 SMs, and some to spare
+  s.items = ((uint64_t)a->requests + (uint64_t)a->rows / s.qt) * c->kv_heads;  // at most
+  s.bytes = round128(s.items * 4) + (uint64_t)s.blocks * att_parts(c->head_dim, s.nt) * s.cols * (c->head_dim + 2) * 4;
   return s;
 }
 
 int check_attn(const cis2b_kv4_cache *c, const cis2b_kv4_attn *a) {
   if (!a) return kv4_fail(CIS2B_ERR_ARG, "attention: arguments are NULL");
-  if (a->reserved) return kv4_fail(CIS2B_ERR_ARG, "attention: reserved must be zero");
+  if (a->flags & ~CIS2B_KV4_WHOLE) return kv4_fail(CIS2B_ERR_ARG, "attention: unknown flags");
   if (a->dtype < CIS2B_F32 || a->dtype > CIS2B_BF16)
     return kv4_fail(CIS2B_ERR_ARG, "attention: dtype must be CIS2B_F32, CIS2B_F16 or CIS2B_BF16");
   if (a->heads < 1 || a->heads % c->kv_heads || a->heads / c->kv_heads > 32)
@@ -738,9 +885,9 @@ int check_attn(const cis2b_kv4_cache *c, const cis2b_kv4_attn *a) {
 }
 
 template <int HD, int NT, int LIMBS>
-int launch(const AttArgs &args, const cis2b_kv4_cache *c, uint64_t units, int sms, cudaStream_t stream) {
+int launch(const AttArgs &args, const cis2b_kv4_cache *c, uint64_t most, int sms, cudaStream_t stream) {
   static std::atomic<int> resident[64];  // blocks per SM, by device; also: the attribute is set
-  const int smem = att_smem_bytes<HD, NT, LIMBS>();
+  const int smem = att_smem_bytes(HD, NT, LIMBS);
   int n = resident[c->device].load(std::memory_order_relaxed);
   if (!n) {
     if (int rc = kv4_cuda(cudaFuncSetAttribute(k_kv4_attention<HD, NT, LIMBS>,
@@ -752,20 +899,22 @@ int launch(const AttArgs &args, const cis2b_kv4_cache *c, uint64_t units, int sm
     n = std::max(n, 1);
     resident[c->device].store(n, std::memory_order_relaxed);
   }
-  const int grid = (int)std::max<uint64_t>(1, std::min<uint64_t>(units, (uint64_t)sms * n));
-  k_kv4_attention<HD, NT, LIMBS><<<grid, ATT_THREADS, smem, stream>>>(args);
+  const int grid = (int)std::max<uint64_t>(1, std::min<uint64_t>(most, (uint64_t)sms * n));
+  AttArgs given = args;
+  given.per_warp = nextafterf(1.0f / (float)(grid * ATT_WARPS), 1.0f);
+  k_kv4_attention<HD, NT, LIMBS><<<grid, ATT_THREADS, smem, stream>>>(given);
   return kv4_cuda(cudaGetLastError());
 }
 
 template <int HD>
-int dispatch(const Shape &s, const AttArgs &args, const cis2b_kv4_cache *c, uint64_t units, int sms, cudaStream_t st) {
+int dispatch(const Shape &s, const AttArgs &args, const cis2b_kv4_cache *c, uint64_t most, int sms, cudaStream_t st) {
   switch (s.nt * 10 + s.limbs) {
-    case 11: return launch<HD, 1, 1>(args, c, units, sms, st);
-    case 12: return launch<HD, 1, 2>(args, c, units, sms, st);
-    case 21: return launch<HD, 2, 1>(args, c, units, sms, st);
-    case 22: return launch<HD, 2, 2>(args, c, units, sms, st);
-    case 41: return launch<HD, 4, 1>(args, c, units, sms, st);
-    default: return launch<HD, 4, 2>(args, c, units, sms, st);
+    case 11: return launch<HD, 1, 1>(args, c, std::min<uint64_t>(most, s.blocks), sms, st);
+    case 12: return launch<HD, 1, 2>(args, c, std::min<uint64_t>(most, s.blocks), sms, st);
+    case 21: return launch<HD, 2, 1>(args, c, std::min<uint64_t>(most, s.blocks), sms, st);
+    case 22: return launch<HD, 2, 2>(args, c, std::min<uint64_t>(most, s.blocks), sms, st);
+    case 41: return launch<HD, 4, 1>(args, c, std::min<uint64_t>(most, s.blocks), sms, st);
+    default: return launch<HD, 4, 2>(args, c, std::min<uint64_t>(most, s.blocks), sms, st);
   }
 }
 
@@ -795,7 +944,7 @@ extern "C" int cis2b_kv4_attention(const cis2b_kv4_cache *c, const cis2b_kv4_att
   if (int rc = kv4_cuda(cudaSetDevice(c->device))) return rc;
   if (!a->rows) return CIS2B_OK;
   const int64_t unit = a->dtype == CIS2B_F32 ? 4 : 8;
-  AttArgs k;
+  AttArgs k{};
   k.q = a->q, k.out = a->out;
   k.q_row = a->q_row_stride, k.q_head = a->q_head_stride, k.o_row = a->out_row_stride, k.o_head = a->out_head_stride;
   k.q_wide = !(reinterpret_cast<uintptr_t>(a->q) & 15) && !(k.q_row % unit | k.q_head % unit);
@@ -803,15 +952,18 @@ extern "C" int cis2b_kv4_attention(const cis2b_kv4_cache *c, const cis2b_kv4_att
   k.pool = static_cast<const uint8_t *>(c->pool), k.status = c->status;
   k.table = a->table, k.length = a->length, k.row_start = a->row_start;
   k.counter = static_cast<uint32_t *>(a->work);
-  k.part = reinterpret_cast<float *>(static_cast<uint8_t *>(a->work) + (s.counters * 4 + 127) / 128 * 128);
+  k.part = reinterpret_cast<float *>(static_cast<uint8_t *>(a->work) + round128(s.items * 4));
   k.dtype = a->dtype, k.requests = a->requests, k.rows = a->rows, k.width = a->width, k.kv_heads = c->kv_heads;
   k.group = a->heads / c->kv_heads, k.pages = c->pages, k.window = a->window, k.sinks = a->sinks;
   k.shift = __builtin_ctz(c->page_size);
   k.qt = s.qt;
-  k.part_units = (int)std::min<uint64_t>(s.part_units, INT_MAX), k.counters = (int)std::min<uint64_t>(s.counters, INT_MAX);
+  k.items = (int)std::min<uint64_t>(s.items, INT_MAX);
   k.scale = a->scale;
   const uint64_t recs = ((uint64_t)a->width * c->page_size + 15) / 16;
-  const uint64_t units = s.counters * std::min<uint64_t>((recs + ATT_CHUNK - 1) / ATT_CHUNK, ATT_MAX_SPLITS);
+  // The row of records is counted in 32 bits; a batch that could pass that has
+  // items enough to take them whole.
+  k.whole = (a->flags & CIS2B_KV4_WHOLE) || s.items * (recs + ATT_SETUP) > INT_MAX;
+  const uint64_t most = std::max(s.items, (s.items * ((recs + ATT_LEAST - 1) / ATT_LEAST) + ATT_WARPS - 1) / ATT_WARPS);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return c->head_dim == 64 ? dispatch<64>(s, k, c, units, sms, st) : dispatch<128>(s, k, c, units, sms, st);
+  return c->head_dim == 64 ? dispatch<64>(s, k, c, most, sms, st) : dispatch<128>(s, k, c, most, sms, st);
 }

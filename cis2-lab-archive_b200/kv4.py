@@ -43,7 +43,7 @@ class _Step(ctypes.Structure):
 
 class _Attn(ctypes.Structure):
     _fields_ = [("dtype", _I32), ("heads", _I32), ("requests", _I32), ("rows", _I32), ("width", _I32),
-                ("max_new", _I32), ("window", _I32), ("sinks", _I32), ("scale", ctypes.c_float), ("reserved", _I32),
+                ("max_new", _I32), ("window", _I32), ("sinks", _I32), ("scale", ctypes.c_float), ("flags", _I32),
                 ("q", _P), ("out", _P), ("q_row_stride", _I64), ("q_head_stride", _I64), ("out_row_stride", _I64),
                 ("out_head_stride", _I64), ("table", _P), ("length", _P), ("row_start", _P), ("work", _P),
                 ("work_bytes", _U64)]
@@ -233,21 +233,23 @@ class Cache:
         return k, v
 
     def attention(self, q, batch: Batch, scale: float | None = None, window: int = 0, sinks: int = 0,
-                  max_new: int | None = None, out=None):
+                  max_new: int | None = None, out=None, whole: bool = False):
         """Causal attention of the step's rows q [rows, heads, head_dim] over
         the cache; their own keys and values are appended before.  With
         window > 0 a row sees its last `window` keys and the first `sinks`.
         max_new is the most rows that one request has in this step (a bound
-        will do; it only chooses the kernel).  Returns out (made if None)."""
+        will do; it only chooses the kernel).  whole: a request's result does
+        not depend on the rest of the batch (slower over long requests).
+        Returns out (made if None)."""
         if q.requires_grad and torch.is_grad_enabled():
             raise ValueError("attention over the 4-bit cache has no gradient")
         if out is None:
             out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         key = (q.dtype, q.shape, q.stride(), out.dtype, out.shape, out.stride(), batch.table.shape, batch.page_size,
-               scale, window, sinks, max_new)
+               scale, window, sinks, max_new, whole)
         call = self._calls.get(key)
         if call is None:
-            call = self._prepare(q, out, batch, scale, window, sinks, max_new)
+            call = self._prepare(q, out, batch, scale, window, sinks, max_new, whole)
             if len(self._calls) >= 64:
                 self._calls.clear()
             self._calls[key] = call
@@ -265,7 +267,7 @@ class Cache:
             _check(_lib().cis2b_kv4_attention(self._ref, ref, stream))
         return out
 
-    def _prepare(self, q, out, batch, scale, window, sinks, max_new):
+    def _prepare(self, q, out, batch, scale, window, sinks, max_new, whole):
         if q.dim() != 3 or q.shape[2] != self.head_dim:
             raise ValueError(f"q must be [rows, heads, {self.head_dim}]")
         if q.dtype not in _DTYPES:
@@ -279,7 +281,7 @@ class Cache:
         rows, heads = q.shape[0], q.shape[1]
         a = _Attn(_DTYPES[q.dtype], heads, batch.table.shape[0], rows, batch.table.shape[1],
                   max(1, rows if max_new is None else max_new), window, sinks,
-                  self.head_dim ** -0.5 if scale is None else scale, 0, None, None, q.stride(0), q.stride(1),
+                  self.head_dim ** -0.5 if scale is None else scale, int(whole), None, None, q.stride(0), q.stride(1),
                   out.stride(0), out.stride(1), None, None, None, None, 0)
         need = _U64()
         _check(_lib().cis2b_kv4_workspace(self._ref, ctypes.byref(a), ctypes.byref(need)))

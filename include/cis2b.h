@@ -355,10 +355,17 @@ int cis2b_kv4_gather(const cis2b_kv4_cache *c, int32_t dtype, void *k, void *v, 
  *   max_new    the most rows of any one request, or a bound (chooses the
  *              kernel; a request with more is still computed)
  *   scale      factor of the scores (1 / sqrt(head_dim) in most models)
+ *   flags      0: the keys of all requests are shared out evenly over the
+ *              GPU, so the grouping of a row's sums goes by the whole batch;
+ *              CIS2B_KV4_WHOLE: a row's sums are grouped by its own request
+ *              alone, and a request's result does not depend on the others
+ *              (given the same max_new), at the cost of parallelism over long
+ *              requests
  *   work       cis2b_kv4_workspace() bytes, zeroed once before the first
  *              call; calls that may overlap on the GPU need one each
  * Softmax statistics and sums are held in fp32; fp32 rows keep 22 bits of
  * every product's operands, 16-bit rows at least 11. */
+#define CIS2B_KV4_WHOLE 1
 typedef struct {
   int32_t dtype;    /* CIS2B_F32, _F16 or _BF16: q and out */
   int32_t heads;    /* a multiple of kv_heads, at most 32 times as many */
@@ -369,7 +376,7 @@ typedef struct {
   int32_t window;   /* 0: none */
   int32_t sinks;    /* >= 0 */
   float scale;
-  int32_t reserved; /* must be zero */
+  int32_t flags;    /* CIS2B_KV4_WHOLE or 0 */
   const void *q;
   void *out;        /* [rows][heads][head_dim]; strides in elements, heads' elements contiguous */
   int64_t q_row_stride, q_head_stride, out_row_stride, out_head_stride;

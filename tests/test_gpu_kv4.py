@@ -330,6 +330,7 @@ def test_attention_matches_64_bits(torch, kv4, dtype, shape):
     # the same bits again, and with a bound on max_new in place of its value
     assert torch.equal(out, w.cache.attention(q, w.batch, window=window, sinks=sinks, max_new=max(new)))
     w.check(q, w.cache.attention(q, w.batch, window=window, sinks=sinks), window, sinks)
+    w.check(q, w.cache.attention(q, w.batch, window=window, sinks=sinks, whole=True), window, sinks)
 
 
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
@@ -421,11 +422,12 @@ def test_a_request_alone_gives_the_bits_it_gives_in_a_batch(torch, kv4):
     lengths, new = [3000, 17, 900, 64, 1999], [1, 1, 1, 1, 1]
     w = World(torch, kv4, lengths, new, 2, 128, 32, "bfloat16")
     q = w.queries(8, 128)
-    both = w.cache.attention(q, w.batch, max_new=1)
+    both = w.cache.attention(q, w.batch, max_new=1, whole=True)
+    w.check(q, both)
     for r in range(len(lengths)):
         one = kv4.Batch.of(w.table[r:r + 1].contiguous(), w.batch.length[r:r + 1].clone(),
                            torch.tensor([0, 1], dtype=torch.int32, device="cuda"), 32)
-        assert torch.equal(w.cache.attention(q[r:r + 1], one, max_new=1)[0], both[r])
+        assert torch.equal(w.cache.attention(q[r:r + 1], one, max_new=1, whole=True)[0], both[r])
 
 
 def test_offsets_past_32_bits(torch, kv4):

@@ -65,7 +65,7 @@ def test_bad_steps_are_refused(kv4, field, value):
 
 @pytest.mark.parametrize("field,value", [("dtype", 3), ("heads", 5), ("heads", 66), ("heads", 0), ("requests", 0), ("rows", -1),
                                          ("width", 0), ("width", 2 ** 28), ("max_new", 0), ("window", -1), ("sinks", -1),
-                                         ("scale", float("inf")), ("reserved", 1), ("q", None), ("out", None), ("table", None),
+                                         ("scale", float("inf")), ("flags", 2), ("q", None), ("out", None), ("table", None),
                                          ("length", None), ("row_start", None), ("work", None), ("work", 8), ("work_bytes", 4)])
 def test_bad_attention_calls_are_refused(kv4, field, value):
     c = kv4._Cache(0, 4, 16, 2, 64, 0, 256, None)
