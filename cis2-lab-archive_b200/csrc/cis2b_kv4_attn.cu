@@ -15,6 +15,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 namespace cis2b {
 namespace {
@@ -845,10 +846,16 @@ __global__ __launch_bounds__(ATT_THREADS, NT == 1 ? 2 : 1) void k_kv4_attention(
   }
 }
 
+#include "cis2b_kv4_prompt.cuh"
+
 struct Shape {
+  bool prompt;  // more than 32 query columns: k_kv4_prompt
   int nt, limbs, qt, cols, blocks;
   uint64_t items, bytes;
+  uint64_t slots;  // parts of k_kv4_prompt
 };
+
+constexpr int PR_BLOCKS = 320;  // of k_kv4_prompt at most: two for each of 148 SMs, and some to spare
 
 uint64_t round128(uint64_t x) { return (x + 127) / 128 * 128; }
 
@@ -860,6 +867,18 @@ Shape shape_of(const cis2b_kv4_cache *c, const cis2b_kv4_attn *a) {
   const int64_t cols = (int64_t)group * a->max_new;
   s.nt = cols <= 8 ? 1 : cols <= 16 ? 2 : 4;
   s.limbs = a->dtype == CIS2B_F32 ? 2 : 1;
+  s.prompt = cols > 32;
+  s.slots = 0;
+  if (s.prompt) {
+    s.cols = PR_ROWS;
+    s.qt = PR_ROWS / group;
+    s.blocks = PR_BLOCKS;
+    s.items = ((uint64_t)a->requests + (uint64_t)a->rows / s.qt) * c->kv_heads;  // at most
+    // Query tiles of more than 1.25 PR_LEAST key tiles may be cut.
+    if ((uint64_t)a->width * c->page_size > PR_KEYS * (PR_LEAST + PR_LEAST / 4)) s.slots = 2 * PR_BLOCKS;
+    s.bytes = round128(8 + 4 * 2 * PR_BLOCKS) + s.slots * PR_ROWS * (c->head_dim + 2) * 4;
+    return s;
+  }
   s.cols = 8 * s.nt;
   s.qt = s.cols / group;
   s.blocks = s.nt == 1 ? 320 : 160;  // at most: two or one for each of 148 SMs, and some to spare
@@ -918,6 +937,38 @@ int dispatch(const Shape &s, const AttArgs &args, const cis2b_kv4_cache *c, uint
   }
 }
 
+// What both kernels are given.
+void fill(AttArgs &k, const cis2b_kv4_cache *c, const cis2b_kv4_attn *a, const Shape &s) {
+  const int64_t unit = a->dtype == CIS2B_F32 ? 4 : 8;
+  k.q = a->q, k.out = a->out;
+  k.q_row = a->q_row_stride, k.q_head = a->q_head_stride, k.o_row = a->out_row_stride, k.o_head = a->out_head_stride;
+  k.q_wide = !(reinterpret_cast<uintptr_t>(a->q) & 15) && !(k.q_row % unit | k.q_head % unit);
+  k.o_wide = !(reinterpret_cast<uintptr_t>(a->out) & 15) && !(k.o_row % unit | k.o_head % unit);
+  k.pool = static_cast<const uint8_t *>(c->pool), k.status = c->status;
+  k.table = a->table, k.length = a->length, k.row_start = a->row_start;
+  k.dtype = a->dtype, k.requests = a->requests, k.rows = a->rows, k.width = a->width, k.kv_heads = c->kv_heads;
+  k.group = a->heads / c->kv_heads, k.pages = c->pages, k.window = a->window, k.sinks = a->sinks;
+  k.shift = __builtin_ctz(c->page_size);
+  k.qt = s.qt;
+  k.items = (int)std::min<uint64_t>(s.items, INT_MAX);
+  k.scale = a->scale;
+}
+
+template <int HD, int LIMBS>
+int launch_prompt(const PromptArgs &args, const cis2b_kv4_cache *c, uint64_t most, int sms, cudaStream_t stream) {
+  static std::atomic<bool> ready[64];  // by device: the attribute is set
+  const int smem = pr_smem_bytes(HD, LIMBS);
+  if (!ready[c->device].load(std::memory_order_relaxed)) {
+    if (int rc = kv4_cuda(cudaFuncSetAttribute(k_kv4_prompt<HD, LIMBS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)))
+      return rc;
+    ready[c->device].store(true, std::memory_order_relaxed);
+  }
+  const int per_sm = HD == 128 && LIMBS == 2 ? 1 : 2;  // as its launch bounds and shared memory allow
+  const int grid = (int)std::max<uint64_t>(1, std::min<uint64_t>(most, std::min(sms * per_sm, PR_BLOCKS)));
+  k_kv4_prompt<HD, LIMBS><<<grid, PR_THREADS, smem, stream>>>(args);
+  return kv4_cuda(cudaGetLastError());
+}
+
 }  // namespace
 }  // namespace cis2b
 
@@ -943,22 +994,25 @@ extern "C" int cis2b_kv4_attention(const cis2b_kv4_cache *c, const cis2b_kv4_att
   if (int rc = kv4_sm_count(c->device, &sms)) return rc;
   if (int rc = kv4_cuda(cudaSetDevice(c->device))) return rc;
   if (!a->rows) return CIS2B_OK;
-  const int64_t unit = a->dtype == CIS2B_F32 ? 4 : 8;
   AttArgs k{};
-  k.q = a->q, k.out = a->out;
-  k.q_row = a->q_row_stride, k.q_head = a->q_head_stride, k.o_row = a->out_row_stride, k.o_head = a->out_head_stride;
-  k.q_wide = !(reinterpret_cast<uintptr_t>(a->q) & 15) && !(k.q_row % unit | k.q_head % unit);
-  k.o_wide = !(reinterpret_cast<uintptr_t>(a->out) & 15) && !(k.o_row % unit | k.o_head % unit);
-  k.pool = static_cast<const uint8_t *>(c->pool), k.status = c->status;
-  k.table = a->table, k.length = a->length, k.row_start = a->row_start;
+  if (s.prompt) {
+    PromptArgs p{};
+    fill(k, c, a, s);
+    k.whole = (a->flags & CIS2B_KV4_WHOLE) || !s.slots;
+    p.a = k;
+    p.ticket = static_cast<uint32_t *>(a->work);
+    p.counter = p.ticket + 2;
+    p.part = reinterpret_cast<float *>(static_cast<uint8_t *>(a->work) + round128(8 + 4 * 2 * PR_BLOCKS));
+    const uint64_t tiles = ((uint64_t)a->width * c->page_size + PR_KEYS - 1) / PR_KEYS;
+    const uint64_t most = s.items * ((tiles + PR_LEAST - 1) / PR_LEAST);
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (c->head_dim == 64)
+      return s.limbs == 1 ? launch_prompt<64, 1>(p, c, most, sms, st) : launch_prompt<64, 2>(p, c, most, sms, st);
+    return s.limbs == 1 ? launch_prompt<128, 1>(p, c, most, sms, st) : launch_prompt<128, 2>(p, c, most, sms, st);
+  }
   k.counter = static_cast<uint32_t *>(a->work);
   k.part = reinterpret_cast<float *>(static_cast<uint8_t *>(a->work) + round128(s.items * 4));
-  k.dtype = a->dtype, k.requests = a->requests, k.rows = a->rows, k.width = a->width, k.kv_heads = c->kv_heads;
-  k.group = a->heads / c->kv_heads, k.pages = c->pages, k.window = a->window, k.sinks = a->sinks;
-  k.shift = __builtin_ctz(c->page_size);
-  k.qt = s.qt;
-  k.items = (int)std::min<uint64_t>(s.items, INT_MAX);
-  k.scale = a->scale;
+  fill(k, c, a, s);
   const uint64_t recs = ((uint64_t)a->width * c->page_size + 15) / 16;
   // The row of records is counted in 32 bits; a batch that could pass that has
   // items enough to take them whole.

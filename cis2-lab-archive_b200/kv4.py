@@ -25,7 +25,7 @@ Cis2Error = _pkg.Cis2Error
 
 _I32, _I64, _U64, _P = ctypes.c_int32, ctypes.c_int64, ctypes.c_uint64, ctypes.c_void_p
 
-BAD_SLOT, BAD_PAGE = 1, 2  # CIS2B_KV4_BAD_*
+BAD_SLOT, BAD_PAGE, STUCK = 1, 2, 4  # CIS2B_KV4_*
 PLAN_FREE, PLAN_WIDTH, PLAN_ROWS, PLAN_NEGATIVE = 1, 2, 4, 8  # CIS2B_KV4_PLAN_*
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # CIS2B_F32, _F16, _BF16
 
@@ -191,7 +191,7 @@ class Cache:
         self._calls = {}  # by shape: filled-in arguments
 
     def errors(self) -> int:
-        """BAD_* bits that calls have left since the last time, 0 if all is well.  Waits for the GPU."""
+        """BAD_* and STUCK bits that calls have left since the last time, 0 if all is well.  Waits for the GPU."""
         bits = int(self.status.item())
         if bits:
             self.status.zero_()

@@ -292,10 +292,11 @@ typedef struct {
   int32_t head_dim;  /* 64 or 128 */
   int32_t reserved;  /* must be zero */
   void *pool;        /* cis2b_kv4_bytes() bytes, 16-byte aligned */
-  int32_t *status;   /* one word or NULL: bits OR-ed in by the kernels, CIS2B_KV4_BAD_* */
+  int32_t *status;   /* one word or NULL: bits OR-ed in by the kernels, below */
 } cis2b_kv4_cache;
 
 #define CIS2B_KV4_BAD_SLOT 1 /* a slot >= pages * page_size; the row was skipped */
+#define CIS2B_KV4_STUCK 4    /* a wait inside a kernel ran out; the call's results are not valid */
 #define CIS2B_KV4_BAD_PAGE 2 /* a visible key on a page that is not in the pool; it was not seen */
 
 /* Bytes of the pool: pages * kv_heads * page_size * (head_dim + 8). */
