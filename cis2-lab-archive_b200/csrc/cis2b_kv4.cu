@@ -188,9 +188,25 @@ struct RowArgs {
 
 constexpr int ROW_THREADS = 256;
 
+// Minimum and maximum that are NaN where an operand is.
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float d;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
 // One group's parameters and codes.  D / 8 lanes hold its elements, eight
-// each; lo and hi are already the group's.  `x != x` and the infinities leave
-// a step that is not finite, which poisons the group.
+// each; lo and hi are already the group's, NaN if an element is.  NaN and the
+// infinities leave a step that is not finite, which poisons the group.
+//   The quotient is at most 15 (1 + 2^-21), since the step is rounded up, and
+// at least 0, since the base is rounded down: no clamp.  Adding 1.5 * 2^23
+// rounds it to a whole number, ties to even, in the low bits of the sum, and
+// eight sums times powers of 16 make the word, less the constant's own part.
 __device__ __forceinline__ uint32_t kv4_quantise(const float (&x)[8], float lo, float hi, uint32_t &step16,
                                                  uint32_t &base16) {
   base16 = bf16_down(lo);
@@ -206,11 +222,9 @@ __device__ __forceinline__ uint32_t kv4_quantise(const float (&x)[8], float lo, 
   const float inv = step > 0.0f ? __frcp_rn(step) : 0.0f;
   uint32_t word = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float c = rintf(__fmul_rn(__fsub_rn(x[i], base), inv));
-    word |= (uint32_t)fminf(fmaxf(c, 0.0f), 15.0f) << (4 * i);
-  }
-  return word;
+  for (int i = 7; i >= 0; --i)
+    word = word * 16 + __float_as_uint(__fadd_rn(__fmul_rn(__fsub_rn(x[i], base), inv), 12582912.0f));
+  return word - 0x4b400000u * 0x11111111u;
 }
 
 // Rows to codes: D / 8 lanes take one (row, head), eight key and eight value
@@ -220,10 +234,10 @@ __device__ __forceinline__ uint32_t kv4_quantise(const float (&x)[8], float lo, 
 template <int HD, int DT>
 __global__ __launch_bounds__(ROW_THREADS) void k_kv4_append(RowArgs a, const void *k, const void *v, bool wide) {
   constexpr int LANES = HD / 8;
-  const int64_t item = ((int64_t)blockIdx.x * ROW_THREADS + threadIdx.x) / LANES;
+  const uint32_t item = (uint32_t)blockIdx.x * (ROW_THREADS / LANES) + threadIdx.x / LANES;
   const int part = threadIdx.x & (LANES - 1);
-  const int64_t row = item / a.kv_heads;
-  const int head = (int)(item - row * a.kv_heads);
+  const int64_t row = item / (uint32_t)a.kv_heads;
+  const int head = (int)(item - (uint32_t)row * a.kv_heads);
   int slot = -1;
   if (row < a.rows) slot = __ldg(a.slot + row);
   if (slot >= a.slots) {
@@ -239,20 +253,15 @@ __global__ __launch_bounds__(ROW_THREADS) void k_kv4_append(RowArgs a, const voi
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = y[i] = 0.0f;
   }
-  // fminf and fmaxf drop NaN, so NaN travels in a sum of its own.
-  float nx = 0.0f, ny = 0.0f;
   xl = xh = x[0], yl = yh = y[0];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    xl = fminf(xl, x[i]), xh = fmaxf(xh, x[i]), yl = fminf(yl, y[i]), yh = fmaxf(yh, y[i]);
-    nx += x[i] != x[i] ? 1.0f : 0.0f, ny += y[i] != y[i] ? 1.0f : 0.0f;
+  for (int i = 1; i < 8; ++i) {
+    xl = min_nan(xl, x[i]), xh = max_nan(xh, x[i]), yl = min_nan(yl, y[i]), yh = max_nan(yh, y[i]);
   }
-  if (nx > 0.0f) xh = __int_as_float(0x7f800000);
-  if (ny > 0.0f) yh = __int_as_float(0x7f800000);
 #pragma unroll
   for (int d = 1; d < LANES; d <<= 1) {
-    xl = fminf(xl, __shfl_xor_sync(0xffffffffu, xl, d)), xh = fmaxf(xh, __shfl_xor_sync(0xffffffffu, xh, d));
-    yl = fminf(yl, __shfl_xor_sync(0xffffffffu, yl, d)), yh = fmaxf(yh, __shfl_xor_sync(0xffffffffu, yh, d));
+    xl = min_nan(xl, __shfl_xor_sync(0xffffffffu, xl, d)), xh = max_nan(xh, __shfl_xor_sync(0xffffffffu, xh, d));
+    yl = min_nan(yl, __shfl_xor_sync(0xffffffffu, yl, d)), yh = max_nan(yh, __shfl_xor_sync(0xffffffffu, yh, d));
   }
   if (slot < 0) return;
   uint32_t ks, kb, vs, vb;
@@ -265,20 +274,22 @@ __global__ __launch_bounds__(ROW_THREADS) void k_kv4_append(RowArgs a, const voi
   if (part == 0) *reinterpret_cast<uint2 *>(rec + 16 * HD + r * 8) = make_uint2(ks | kb << 16, vs | vb << 16);
 }
 
+// base + step * code: the product is exact (12 bits), so one rounding.  A code
+// under the exponent of 2^23 is the number 2^23 + code.
 __device__ __forceinline__ void kv4_values(uint32_t word, uint32_t params, float (&x)[8]) {
   const float step = bf16_lo(params), base = bf16_hi(params);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = __fadd_rn(__fmul_rn(step, (float)((word >> (4 * i)) & 15)), base);
+  for (int i = 0; i < 8; ++i) x[i] = fmaf(step, __uint_as_float(((word >> (4 * i)) & 15) | 0x4b000000u) - 8388608.0f, base);
 }
 
 // Codes to rows, the same split.
 template <int HD>
 __global__ __launch_bounds__(ROW_THREADS) void k_kv4_gather(RowArgs a, void *k, void *v, int dt, bool wide) {
   constexpr int LANES = HD / 8;
-  const int64_t item = ((int64_t)blockIdx.x * ROW_THREADS + threadIdx.x) / LANES;
+  const uint32_t item = (uint32_t)blockIdx.x * (ROW_THREADS / LANES) + threadIdx.x / LANES;
   const int part = threadIdx.x & (LANES - 1);
-  const int64_t row = item / a.kv_heads;
-  const int head = (int)(item - row * a.kv_heads);
+  const int64_t row = item / (uint32_t)a.kv_heads;
+  const int head = (int)(item - (uint32_t)row * a.kv_heads);
   if (row >= a.rows) return;
   int slot = __ldg(a.slot + row);
   if (slot >= a.slots) {
@@ -299,7 +310,7 @@ __global__ __launch_bounds__(ROW_THREADS) void k_kv4_gather(RowArgs a, void *k, 
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = y[i] = 0.0f;
   }
-  const int64_t at = item * HD + part * 8;
+  const int64_t at = (int64_t)item * HD + part * 8;
   store8(k, dt, at, wide, x);
   store8(v, dt, at, wide, y);
 }
@@ -321,7 +332,8 @@ static int row_args(const cis2b_kv4_cache *c, int32_t dtype, const void *k, cons
   if (rows < 0) return kv4_fail(CIS2B_ERR_ARG, "rows must be >= 0");
   if (rows && (!k || !v || !slot)) return kv4_fail(CIS2B_ERR_ARG, "k, v and slot must be device pointers");
   const int64_t blocks = ((int64_t)rows * c->kv_heads * (c->head_dim / 8) + ROW_THREADS - 1) / ROW_THREADS;
-  if (blocks > INT_MAX) return kv4_fail(CIS2B_ERR_ARG, "rows * kv_heads is too large");
+  if ((int64_t)rows * c->kv_heads > INT_MAX || blocks > INT_MAX)
+    return kv4_fail(CIS2B_ERR_ARG, "rows * kv_heads must be < 2^31");
   *grid = (int)blocks;
   *a = RowArgs{static_cast<const uint8_t *>(c->pool), c->status, slot, rows, c->kv_heads, page_shift(c->page_size),
                c->pages * c->page_size, 0, 0, 0, 0};

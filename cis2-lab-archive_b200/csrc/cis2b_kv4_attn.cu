@@ -197,17 +197,17 @@ template <bool EXACT> __device__ __forceinline__ uint32_t codes_high(uint32_t x)
 // Records that a warp takes per iteration (one where 32 columns fill the
 // registers), iterations in its ring, and the shared memory of a block: its
 // warps' rings, then their query operands.
-__host__ __device__ constexpr int att_pair(int nt) { return nt < 4 ? 2 : 1; }
-__host__ __device__ constexpr int att_stages(int hd, int nt) { return nt < 4 ? (hd == 64 ? 4 : 3) : (hd == 64 ? 6 : 4); }
+__host__ __device__ constexpr int att_pair(int hd, int nt) { return nt < 4 && !(hd == 128 && nt == 1) ? 2 : 1; }
+__host__ __device__ constexpr int att_stages(int hd, int nt) { return hd == 128 && nt == 1 ? 6 : nt < 4 ? (hd == 64 ? 4 : 3) : (hd == 64 ? 6 : 4); }
 __host__ __device__ constexpr int att_ring_bytes(int hd, int nt) {
-  return ATT_WARPS * att_stages(hd, nt) * att_pair(nt) * kv4_rec_bytes(hd);
+  return ATT_WARPS * att_stages(hd, nt) * att_pair(hd, nt) * kv4_rec_bytes(hd);
 }
 __host__ __device__ constexpr int att_smem_bytes(int hd, int nt, int limbs) {
   return att_ring_bytes(hd, nt) + (nt > 1 ? ATT_WARPS * nt * limbs * (hd / 32) * 512 : 0);
 }
 
 __host__ __device__ constexpr bool att_on_shared(int hd, int nt) {
-  return 8 * nt * (hd + 2) * 4 <= att_stages(hd, nt) * att_pair(nt) * kv4_rec_bytes(hd);
+  return 8 * nt * (hd + 2) * 4 <= att_stages(hd, nt) * att_pair(hd, nt) * kv4_rec_bytes(hd);
 }
 __host__ __device__ constexpr int att_parts(int hd, int nt) { return ATT_WARPS + 2 + (att_on_shared(hd, nt) ? 0 : ATT_WARPS); }
 
@@ -248,7 +248,7 @@ __host__ __device__ constexpr int att_parts(int hd, int nt) { return ATT_WARPS +
 // weights (a product with ones) for 16-bit rows.
 template <int HD, int NT, int LIMBS>
 __global__ __launch_bounds__(ATT_THREADS, NT == 1 ? 2 : 1) void k_kv4_attention(AttArgs a) {
-  constexpr int REC = kv4_rec_bytes(HD), ST = att_stages(HD, NT), RP = att_pair(NT);
+  constexpr int REC = kv4_rec_bytes(HD), ST = att_stages(HD, NT), RP = att_pair(HD, NT);
   constexpr int KS = HD / 16;            // k-steps of the first product, row tiles of the second
   constexpr int W = HD / 32;             // 32-bit words of a key row per lane
   constexpr int COLS = 8 * NT;
@@ -954,18 +954,18 @@ void fill(AttArgs &k, const cis2b_kv4_cache *c, const cis2b_kv4_attn *a, const S
   k.scale = a->scale;
 }
 
-template <int HD, int LIMBS>
+template <int HD, int LIMBS, bool ROUNDED>
 int launch_prompt(const PromptArgs &args, const cis2b_kv4_cache *c, uint64_t most, int sms, cudaStream_t stream) {
   static std::atomic<bool> ready[64];  // by device: the attribute is set
   const int smem = pr_smem_bytes(HD, LIMBS);
   if (!ready[c->device].load(std::memory_order_relaxed)) {
-    if (int rc = kv4_cuda(cudaFuncSetAttribute(k_kv4_prompt<HD, LIMBS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)))
+    if (int rc = kv4_cuda(cudaFuncSetAttribute(k_kv4_prompt<HD, LIMBS, ROUNDED>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)))
       return rc;
     ready[c->device].store(true, std::memory_order_relaxed);
   }
   const int per_sm = HD == 128 && LIMBS == 2 ? 1 : 2;  // as its launch bounds and shared memory allow
   const int grid = (int)std::max<uint64_t>(1, std::min<uint64_t>(most, std::min(sms * per_sm, PR_BLOCKS)));
-  k_kv4_prompt<HD, LIMBS><<<grid, PR_THREADS, smem, stream>>>(args);
+  k_kv4_prompt<HD, LIMBS, ROUNDED><<<grid, PR_THREADS, smem, stream>>>(args);
   return kv4_cuda(cudaGetLastError());
 }
 
@@ -1006,9 +1006,11 @@ extern "C" int cis2b_kv4_attention(const cis2b_kv4_cache *c, const cis2b_kv4_att
     const uint64_t tiles = ((uint64_t)a->width * c->page_size + PR_KEYS - 1) / PR_KEYS;
     const uint64_t most = s.items * ((tiles + PR_LEAST - 1) / PR_LEAST);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (c->head_dim == 64)
-      return s.limbs == 1 ? launch_prompt<64, 1>(p, c, most, sms, st) : launch_prompt<64, 2>(p, c, most, sms, st);
-    return s.limbs == 1 ? launch_prompt<128, 1>(p, c, most, sms, st) : launch_prompt<128, 2>(p, c, most, sms, st);
+    if (a->dtype == CIS2B_BF16)
+      return c->head_dim == 64 ? launch_prompt<64, 1, true>(p, c, most, sms, st) : launch_prompt<128, 1, true>(p, c, most, sms, st);
+    if (a->dtype == CIS2B_F16)
+      return c->head_dim == 64 ? launch_prompt<64, 1, false>(p, c, most, sms, st) : launch_prompt<128, 1, false>(p, c, most, sms, st);
+    return c->head_dim == 64 ? launch_prompt<64, 2, false>(p, c, most, sms, st) : launch_prompt<128, 2, false>(p, c, most, sms, st);
   }
   k.counter = static_cast<uint32_t *>(a->work);
   k.part = reinterpret_cast<float *>(static_cast<uint8_t *>(a->work) + round128(s.items * 4));

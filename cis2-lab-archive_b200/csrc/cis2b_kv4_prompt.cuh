@@ -17,13 +17,21 @@
 // take 1,024 and the instructions of all warps about 1,100.
 //
 // M is an integer (a power of two scales exactly) and moves only when a weight
-// could pass 2^14 (by the row's top score and the tile's largest step) or p
+// could pass 2^14 (by the row's top score and the largest step of 32 keys) or p
 // 2^60; then the row's weights already written, its sums and its O are scaled.  LIMBS = 2 (fp32 rows): two
 // half-precision limbs of the query and of the weights, twice the products.
+//
+// Each key's four parameters cost the row warps two 16-byte broadcasts from
+// shared memory per pair of keys, 2,048 cycles a tile, more than anything else.
+// ROUNDED (bf16 rows) does without: the code warps store keys and values
+// themselves, base + step * c rounded once to half precision (11 bits, where
+// the rows and the result have 8), scaled by a power of two per 32 keys that the
+// row warps take into the exponent.  A key with a NaN (or of 2^119 or more) is
+// stored as zero and noted; rows that see it become NaN.
 #pragma once
 
 constexpr int PR_ROWS = 128, PR_KEYS = 128, PR_RECS = PR_KEYS / KV4_REC;
-constexpr int PR_THREADS = 256;      // warps 0-3 rows, 4-7 codes; warp 7 also issues the products
+constexpr int PR_THREADS = 256;      // warps 0-3 rows, 4-7 codes; warp 0 also issues the products
 constexpr int PR_MAX_SORT = 512;     // query tiles whose order is chosen (longest first)
 constexpr int PR_LEAST = 16;         // least key tiles of a part
 constexpr int PR_WAIT = 1 << 20;     // polls of a barrier before the kernel gives up
@@ -114,6 +122,17 @@ __device__ __forceinline__ void tc_st8(uint32_t at, const uint32_t (&r)[8]) {
                "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                : "memory");
 }
+// Two codes (bits 0-3, or 4-7, of each 16-bit half) as base + step * c.
+__device__ __forceinline__ uint32_t value_low(uint32_t x, __half2 step, __half2 base) {
+  const uint32_t y = x & 0x000f000fu;
+  const __half2 v = __hfma2(*reinterpret_cast<const __half2 *>(&y), step, base);
+  return *reinterpret_cast<const uint32_t *>(&v);
+}
+__device__ __forceinline__ uint32_t value_high(uint32_t x, __half2 step16, __half2 base) {
+  const uint32_t y = x & 0x00f000f0u;
+  const __half2 v = __hfma2(*reinterpret_cast<const __half2 *>(&y), step16, base);
+  return *reinterpret_cast<const uint32_t *>(&v);
+}
 // Shared-memory operand with rows of 128 bytes in the 128-byte swizzle (16-byte
 // piece p of row r at p ^ (r & 7)), groups of 8 rows 1,024 bytes apart.
 __device__ __forceinline__ uint64_t tc_desc(uint32_t at) {
@@ -132,14 +151,14 @@ __device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, ui
                "r"(a), "l"(b), "r"(idesc), "r"((int)add) : "memory");
 }
 
-template <int HD, int LIMBS>
+template <int HD, int LIMBS, bool ROUNDED>
 __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k_kv4_prompt(PromptArgs pa) {
   const AttArgs &a = pa.a;
   constexpr int REC = kv4_rec_bytes(HD);
   constexpr int KB = HD / 64;                  // 64-element column blocks of Q and K
   constexpr uint32_t QB = PR_ROWS * 128, VB = HD * 128;  // bytes of a block of Q or K; of V
   extern __shared__ uint8_t pr_smem[];
-  __shared__ __align__(8) uint64_t bars[5];
+  __shared__ __align__(8) uint64_t bars[6];
   __shared__ int scan_q[256], req_len[256], req_row[256], req_n[256], warp_sum[8];
   __shared__ uint16_t order[PR_MAX_SORT], tiles_of[PR_MAX_SORT];
   __shared__ int part0[PR_MAX_SORT + 1];       // parts before each query tile, in order
@@ -147,15 +166,20 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
   __shared__ uint32_t tmem_base;
   __shared__ int next_unit, dead, last;
   __shared__ uint32_t held[2][PR_RECS];        // records of each tile that the pool holds
-  __shared__ float value_part[2][4];           // log2 of each code warp's largest value step
+  __shared__ float value_part[2][4];           // log2 of the largest value step of each 32 keys
+  // ROUNDED: each chunk's factor of the scores and exponent of the values, and
+  // the keys with a NaN, by record.
+  __shared__ float2 chunk_scale[2][4];
+  __shared__ uint32_t bad[2][PR_RECS];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   uint8_t *base = pr_smem + ((1024 - (smem_of(pr_smem) & 1023)) & 1023);
   uint8_t *sq = base, *sk = sq + LIMBS * KB * QB, *sv = sk + KB * QB;
   float4 *sp = reinterpret_cast<float4 *>(sv + 2 * VB);  // [2][64 key pairs][2]: (ks, ks, kz, kz), (vs, vs, vz, vz)
   const uint32_t b_k = smem_of(&bars[0]), b_v = smem_of(&bars[1]), b_s = smem_of(&bars[2]), b_p = smem_of(&bars[3]),
-                 b_o = smem_of(&bars[4]);
+                 b_o = smem_of(&bars[4]), b_c = smem_of(&bars[5]);
   if (tid == 0) {
     bar_init(b_k, 128), bar_init(b_v, 128), bar_init(b_s, 1), bar_init(b_p, 128), bar_init(b_o, 1);
+    bar_init(b_c, 128);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     dead = 0;
   }
@@ -306,11 +330,11 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
         if (tid < nrow) pos = s.p0 + tok;
         float top = 0.0f;
 #pragma unroll 1
-        for (int d = 0; d < HD; d += 8) {
-          float e[8];
-          load_query<LIMBS == 2, 8>(a.q, a.dtype == KV4_BF16, from + d, a.q_wide, on, e);
+        for (int d = 0; d < HD; d += 32) {
+          float e[32];
+          load_query<LIMBS == 2, 32>(a.q, a.dtype == KV4_BF16, from + d, a.q_wide, on, e);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(e[i])), sum_s += e[i];
+          for (int i = 0; i < 32; ++i) top = fmaxf(top, fabsf(e[i])), sum_s += e[i];
         }
         sum_s *= sl;
 #pragma unroll
@@ -321,28 +345,35 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
       const float top = fmaxf(fmaxf(row_top[0], row_top[1]), fmaxf(row_top[2], row_top[3]));
       const int e2 = (int)(__float_as_uint(top) >> 23);
       const int up = e2 == 0 || e2 == 255 ? 0 : min(max(13 - (e2 - 127), -100), 100);
-      const float f = __uint_as_float((uint32_t)(127 + up) << 23);
+      float f = __uint_as_float((uint32_t)(127 + up) << 23);
       code_scale = sl * __uint_as_float((uint32_t)(127 - up) << 23);
+      if constexpr (ROUNDED) {  // a positive factor of the scores
+        if (!(code_scale > 0.0f)) f = code_scale < 0.0f ? -f : code_scale == 0.0f ? 0.0f : f;
+        code_scale = code_scale == 0.0f ? 1.0f : fabsf(code_scale);
+      }
       if (warp < 4) {
 #pragma unroll 1
-        for (int d = 0; d < HD; d += 8) {
-          float e[8];
-          load_query<LIMBS == 2, 8>(a.q, a.dtype == KV4_BF16, from + d, a.q_wide, on, e);
-          uint32_t v[LIMBS][4];
+        for (int d0 = 0; d0 < HD; d0 += 32) {
+          float e[32];
+          load_query<LIMBS == 2, 32>(a.q, a.dtype == KV4_BF16, from + d0, a.q_wide, on, e);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {  // elements i and i + 4, as a word's codes come out
-            const float k = (i & 1) ? f * 0.0625f : f;
-            const float y0 = e[i] * k, y1 = e[i + 4] * k;
-            v[0][i] = pack_half(y0, y1);
-            if constexpr (LIMBS == 2) {
-              const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&v[0][i]));
-              v[1][i] = pack_half(y0 - h.x, y1 - h.y);
+          for (int d = d0; d < d0 + 32; d += 8) {
+            uint32_t v[LIMBS][4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {  // elements i and i + 4, as a word's codes come out
+              const float k = (i & 1) && !ROUNDED ? f * 0.0625f : f;
+              const float y0 = e[d - d0 + i] * k, y1 = e[d - d0 + i + 4] * k;
+              v[0][i] = pack_half(y0, y1);
+              if constexpr (LIMBS == 2) {
+                const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&v[0][i]));
+                v[1][i] = pack_half(y0 - h.x, y1 - h.y);
+              }
             }
-          }
 #pragma unroll
-          for (int l = 0; l < LIMBS; ++l)
-            *reinterpret_cast<uint4 *>(sq + (l * KB + d / 64) * QB + tid * 128 + (((d / 8) & 7) ^ (tid & 7)) * 16) =
-                make_uint4(v[l][0], v[l][1], v[l][2], v[l][3]);
+            for (int l = 0; l < LIMBS; ++l)
+              *reinterpret_cast<uint4 *>(sq + (l * KB + d / 64) * QB + tid * 128 + (((d / 8) & 7) ^ (tid & 7)) * 16) =
+                  make_uint4(v[l][0], v[l][1], v[l][2], v[l][3]);
+          }
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       }
@@ -351,29 +382,35 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
 
     float M = -1e30f, l = 0.0f, z = 0.0f;
     if (warp >= 4) {
-      // ---- codes, and the products
+      // ---- codes
       const int pt = tid - 128, pw = warp - 4;
       const int32_t *row_table = a.table + (int64_t)t.r * a.width;
       const int shift = a.shift - 4;
       constexpr uint32_t NONE = 0xffffffffu;
-      auto look_up = [&](int j) {  // lanes 0-7: the pool's index of the tile's records
+      // Lanes 0-7: the page of a tile's records, which is asked for a tile
+      // before it is needed, and the records' index in the pool.
+      auto page_of = [&](int j) {
         const int rec = j * PR_RECS + lane;
-        if (lane >= PR_RECS || j >= j1 || rec >= s.tiles) return NONE;
-        const int k = key_rec(rec), p = k >> shift;
-        const int pg = p < a.width ? __ldg(row_table + p) : -1;
+        if (lane >= PR_RECS || j >= j1 || rec >= s.tiles) return -2;
+        const int p = key_rec(rec) >> shift;
+        return p < a.width ? __ldg(row_table + p) : -1;
+      };
+      auto index_of = [&](int j, int pg) {
+        if (pg == -2) return NONE;
         if (pg >= a.pages || pg < 0) {
           if (a.status) atomicOr(a.status, CIS2B_KV4_BAD_PAGE);
           return NONE;
         }
-        return (((uint32_t)pg * a.kv_heads + head) << shift) + (k & ((1 << shift) - 1));
+        return (((uint32_t)pg * a.kv_heads + head) << shift) + (key_rec(j * PR_RECS + lane) & ((1 << shift) - 1));
       };
       constexpr int KN = HD / 32;          // 16-byte pieces of keys per thread
       constexpr int VN = HD / 64;          // value tasks (8 keys x 8 elements) per thread
       uint4 kw[KN];
       uint32_t vw[VN][8];
       uint2 par;
-      uint32_t ids = look_up(j0), ids_next = look_up(j0 + 1);
-      auto load = [&]() {
+      uint32_t ids = index_of(j0, page_of(j0));
+      int page_next = page_of(j0 + 1);
+      auto load_keys = [&]() {
 #pragma unroll
         for (int i = 0; i < KN; ++i) {
           const int key = HD == 128 ? i * 32 + pw * 8 + (lane & 7) : i * 64 + pw * 16 + (lane >> 4) * 8 + (lane & 7);
@@ -383,6 +420,11 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
           if (id != NONE)
             kw[i] = __ldg(reinterpret_cast<const uint4 *>(a.pool + (int64_t)id * REC + (key & 15) * (HD / 2) + c * 16));
         }
+        const uint32_t id = __shfl_sync(0xffffffffu, ids, pt >> 4 & 7);
+        par = id == NONE ? make_uint2(0, 0)
+                         : __ldg(reinterpret_cast<const uint2 *>(a.pool + (int64_t)id * REC + 16 * HD + (pt & 15) * 8));
+      };
+      auto load_values = [&]() {
 #pragma unroll
         for (int i = 0; i < VN; ++i) {
           const int kg = HD == 128 ? i * 8 + pw * 2 + (lane >> 4) : pw * 4 + (lane >> 3), word = lane & (HD / 8 - 1);
@@ -392,12 +434,34 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
           for (int k = 0; k < 8; ++k)
             vw[i][k] = id == NONE ? 0u : __ldg(reinterpret_cast<const uint32_t *>(p + k * (HD / 2)));
         }
-        const uint32_t id = __shfl_sync(0xffffffffu, ids, pt >> 4 & 7);
-        par = id == NONE ? make_uint2(0, 0)
-                         : __ldg(reinterpret_cast<const uint2 *>(a.pool + (int64_t)id * REC + 16 * HD + (pt & 15) * 8));
+      };
+      // ROUNDED: the power of two of this warp's 32 keys (the row warps' chunk),
+      // and each key's constants as halves: step * 2^24 (a code in bits 0-3 is
+      // c 2^-24) and base of keys, of values.
+      __half *consts = reinterpret_cast<__half *>(sp);  // [2][4][128 keys]
+      auto prepare = [&](uint32_t now) {
+        const float ks = bf16_lo(par.x), kb = bf16_hi(par.x), vs = bf16_lo(par.y), vb = bf16_hi(par.y);
+        const float k_top = fmaxf(fabsf(kb), fabsf(fmaf(15.0f, ks, kb))), v_top = fmaxf(fabsf(vb), fabsf(fmaf(15.0f, vs, vb)));
+        const bool fine = ks + vs == ks + vs && k_top < 0x1p119f && v_top < 0x1p119f;
+        const uint32_t not_fine = __ballot_sync(0xffffffffu, !fine);
+        const uint32_t mk = __reduce_max_sync(0xffffffffu, fine ? __float_as_uint(k_top) : 0u);
+        const uint32_t mv = __reduce_max_sync(0xffffffffu, fine ? __float_as_uint(v_top) : 0u);
+        // The largest comes to 2^-7 .. 2^-6, so that step * 2^24 fits.
+        const int ek = mk ? max((int)(mk >> 23) - 120, -100) : 0, ev = mv ? max((int)(mv >> 23) - 120, -100) : 0;
+        const float fk = fine ? __uint_as_float((uint32_t)(127 - ek) << 23) : 0.0f;
+        const float fv = fine ? __uint_as_float((uint32_t)(127 - ev) << 23) : 0.0f;
+        __half *c = consts + (now & 1) * 512 + pt;
+        c[0] = __float2half_rn(fine ? ks * fk * 0x1p24f : 0.0f), c[128] = __float2half_rn(fine ? kb * fk : 0.0f);
+        c[256] = __float2half_rn(fine ? vs * fv * 0x1p24f : 0.0f), c[384] = __float2half_rn(fine ? vb * fv : 0.0f);
+        if (lane == 0) {
+          chunk_scale[now & 1][pw] = make_float2(code_scale * __uint_as_float((uint32_t)(127 + ek) << 23), (float)ev);
+          bad[now & 1][2 * pw] = not_fine & 0xffffu, bad[now & 1][2 * pw + 1] = not_fine >> 16;
+        }
+        bar_arrive(b_c);
       };
       auto store_keys = [&](uint32_t now) {
         if (pw == 0 && lane < PR_RECS) held[now & 1][lane] = ids != NONE;
+        if constexpr (!ROUNDED) {
         float *dst = reinterpret_cast<float *>(sp + (now & 1) * 128 + (pt >> 1) * 2) + (pt & 1);
         const float ks = bf16_lo(par.x), vs = bf16_lo(par.y);
         dst[0] = ks * code_scale, dst[2] = fmaf(8.0f, ks, bf16_hi(par.x));
@@ -405,26 +469,46 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
         // (a step that is not a number, or zero, bounds nothing)
         const uint32_t most = __reduce_max_sync(0xffffffffu, vs == vs ? __float_as_uint(vs) : 0u);
         if (lane == 0) value_part[now & 1][pw] = lg2(__uint_as_float(most));
+        }
 #pragma unroll
         for (int i = 0; i < KN; ++i) {
           const int key = HD == 128 ? i * 32 + pw * 8 + (lane & 7) : i * 64 + pw * 16 + (lane >> 4) * 8 + (lane & 7);
           const int c = HD == 128 ? lane >> 3 : (lane >> 3) & 1;
           const uint32_t w[4] = {kw[i].x, kw[i].y, kw[i].z, kw[i].w};
+          __half2 step, step16, at_zero;
+          if constexpr (ROUNDED) {
+            step = __half2half2(consts[(now & 1) * 512 + key]), at_zero = __half2half2(consts[(now & 1) * 512 + 128 + key]);
+            step16 = __hmul2(step, __half2half2(__ushort_as_half(0x2c00)));  // 1/16
+          }
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const uint32_t x = w[k], y = x >> 8;
             const int piece = (c & 1) * 4 + k;
             *reinterpret_cast<uint4 *>(sk + (c >> 1) * QB + key * 128 + (piece ^ (key & 7)) * 16) =
-                make_uint4(codes_low<true>(x), codes_high<true>(x), codes_low<true>(y), codes_high<true>(y));
+                ROUNDED ? make_uint4(value_low(x, step, at_zero), value_high(x, step16, at_zero), value_low(y, step, at_zero),
+                                     value_high(y, step16, at_zero))
+                        : make_uint4(codes_low<true>(x), codes_high<true>(x), codes_low<true>(y), codes_high<true>(y));
           }
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         bar_arrive(b_k);
       };
-      auto store_values = [&]() {
+      auto store_values = [&](uint32_t now) {
 #pragma unroll
         for (int i = 0; i < VN; ++i) {
           const int kg = HD == 128 ? i * 8 + pw * 2 + (lane >> 4) : pw * 4 + (lane >> 3), word = lane & (HD / 8 - 1);
+          uint4 steps, bases;
+          __half2 step[4], step16[4], at_zero[4];  // of keys 2 k and 2 k + 1
+          if constexpr (ROUNDED) {
+            steps = *reinterpret_cast<const uint4 *>(consts + (now & 1) * 512 + 256 + kg * 8);
+            bases = *reinterpret_cast<const uint4 *>(consts + (now & 1) * 512 + 384 + kg * 8);
+            const uint32_t st[4] = {steps.x, steps.y, steps.z, steps.w}, ba[4] = {bases.x, bases.y, bases.z, bases.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              step[k] = *reinterpret_cast<const __half2 *>(&st[k]), at_zero[k] = *reinterpret_cast<const __half2 *>(&ba[k]);
+              step16[k] = __hmul2(step[k], __half2half2(__ushort_as_half(0x2c00)));
+            }
+          }
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             uint32_t x[4];
@@ -436,7 +520,8 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
 #pragma unroll
               for (int k = 0; k < 4; ++k) {
                 const uint32_t u = e < 2 ? x[k] : x[k] >> 8;
-                y[k] = (e & 1) ? codes_high<true>(u) : codes_low<true>(u);
+                if constexpr (ROUNDED) y[k] = (e & 1) ? value_high(u, step16[k], at_zero[k]) : value_low(u, step[k], at_zero[k]);
+                else y[k] = (e & 1) ? codes_high<true>(u) : codes_low<true>(u);
               }
               const int n = (word >> 3) * 64 + (4 * h + e) * 8 + (word & 7);
               *reinterpret_cast<uint4 *>(sv + (kg >> 3) * VB + n * 128 + ((kg & 7) ^ (n & 7)) * 16) =
@@ -447,18 +532,42 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         bar_arrive(b_v);
       };
-      constexpr uint32_t S_DESC = tc_idesc(PR_ROWS, PR_KEYS), O_DESC = tc_idesc(PR_ROWS, HD);
-      const uint32_t aq = smem_of(sq), ak = smem_of(sk), av = smem_of(sv);
       if (j0 < j1) {
-        load();
-        store_keys(phase);
+        load_keys();
+        load_values();
+        if constexpr (ROUNDED) prepare(phase);
+        if (!ROUNDED || bar_wait(b_c, phase & 1, &dead)) store_keys(phase);
       }
       for (int j = j0; j < j1; ++j) {
         const uint32_t now = phase + (j - j0), parity = now & 1;
+        // The next tile's keys are asked for now, its values when these are stored.
+        if (j + 1 < j1) {
+          ids = index_of(j + 1, page_next);
+          page_next = page_of(j + 2);
+          load_keys();
+        }
         // The last tile's products are done: the values' place is free, and
-        // that of the weights, which the scores take.
+        // every warp has read the constants before last.
         if (j > j0 && !bar_wait(b_o, parity ^ 1, &dead)) break;
-        if (pw == 3) {
+        store_values(now);
+        if (j + 1 < j1) {
+          if constexpr (ROUNDED) prepare(now + 1);
+          load_values();
+          // The scores are done: the keys' place is free.
+          if (!bar_wait(b_s, parity, &dead) || (ROUNDED && !bar_wait(b_c, parity ^ 1, &dead))) break;
+          store_keys(now + 1);
+        }
+      }
+    } else {
+      // ---- weights: one row per thread
+      const uint32_t mine = tmem + ((uint32_t)warp << 21);  // lanes 32 warp ..
+      constexpr uint32_t S_DESC = tc_idesc(PR_ROWS, PR_KEYS), O_DESC = tc_idesc(PR_ROWS, HD);
+      const uint32_t aq = smem_of(sq), ak = smem_of(sk), av = smem_of(sv);
+      for (int j = j0; j < j1; ++j) {
+        const uint32_t now = phase + (j - j0), parity = now & 1;
+        if (warp == 0) {
+          // the scores take the place of the last tile's weights
+          if (j > j0 && !bar_wait(b_o, parity ^ 1, &dead)) break;
           if (!bar_wait(b_k, parity, &dead)) break;
           if (lane == 0) {
             tc_after();
@@ -466,40 +575,12 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
             for (int l2 = 0; l2 < LIMBS; ++l2)
 #pragma unroll
               for (int k = 0; k < HD / 16; ++k)
-                tc_mma_ss(tmem, tc_desc(aq + (l2 * KB + k / 4) * QB + (k & 3) * 32), tc_desc(ak + (k / 4) * QB + (k & 3) * 32),
-                          S_DESC, l2 || k);
+                tc_mma_ss(tmem, tc_desc(aq + ((LIMBS - 1 - l2) * KB + k / 4) * QB + (k & 3) * 32),
+                          tc_desc(ak + (k / 4) * QB + (k & 3) * 32), S_DESC, l2 || k);  // the small limb first
             tc_commit(b_s);
           }
           __syncwarp();
         }
-        store_values();
-        if (j + 1 < j1) {
-          ids = ids_next, ids_next = look_up(j + 2);
-          load();
-          // The scores are done: the keys' place is free.
-          if (!bar_wait(b_s, parity, &dead)) break;
-          store_keys(now + 1);
-        }
-        if (pw == 3) {
-          if (!bar_wait(b_v, parity, &dead) || !bar_wait(b_p, parity, &dead)) break;
-          if (lane == 0) {
-            tc_after();
-#pragma unroll
-            for (int k = 0; k < PR_KEYS / 16; ++k)
-#pragma unroll
-              for (int l2 = 0; l2 < LIMBS; ++l2)
-                tc_mma_ts(tmem + 128, tmem + k * 16 + l2 * 8, tc_desc(av + (k / 4) * VB + (k & 3) * 32),
-                          O_DESC, j > j0 || k || l2);
-            tc_commit(b_o);
-          }
-          __syncwarp();
-        }
-      }
-    } else {
-      // ---- weights: one row per thread
-      const uint32_t mine = tmem + ((uint32_t)warp << 21);  // lanes 32 warp ..
-      for (int j = j0; j < j1; ++j) {
-        const uint32_t now = phase + (j - j0), parity = now & 1;
         // the parameters come from the code warps, the scores from the products
         if (!bar_wait(b_k, parity, &dead) || !bar_wait(b_s, parity, &dead)) break;
         tc_after();
@@ -510,22 +591,27 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
           const int lo = key_rec(rec0) * 16, hi = key_rec(rec0 + PR_RECS - 1) * 16 + 15;
           unmasked = hi <= s.p0 && (a.window == 0 || lo > s.p1 - a.window || hi < a.sinks);
 #pragma unroll
-          for (int k = 0; k < PR_RECS; ++k) unmasked = unmasked && held[parity][k];
+          for (int k = 0; k < PR_RECS; ++k) unmasked = unmasked && held[parity][k] && !(ROUNDED && bad[parity][k]);
         }
         const float4 *params = sp + parity * 128;
-        // log2 of the tile's largest value step
-        const float lv_top = fmaxf(fmaxf(value_part[parity][0], value_part[parity][1]),
-                                   fmaxf(value_part[parity][2], value_part[parity][3]));
         // A chunk is two records: 32 scores in; 8 words of weights (and 8 of
         // the second limb) per record out, over the record's scores.
 #pragma unroll 1
         for (int c = 0; c < PR_RECS / 2; ++c) {
+          // log2 of the chunk's largest value step (ROUNDED: the exponent of
+          // its values; its scores are `factor` times S)
+          const float lv_top = ROUNDED ? chunk_scale[parity][c].y : value_part[parity][c];
+          const float factor = ROUNDED ? chunk_scale[parity][c].x : 1.0f;
           uint32_t raw[32];
           tc_ld32(raw, mine + c * 32);
           tc_wait_ld32(raw);
           float2 u[16];  // scores in units of log2
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
+            if constexpr (ROUNDED) {
+              u[i] = make_float2(__uint_as_float(raw[2 * i]), __uint_as_float(raw[2 * i + 1]));
+              continue;
+            }
             const float4 kp = params[(c * 16 + i) * 2];
             u[i] = fma2(make_float2(__uint_as_float(raw[2 * i]), __uint_as_float(raw[2 * i + 1])), make_float2(kp.x, kp.y),
                         mul2(make_float2(kp.z, kp.w), make_float2(sum_s, sum_s)));
@@ -545,6 +631,7 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
                 const uint32_t sink = sink_i <= 0 ? 0u : sink_i > 15 ? 0xffffu : (1u << sink_i) - 1;
                 bits &= late | sink;
               }
+              if (ROUNDED && (bits & bad[parity][c * 2 + h])) l = __int_as_float(0x7fffffff);
               see |= bits << (16 * h);
             }
 #pragma unroll
@@ -556,6 +643,7 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
           float top = -INFINITY;
 #pragma unroll
           for (int i = 0; i < 16; i += 2) top = fmaxf(top, fmaxf(fmaxf(u[i].x, u[i].y), fmaxf(u[i + 1].x, u[i + 1].y)));
+          top *= factor;
           // Weights stay below 2^14, p below 2^60; if not, M rises to 2^8 below the top.
           const bool raise = top - M > fminf(14.0f - lv_top, 60.0f);
           if (__any_sync(0xffffffffu, raise)) {
@@ -595,13 +683,20 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
             tc_wait_st();
           }
           float2 l2 = make_float2(0.0f, 0.0f), z2 = l2;
-          const float2 minus = make_float2(-M, -M);
+          const float2 minus = make_float2(ROUNDED ? lv_top - M : -M, ROUNDED ? lv_top - M : -M);
           auto weigh = [&](auto masked) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              uint32_t hi[8], lo[8];
+              uint32_t hi[8];
+              [[maybe_unused]] uint32_t lo[8];
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
+                if constexpr (ROUNDED) {
+                  const float2 e = fma2(u[8 * h + i], make_float2(factor, factor), minus), w = make_float2(ex2(e.x), ex2(e.y));
+                  l2 = add2(l2, w);
+                  hi[i] = pack_half(w.x, w.y);
+                  continue;
+                }
                 const float2 e = add2(u[8 * h + i], minus), p = make_float2(ex2(e.x), ex2(e.y));
                 const float4 vp = params[(c * 16 + 8 * h + i) * 2 + 1];
                 float2 vs = make_float2(vp.x, vp.y), vz = make_float2(vp.z, vp.w);
@@ -621,12 +716,27 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
               if constexpr (LIMBS == 2) tc_st8(mine + c * 32 + h * 16 + 8, lo);
             }
           };
-          if (unmasked) weigh(std::false_type()); else weigh(std::true_type());
-          l += l2.x + l2.y, z += z2.x + z2.y;
+          if (ROUNDED || unmasked) weigh(std::false_type()); else weigh(std::true_type());
+          if constexpr (ROUNDED) l += (l2.x + l2.y) * ex2(-lv_top);
+          else l += l2.x + l2.y, z += z2.x + z2.y;
         }
         tc_wait_st();
         tc_before();
         bar_arrive(b_p);
+        if (warp == 0) {
+          if (!bar_wait(b_v, parity, &dead) || !bar_wait(b_p, parity, &dead)) break;
+          if (lane == 0) {
+            tc_after();
+#pragma unroll
+            for (int k = 0; k < PR_KEYS / 16; ++k)
+#pragma unroll
+              for (int l2 = 0; l2 < LIMBS; ++l2)
+                tc_mma_ts(tmem + 128, tmem + k * 16 + l2 * 8, tc_desc(av + (k / 4) * VB + (k & 3) * 32),
+                          O_DESC, j > j0 || k || l2);
+            tc_commit(b_o);
+          }
+          __syncwarp();
+        }
       }
     }
 
@@ -659,7 +769,7 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const float v = __uint_as_float(i < 4 ? x0[i * 8 + word] : x1[(i - 4) * 8 + word]);
-            y[i] = (i & 1) ? fmaf(v, 0.0625f, z) : v + z;
+            y[i] = ROUNDED ? v : (i & 1) ? fmaf(v, 0.0625f, z) : v + z;
           }
           const int d = 8 * (8 * b + word);
           if (parts > 1) {

@@ -72,6 +72,19 @@ def _check(rc: int) -> None:
 
 
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
+
+
+def _call(device: int, fn, *args) -> None:
+    """fn(*args, torch's current stream), leaving the current device as it
+    was: the C entry points make theirs current."""
+    if _current_device() == device:
+        rc = fn(*args, _raw_stream(device))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, _raw_stream(device))
+    if rc:
+        _pkg._check(rc)
 
 
 def _device_index(device) -> int:
@@ -79,22 +92,6 @@ def _device_index(device) -> int:
     if d.type != "cuda":
         raise ValueError(f"device must be a CUDA device, not {d}")
     return torch.cuda.current_device() if d.index is None else d.index
-
-
-class _On:
-    """Leaves torch's current device as it was: the C entry points make theirs current."""
-
-    __slots__ = ("device", "before")
-
-    def __init__(self, device: int):
-        self.device = device
-
-    def __enter__(self):
-        self.before = torch.cuda.current_device()
-
-    def __exit__(self, *exc):
-        if self.before != self.device:
-            torch.cuda.set_device(self.before)
 
 
 def _ints(t, name: str, device: int, shape: tuple | None = None):
@@ -158,8 +155,7 @@ class Batch:
         _ints(cached, "cached", dev, (n,)), _ints(new, "new", dev, (n,)), _ints(free_pages, "free_pages", dev)
         s.cached, s.new_tokens = cached.data_ptr(), new.data_ptr()
         s.free_pages, s.free_count = free_pages.data_ptr(), free_pages.numel()
-        with _On(dev):
-            _check(_lib().cis2b_kv4_plan(self._ref, _raw_stream(dev)))
+        _call(dev, _lib().cis2b_kv4_plan, self._ref)
 
     def errors(self) -> int:
         """PLAN_* bits of the last plan, 0 if all is well.  Waits for the GPU."""
@@ -215,9 +211,8 @@ class Cache:
         if v.shape[0] != n or v.dtype is not k.dtype:
             raise ValueError("k and v must have the same rows and type")
         _ints(slot, "slot", self.device, (n,))
-        with _On(self.device):
-            _check(_lib().cis2b_kv4_append(self._ref, _DTYPES[k.dtype], k.data_ptr(), v.data_ptr(), ks[0], ks[1],
-                                           vs[0], vs[1], slot.data_ptr(), n, _raw_stream(self.device)))
+        _call(self.device, _lib().cis2b_kv4_append, self._ref, _DTYPES[k.dtype], k.data_ptr(), v.data_ptr(), ks[0], ks[1],
+              vs[0], vs[1], slot.data_ptr(), n)
 
     def gather(self, slot, dtype=torch.float32):
         """The keys and values of the slots as the values that their codes
@@ -227,9 +222,7 @@ class Cache:
             raise ValueError("dtype must be float32, float16 or bfloat16 and slot [rows]")
         n = slot.shape[0]
         k, v = torch.empty((2, n, self.kv_heads, self.head_dim), dtype=dtype, device=slot.device).unbind(0)
-        with _On(self.device):
-            _check(_lib().cis2b_kv4_gather(self._ref, _DTYPES[dtype], k.data_ptr(), v.data_ptr(), slot.data_ptr(), n,
-                                           _raw_stream(self.device)))
+        _call(self.device, _lib().cis2b_kv4_gather, self._ref, _DTYPES[dtype], k.data_ptr(), v.data_ptr(), slot.data_ptr(), n)
         return k, v
 
     def attention(self, q, batch: Batch, scale: float | None = None, window: int = 0, sinks: int = 0,
@@ -263,8 +256,7 @@ class Cache:
             work = self._work[stream] = torch.zeros(need, dtype=torch.uint8, device=q.device)
         a.q, a.out, a.work, a.work_bytes = q.data_ptr(), out.data_ptr(), work.data_ptr(), work.numel()
         a.table, a.length, a.row_start = batch.table.data_ptr(), batch.length.data_ptr(), batch.row_start.data_ptr()
-        with _On(dev):
-            _check(_lib().cis2b_kv4_attention(self._ref, ref, stream))
+        _call(dev, _lib().cis2b_kv4_attention, self._ref, ref)
         return out
 
     def _prepare(self, q, out, batch, scale, window, sinks, max_new, whole):
