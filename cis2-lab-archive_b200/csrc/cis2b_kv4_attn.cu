@@ -177,21 +177,31 @@ __device__ __forceinline__ Joined join_parts(const float *p, int64_t stride, int
   return s;
 }
 
-// Codes of a 16-bit half each, as half-precision operands.  EXACT: the normal
-// numbers c - 8 (low: bits 0-3) and 16 (c - 8) (high: bits 4-7), one more
-// instruction each; else the bits themselves, the subnormals c 2^-24 and
-// c 2^-20.
-template <bool EXACT> __device__ __forceinline__ uint32_t codes_low(uint32_t x) {
-  if constexpr (!EXACT) return x & 0x000f000fu;
-  const uint32_t y = (x & 0x000f000fu) | 0x64006400u;  // 1024 + c
-  const __half2 h = __hsub2(*reinterpret_cast<const __half2 *>(&y), __half2half2(__ushort_as_half(0x6408)));
+// The codes in bits 4-7 (high) or 0-3 (low) of each 16-bit half as the normal
+// half-precision numbers 16 (c - 7.5).  Centred at 7.5, sums over many values
+// have no drift that the bases' sums would have to cancel.  The low codes'
+// second operation is on the multiply-add pipe, which has room; a shift into
+// the high ones' place would be on the other, which has not.
+__device__ __forceinline__ uint32_t codes_high(uint32_t x) {
+  const uint32_t y = (x & 0x00f000f0u) | 0x64006400u;  // 1024 + 16 c
+  const __half2 h = __hsub2(*reinterpret_cast<const __half2 *>(&y), __half2half2(__ushort_as_half(0x6478)));
   return *reinterpret_cast<const uint32_t *>(&h);
 }
-template <bool EXACT> __device__ __forceinline__ uint32_t codes_high(uint32_t x) {
-  if constexpr (!EXACT) return x & 0x00f000f0u;
-  const uint32_t y = (x & 0x00f000f0u) | 0x64006400u;  // 1024 + 16 c
-  const __half2 h = __hsub2(*reinterpret_cast<const __half2 *>(&y), __half2half2(__ushort_as_half(0x6480)));
+__device__ __forceinline__ uint32_t codes_low(uint32_t x) {
+  const uint32_t y = (x & 0x000f000fu) | 0x64006400u;  // 1024 + c
+  const __half2 c = __hsub2(*reinterpret_cast<const __half2 *>(&y), __half2half2(__ushort_as_half(0x6400)));
+  const __half2 h = __hfma2(c, __half2half2(__ushort_as_half(0x4c00)), __half2half2(__ushort_as_half(0xd780)));  // 16 c - 120
   return *reinterpret_cast<const uint32_t *>(&h);
+}
+// The four codes of each half in order, as operands that stand for 1 / unit of
+// a code: 16 exactly, else 2^-24 (even) and 2^-20 (odd).
+template <bool EXACT> __device__ __forceinline__ void codes_of(uint32_t x, uint32_t (&c)[4]) {
+  const uint32_t y = x >> 8;
+  if constexpr (EXACT) {
+    c[0] = codes_low(x), c[1] = codes_high(x), c[2] = codes_low(y), c[3] = codes_high(y);
+  } else {
+    c[0] = x & 0x000f000fu, c[1] = x & 0x00f000f0u, c[2] = y & 0x000f000fu, c[3] = y & 0x00f000f0u;
+  }
 }
 
 // Records that a warp takes per iteration (one where 32 columns fill the
@@ -224,14 +234,15 @@ __host__ __device__ constexpr int att_parts(int hd, int nt) { return ATT_WARPS +
 // warp, and nothing is left for other blocks; a row's result then does not
 // depend on the rest of the batch.
 //
-// The codes reach the tensor pipe without being converted: a code in bits
-// 0-3 of a 16-bit word IS the half-precision number c * 2^-24 (a subnormal),
-// and in bits 4-7 c * 2^-20, so `and` makes two operands out of a 32-bit
-// word, and the factor of 16 is divided out of every other query element
-// (keys) or output row (values).  The tensor pipe lines subnormal products up
-// by their exponent field, so its sums keep about 15 bits (measured: 4e-5 of
-// fp32 rows' results), enough for 16-bit rows; fp32 rows pay one subtraction
-// per operand for the normal numbers c - 8.
+// The codes reach the tensor pipe almost as they are.  Of bf16 rows: a code in
+// bits 0-3 of a 16-bit word IS the half-precision number c * 2^-24 (a
+// subnormal), and in bits 4-7 c * 2^-20, so `and` makes two operands out of a
+// 32-bit word, and the factor of 16 is divided out of every other query
+// element (keys) or output row (values).  The tensor pipe lines subnormal
+// products up by their exponent field, so its sums keep about 15 bits
+// (measured: 4e-5 of fp32 rows' results, 2.4 times plain fp16's error at
+// 130,051 keys), enough for 8-bit results; fp16 and fp32 rows (EXACT) pay
+// one or two more operations for the normal numbers 16 (c - 7.5).
 //
 // Keys are the 16 rows of the first product and head_dim the 16 rows of the
 // second, with the query rows (tokens x group) as its 8 columns, so that a
@@ -243,22 +254,22 @@ __host__ __device__ constexpr int att_parts(int hd, int nt) { return ATT_WARPS +
 // number that is rounded to half precision) passes 2^14, or p passes 2^60,
 // and then to 2^8 below the top.  Weights keep 11 bits down to 2^-22 of the
 // largest; LIMBS = 2 (fp32 rows) adds a second half-precision limb to the
-// weights and the query, 22 bits.  Codes are centred at 8, which halves the
-// rounding's effect: directly for fp32 rows, by the sum of the rounded
-// weights (a product with ones) for 16-bit rows.
-template <int HD, int NT, int LIMBS>
+// weights and the query, 22 bits.  Codes are centred at 7.5, which halves the
+// rounding's effect: directly where EXACT, else by the sum of the rounded
+// weights (a product with ones).
+template <int HD, int NT, int LIMBS, bool EXACT>
 __global__ __launch_bounds__(ATT_THREADS, NT == 1 ? 2 : 1) void k_kv4_attention(AttArgs a) {
   constexpr int REC = kv4_rec_bytes(HD), ST = att_stages(HD, NT), RP = att_pair(HD, NT);
   constexpr int KS = HD / 16;            // k-steps of the first product, row tiles of the second
   constexpr int W = HD / 32;             // 32-bit words of a key row per lane
   constexpr int COLS = 8 * NT;
-  constexpr bool EXACT = LIMBS == 2;
   // Parts that a block has in the workspace: items that end in each warp, the
   // block's first and last item, and, where a ring cannot hold one, items
   // that go on after each warp.
   constexpr bool ON_SHARED = att_on_shared(HD, NT);
   constexpr int PARTS = att_parts(HD, NT);
-  constexpr float UNIT = EXACT ? 1.0f : 16777216.0f;  // what a code's operand is divided by
+  // A code's operand is the code over this, of even and odd elements.
+  constexpr float EVEN = EXACT ? 1.0f / 16.0f : 16777216.0f, ODD = EXACT ? 1.0f / 16.0f : 1048576.0f;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int scan_t[ATT_THREADS], scan_q[ATT_THREADS], warp_t[ATT_WARPS], warp_q[ATT_WARPS], warp_top[ATT_WARPS];
   __shared__ int req_len[ATT_THREADS], req_row[ATT_THREADS], req_n[ATT_THREADS];  // of up to as many requests
@@ -461,7 +472,7 @@ __global__ __launch_bounds__(ATT_THREADS, NT == 1 ? 2 : 1) void k_kv4_attention(
       const int e = (int)(__float_as_uint(top) >> 23);  // biased exponent
       const int up = e == 0 || e == 255 ? 0 : min(max(13 - (e - 127), -100), 100);
       const float f = __uint_as_float((uint32_t)(127 + up) << 23), back = __uint_as_float((uint32_t)(127 - up) << 23);
-      code_scale = sl * UNIT * back;
+      code_scale = sl * EVEN * back;
 #pragma unroll
       for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -469,7 +480,7 @@ __global__ __launch_bounds__(ATT_THREADS, NT == 1 ? 2 : 1) void k_kv4_attention(
           uint32_t v[LIMBS][4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float k = (i & 1) ? f * 0.0625f : f;
+            const float k = (i & 1) && !EXACT ? f * 0.0625f : f;
             const float y0 = x[j][4 * w + i][0] * k, y1 = x[j][4 * w + i][1] * k;
             v[0][i] = pack_half(y0, y1);
             if constexpr (LIMBS == 2) {
@@ -544,33 +555,33 @@ __global__ __launch_bounds__(ATT_THREADS, NT == 1 ? 2 : 1) void k_kv4_attention(
         }
 #pragma unroll
         for (int w = 0; w < W; ++w) {
-          const uint32_t x = ka[w], y = kb[w], xs = x >> 8, ys = y >> 8;
-          const uint32_t a0 = codes_low<EXACT>(x), a1 = codes_low<EXACT>(y), a2 = codes_high<EXACT>(x), a3 = codes_high<EXACT>(y);
-          const uint32_t c0 = codes_low<EXACT>(xs), c1 = codes_low<EXACT>(ys), c2 = codes_high<EXACT>(xs), c3 = codes_high<EXACT>(ys);
+          uint32_t x[4], y[4];
+          codes_of<EXACT>(ka[w], x);
+          codes_of<EXACT>(kb[w], y);
 #pragma unroll
           for (int j = 0; j < NT; ++j)
 #pragma unroll
             for (int lm = 0; lm < LIMBS; ++lm) {
               if constexpr (NT == 1) {
-                mma16816(sc[k][j], a0, a1, a2, a3, bq[lm][2 * w][0], bq[lm][2 * w][1]);
-                mma16816(sc[k][j], c0, c1, c2, c3, bq[lm][2 * w + 1][0], bq[lm][2 * w + 1][1]);
+                mma16816(sc[k][j], x[0], y[0], x[1], y[1], bq[lm][2 * w][0], bq[lm][2 * w][1]);
+                mma16816(sc[k][j], x[2], y[2], x[3], y[3], bq[lm][2 * w + 1][0], bq[lm][2 * w + 1][1]);
               } else {
                 const uint4 f = qfrag[((j * LIMBS + lm) * W + w) * 32 + lane];
-                mma16816(sc[k][j], a0, a1, a2, a3, f.x, f.y);
-                mma16816(sc[k][j], c0, c1, c2, c3, f.z, f.w);
+                mma16816(sc[k][j], x[0], y[0], x[1], y[1], f.x, f.y);
+                mma16816(sc[k][j], x[2], y[2], x[3], y[3], f.z, f.w);
               }
             }
         }
       }
-      // parameters of keys g and g + 8; a value's base is taken at code 8
+      // parameters of keys g and g + 8; a value's base is taken at code 7.5
       float ks[2 * RP], kz[2 * RP], vs[2 * RP], vz[2 * RP];
 #pragma unroll
       for (int i = 0; i < 2 * RP; ++i) {
         const uint8_t *rec = ring + (stage * RP + (i >> 1)) * REC;
         const uint2 p = *reinterpret_cast<const uint2 *>(rec + 16 * HD + (g + 8 * (i & 1)) * 8);
         ks[i] = bf16_lo(p.x) * code_scale;
-        kz[i] = EXACT ? fmaf(8.0f, bf16_lo(p.x), bf16_hi(p.x)) : bf16_hi(p.x);
-        vs[i] = bf16_lo(p.y), vz[i] = fmaf(8.0f, vs[i], bf16_hi(p.y));
+        kz[i] = EXACT ? fmaf(7.5f, bf16_lo(p.x), bf16_hi(p.x)) : bf16_hi(p.x);
+        vs[i] = bf16_lo(p.y), vz[i] = fmaf(7.5f, vs[i], bf16_hi(p.y));
       }
       uint32_t bw[RP][NT][LIMBS][2];
 #pragma unroll
@@ -667,16 +678,17 @@ __global__ __launch_bounds__(ATT_THREADS, NT == 1 ? 2 : 1) void k_kv4_attention(
         }
 #pragma unroll
         for (int w = 0; w < W; ++w) {
-          uint32_t x = v[0][w], y = v[1][w];
+          uint32_t x[4], y[4];
+          codes_of<EXACT>(v[0][w], x);
+          codes_of<EXACT>(v[1][w], y);
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
             const int m = 2 * w + q;  // rows of elements 32 w + 4 g + 2 q and the next
-            const uint32_t a0 = codes_low<EXACT>(x), a1 = codes_high<EXACT>(x), a2 = codes_low<EXACT>(y), a3 = codes_high<EXACT>(y);
 #pragma unroll
             for (int j = 0; j < NT; ++j)
 #pragma unroll
-              for (int lm = 0; lm < LIMBS; ++lm) mma16816(o[j][m], a0, a1, a2, a3, bw[k][j][lm][0], bw[k][j][lm][1]);
-            x >>= 8, y >>= 8;
+              for (int lm = 0; lm < LIMBS; ++lm)
+                mma16816(o[j][m], x[2 * q], x[2 * q + 1], y[2 * q], y[2 * q + 1], bw[k][j][lm][0], bw[k][j][lm][1]);
           }
         }
 #pragma unroll
@@ -721,11 +733,11 @@ __global__ __launch_bounds__(ATT_THREADS, NT == 1 ? 2 : 1) void k_kv4_attention(
         const int col = 8 * j + 2 * t + c;
         if (col >= ncol) continue;
         const float den = c ? l[j].y : l[j].x, zs = c ? z[j].y : z[j].x;
-        const float add = EXACT ? zs : fmaf(-8.0f, ones[j][c], zs);
+        const float add = EXACT ? zs : fmaf(-7.5f, ones[j][c], zs);
 #pragma unroll
         for (int k = 0; k < KS; k += 2) {
-          const float4 x = make_float4(fmaf(o[j][k][c], UNIT, add), fmaf(o[j][k][c + 2], UNIT / 16.0f, add),
-                                       fmaf(o[j][k + 1][c], UNIT, add), fmaf(o[j][k + 1][c + 2], UNIT / 16.0f, add));
+          const float4 x = make_float4(fmaf(o[j][k][c], EVEN, add), fmaf(o[j][k][c + 2], ODD, add),
+                                       fmaf(o[j][k + 1][c], EVEN, add), fmaf(o[j][k + 1][c + 2], ODD, add));
           const int d = 16 * k + 4 * g;
           if (alone) emit(a, row0, head, col, d, x, den);
           else *reinterpret_cast<float4 *>(mine + col * HD + d) = x;
@@ -903,16 +915,16 @@ int check_attn(const cis2b_kv4_cache *c, const cis2b_kv4_attn *a) {
   return CIS2B_OK;
 }
 
-template <int HD, int NT, int LIMBS>
+template <int HD, int NT, int LIMBS, bool EXACT>
 int launch(const AttArgs &args, const cis2b_kv4_cache *c, uint64_t most, int sms, cudaStream_t stream) {
   static std::atomic<int> resident[64];  // blocks per SM, by device; also: the attribute is set
   const int smem = att_smem_bytes(HD, NT, LIMBS);
   int n = resident[c->device].load(std::memory_order_relaxed);
   if (!n) {
-    if (int rc = kv4_cuda(cudaFuncSetAttribute(k_kv4_attention<HD, NT, LIMBS>,
+    if (int rc = kv4_cuda(cudaFuncSetAttribute(k_kv4_attention<HD, NT, LIMBS, EXACT>,
                                                cudaFuncAttributeMaxDynamicSharedMemorySize, smem)))
       return rc;
-    if (int rc = kv4_cuda(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, k_kv4_attention<HD, NT, LIMBS>,
+    if (int rc = kv4_cuda(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, k_kv4_attention<HD, NT, LIMBS, EXACT>,
                                                                         ATT_THREADS, smem)))
       return rc;
     n = std::max(n, 1);
@@ -921,19 +933,23 @@ int launch(const AttArgs &args, const cis2b_kv4_cache *c, uint64_t most, int sms
   const int grid = (int)std::max<uint64_t>(1, std::min<uint64_t>(most, (uint64_t)sms * n));
   AttArgs given = args;
   given.per_warp = nextafterf(1.0f / (float)(grid * ATT_WARPS), 1.0f);
-  k_kv4_attention<HD, NT, LIMBS><<<grid, ATT_THREADS, smem, stream>>>(given);
+  k_kv4_attention<HD, NT, LIMBS, EXACT><<<grid, ATT_THREADS, smem, stream>>>(given);
   return kv4_cuda(cudaGetLastError());
 }
 
 template <int HD>
 int dispatch(const Shape &s, const AttArgs &args, const cis2b_kv4_cache *c, uint64_t most, int sms, cudaStream_t st) {
-  switch (s.nt * 10 + s.limbs) {
-    case 11: return launch<HD, 1, 1>(args, c, std::min<uint64_t>(most, s.blocks), sms, st);
-    case 12: return launch<HD, 1, 2>(args, c, std::min<uint64_t>(most, s.blocks), sms, st);
-    case 21: return launch<HD, 2, 1>(args, c, std::min<uint64_t>(most, s.blocks), sms, st);
-    case 22: return launch<HD, 2, 2>(args, c, std::min<uint64_t>(most, s.blocks), sms, st);
-    case 41: return launch<HD, 4, 1>(args, c, std::min<uint64_t>(most, s.blocks), sms, st);
-    default: return launch<HD, 4, 2>(args, c, std::min<uint64_t>(most, s.blocks), sms, st);
+  const bool one = s.limbs == 1, bf16 = args.dtype == KV4_BF16;
+  switch (s.nt) {
+    case 1:
+      return !one ? launch<HD, 1, 2, true>(args, c, most, sms, st)
+                  : bf16 ? launch<HD, 1, 1, false>(args, c, most, sms, st) : launch<HD, 1, 1, true>(args, c, most, sms, st);
+    case 2:
+      return !one ? launch<HD, 2, 2, true>(args, c, most, sms, st)
+                  : bf16 ? launch<HD, 2, 1, false>(args, c, most, sms, st) : launch<HD, 2, 1, true>(args, c, most, sms, st);
+    default:
+      return !one ? launch<HD, 4, 2, true>(args, c, most, sms, st)
+                  : bf16 ? launch<HD, 4, 1, false>(args, c, most, sms, st) : launch<HD, 4, 1, true>(args, c, most, sms, st);
   }
 }
 
@@ -1021,5 +1037,6 @@ extern "C" int cis2b_kv4_attention(const cis2b_kv4_cache *c, const cis2b_kv4_att
   k.whole = (a->flags & CIS2B_KV4_WHOLE) || s.items * (recs + ATT_SETUP) > INT_MAX;
   const uint64_t most = std::max(s.items, (s.items * ((recs + ATT_LEAST - 1) / ATT_LEAST) + ATT_WARPS - 1) / ATT_WARPS);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return c->head_dim == 64 ? dispatch<64>(s, k, c, most, sms, st) : dispatch<128>(s, k, c, most, sms, st);
+  return c->head_dim == 64 ? dispatch<64>(s, k, c, std::min<uint64_t>(most, s.blocks), sms, st)
+                           : dispatch<128>(s, k, c, std::min<uint64_t>(most, s.blocks), sms, st);
 }

@@ -5,8 +5,7 @@
 // A unit is 128 query rows (tokens x the group of one KV head) of one request
 // against a stretch of its keys.  Per tile of 128 keys:
 //   four warps turn codes into half-precision operands in shared memory
-//     (c - 8, exact; odd elements times 16, divided out of the query and of
-//     the result), keys as [key][element], values as [element][key];
+//     (16 (c - 7.5), exact), keys as [key][element], values as [element][key];
 //   one thread issues S = Q K^T into TMEM (128 x 128 fp32);
 //   four warps, one query row per thread, turn S into weights: score =
 //     S * ks_j + kz_j sum(q), p = 2^(score - M), w = p vs_j rounded to half
@@ -354,6 +353,8 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
       if constexpr (ROUNDED) {  // a positive factor of the scores
         if (!(code_scale > 0.0f)) f = code_scale < 0.0f ? -f : code_scale == 0.0f ? 0.0f : f;
         code_scale = code_scale == 0.0f ? 1.0f : fabsf(code_scale);
+      } else {
+        code_scale *= 0.0625f;  // the codes' operands are 16 times as large
       }
       if (warp < 4) {
 #pragma unroll 1
@@ -365,8 +366,7 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
             uint32_t v[LIMBS][4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {  // elements i and i + 4, as a word's codes come out
-              const float k = (i & 1) && !ROUNDED ? f * 0.0625f : f;
-              const float y0 = e[d - d0 + i] * k, y1 = e[d - d0 + i + 4] * k;
+              const float y0 = e[d - d0 + i] * f, y1 = e[d - d0 + i + 4] * f;
               v[0][i] = pack_half(y0, y1);
               if constexpr (LIMBS == 2) {
                 const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&v[0][i]));
@@ -468,8 +468,8 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
         if constexpr (!ROUNDED) {
         float *dst = reinterpret_cast<float *>(sp + (now & 1) * 128 + (pt >> 1) * 2) + (pt & 1);
         const float ks = bf16_lo(par.x), vs = bf16_lo(par.y);
-        dst[0] = ks * code_scale, dst[2] = fmaf(8.0f, ks, bf16_hi(par.x));
-        dst[4] = vs, dst[6] = fmaf(8.0f, vs, bf16_hi(par.y));
+        dst[0] = ks * code_scale, dst[2] = fmaf(7.5f, ks, bf16_hi(par.x));
+        dst[4] = vs, dst[6] = fmaf(7.5f, vs, bf16_hi(par.y));
         // (a step that is not a number, or zero, bounds nothing)
         const uint32_t most = __reduce_max_sync(0xffffffffu, vs == vs ? __float_as_uint(vs) : 0u);
         if (lane == 0) value_part[now & 1][pw] = lg2(__uint_as_float(most));
@@ -486,12 +486,16 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
           }
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const uint32_t x = w[k], y = x >> 8;
+            uint32_t v[4];  // elements 0 and 4, 1 and 5, 2 and 6, 3 and 7 of the word
+            if constexpr (ROUNDED) {
+              const uint32_t x = w[k], y = x >> 8;
+              v[0] = value_low(x, step, at_zero), v[1] = value_high(x, step16, at_zero);
+              v[2] = value_low(y, step, at_zero), v[3] = value_high(y, step16, at_zero);
+            } else {
+              codes_of<true>(w[k], v);
+            }
             const int piece = (c & 1) * 4 + k;
-            *reinterpret_cast<uint4 *>(sk + (c >> 1) * QB + key * 128 + (piece ^ (key & 7)) * 16) =
-                ROUNDED ? make_uint4(value_low(x, step, at_zero), value_high(x, step16, at_zero), value_low(y, step, at_zero),
-                                     value_high(y, step16, at_zero))
-                        : make_uint4(codes_low<true>(x), codes_high<true>(x), codes_low<true>(y), codes_high<true>(y));
+            *reinterpret_cast<uint4 *>(sk + (c >> 1) * QB + key * 128 + (piece ^ (key & 7)) * 16) = make_uint4(v[0], v[1], v[2], v[3]);
           }
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -518,18 +522,24 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
             uint32_t x[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) x[k] = __byte_perm(vw[i][2 * k], vw[i][2 * k + 1], h ? 0x7632 : 0x5410);
+            uint32_t y[4][4];  // [element 8 word + 4 h + e][keys 2 k and 2 k + 1]
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {  // element 8 word + 4 h + e of eight keys
-              uint32_t y[4];
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const uint32_t u = e < 2 ? x[k] : x[k] >> 8;
-                if constexpr (ROUNDED) y[k] = (e & 1) ? value_high(u, step16[k], at_zero[k]) : value_low(u, step[k], at_zero[k]);
-                else y[k] = (e & 1) ? codes_high<true>(u) : codes_low<true>(u);
+            for (int k = 0; k < 4; ++k) {
+              if constexpr (ROUNDED) {
+                const uint32_t u = x[k] >> 8;
+                y[0][k] = value_low(x[k], step[k], at_zero[k]), y[1][k] = value_high(x[k], step16[k], at_zero[k]);
+                y[2][k] = value_low(u, step[k], at_zero[k]), y[3][k] = value_high(u, step16[k], at_zero[k]);
+              } else {
+                uint32_t v[4];
+                codes_of<true>(x[k], v);
+                y[0][k] = v[0], y[1][k] = v[1], y[2][k] = v[2], y[3][k] = v[3];
               }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
               const int n = (word >> 3) * 64 + (4 * h + e) * 8 + (word & 7);
               *reinterpret_cast<uint4 *>(sv + (kg >> 3) * VB + n * 128 + ((kg & 7) ^ (n & 7)) * 16) =
-                  make_uint4(y[0], y[1], y[2], y[3]);
+                  make_uint4(y[e][0], y[e][1], y[e][2], y[e][3]);
             }
           }
         }
@@ -786,7 +796,7 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const float v = __uint_as_float(i < 4 ? x0[i * 8 + word] : x1[(i - 4) * 8 + word]);
-            y[i] = ROUNDED ? v : (i & 1) ? fmaf(v, 0.0625f, z) : v + z;
+            y[i] = ROUNDED ? v : fmaf(v, 0.0625f, z);
           }
           const int d = 8 * (8 * b + word);
           if (parts > 1) {
