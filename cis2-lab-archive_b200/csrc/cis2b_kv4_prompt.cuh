@@ -158,6 +158,7 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
   const AttArgs &a = pa.a;
   constexpr int REC = kv4_rec_bytes(HD);
   constexpr int TMEM = 128 + LIMBS * HD <= 256 ? 256 : 512;  // columns: S, O of each limb
+  constexpr float P_TOP = ROUNDED ? 90.0f : 54.0f;  // log2 of the largest p that M rises to
   constexpr int KB = HD / 64;                  // 64-element column blocks of Q and K
   constexpr uint32_t QB = PR_ROWS * 128, VB = HD * 128;  // bytes of a block of Q or K; of V
   extern __shared__ uint8_t pr_smem[];
@@ -658,12 +659,13 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
 #pragma unroll
           for (int i = 0; i < 16; i += 2) top = fmaxf(top, fmaxf(fmaxf(u[i].x, u[i].y), fmaxf(u[i + 1].x, u[i + 1].y)));
           top *= factor;
-          // Weights stay below 2^14, p below 2^60; if not, M rises to 2^8 below the top.
-          const bool raise = top - M > fminf(14.0f - lv_top, 60.0f);
+          // Weights stay below 2^14, p below 2^60 (ROUNDED, where it is only
+          // summed: 2^96); if not, M rises to 2^8 below the top.
+          const bool raise = top - M > fminf(14.0f - lv_top, P_TOP + 6.0f);
           if (__any_sync(0xffffffffu, raise)) {
             float f = 1.0f;
             if (raise) {
-              const float m = ceilf(top + fmaxf(lv_top - 8.0f, -54.0f));
+              const float m = ceilf(top + fmaxf(lv_top - 8.0f, -P_TOP));
               f = ex2(M - m);
               M = m, l *= f, z *= f;
             }
