@@ -38,7 +38,7 @@ struct AttArgs {
   int dtype, requests, rows, width, kv_heads, group, shift, pages, window, sinks;
   int q_wide, o_wide;
   int qt;             // tokens per query tile
-  int items, whole;   // a bound on the items; whole items per block
+  int items, whole;   // a bound on the items that may be cut; whole items per block
   float scale;
   float per_warp;     // 1 / warps of the grid, rounded up
 };
@@ -204,9 +204,10 @@ template <bool EXACT> __device__ __forceinline__ void codes_of(uint32_t x, uint3
   }
 }
 
-// Records that a warp takes per iteration (one where 32 columns fill the
-// registers), iterations in its ring, and the shared memory of a block: its
-// warps' rings, then their query operands.
+// Records that a warp takes per iteration (one where two would spill: spilled
+// registers come back from L2, since the rings take L1's place; 48 against 44 us
+// at 130,051 keys), iterations in its ring, and the shared memory of a block:
+// its warps' rings, then their query operands.
 __host__ __device__ constexpr int att_pair(int hd, int nt) { return nt < 4 && !(hd == 128 && nt == 1) ? 2 : 1; }
 __host__ __device__ constexpr int att_stages(int hd, int nt) { return hd == 128 && nt == 1 ? 6 : nt < 4 ? (hd == 64 ? 4 : 3) : (hd == 64 ? 6 : 4); }
 __host__ __device__ constexpr int att_ring_bytes(int hd, int nt) {
@@ -216,6 +217,8 @@ __host__ __device__ constexpr int att_smem_bytes(int hd, int nt, int limbs) {
   return att_ring_bytes(hd, nt) + (nt > 1 ? ATT_WARPS * nt * limbs * (hd / 32) * 512 : 0);
 }
 
+// Whether a ring has room for the part of an item that goes on after the warp;
+// parts that a block has in the workspace.
 __host__ __device__ constexpr bool att_on_shared(int hd, int nt) {
   return 8 * nt * (hd + 2) * 4 <= att_stages(hd, nt) * att_pair(hd, nt) * kv4_rec_bytes(hd);
 }
@@ -243,6 +246,14 @@ __host__ __device__ constexpr int att_parts(int hd, int nt) { return ATT_WARPS +
 // (measured: 4e-5 of fp32 rows' results, 2.4 times plain fp16's error at
 // 130,051 keys), enough for 8-bit results; fp16 and fp32 rows (EXACT) pay
 // one or two more operations for the normal numbers 16 (c - 7.5).
+//
+// The cache's bytes bound it: at 16 warps per SM a record of head_dim 128 takes
+// 101 cycles per SM (bf16; HBM's 93 at its measured rate), 345 instructions with
+// exact codes, which issue bounds at about 125.  Around that a call spends about
+// 10,000 cycles until the first record is there and 10,000 to 20,000 joining
+// parts.  Measured on the way: a block per 512 keys with tickets 184 us for the
+// ragged batch of 64 (a unit's fixed costs are 12,000 cycles), even stretches
+// per block 132, per warp 119 to 105.
 //
 // Keys are the 16 rows of the first product and head_dim the 16 rows of the
 // second, with the query rows (tokens x group) as its 8 columns, so that a
@@ -869,7 +880,12 @@ struct Shape {
 
 constexpr int PR_BLOCKS = 320;  // of k_kv4_prompt at most: two for each of 148 SMs, and some to spare
 
-uint64_t round128(uint64_t x) { return (x + 127) / 128 * 128; }
+// The workspace begins with every word that has to be zero between calls, at
+// places that do not depend on a call's sizes: k_kv4_prompt's tickets and
+// counters, then k_kv4_attention's counters.  Parts follow; nothing reads a
+// part that its own call has not written.
+constexpr uint64_t WORK_PROMPT = 4096, WORK_ITEMS = 65536, WORK_PARTS = WORK_PROMPT + 4 * WORK_ITEMS;
+static_assert(8 + 4 * 2 * PR_BLOCKS <= WORK_PROMPT, "tickets and counters of k_kv4_prompt");
 
 // Query columns per item: the fewest groups of 8 that hold one request's rows,
 // up to 32.
@@ -888,14 +904,14 @@ Shape shape_of(const cis2b_kv4_cache *c, const cis2b_kv4_attn *a) {
     s.items = ((uint64_t)a->requests + (uint64_t)a->rows / s.qt) * c->kv_heads;  // at most
     // Query tiles of more than 1.25 PR_LEAST key tiles may be cut.
     if ((uint64_t)a->width * c->page_size > PR_KEYS * (PR_LEAST + PR_LEAST / 4)) s.slots = 2 * PR_BLOCKS;
-    s.bytes = round128(8 + 4 * 2 * PR_BLOCKS) + s.slots * PR_ROWS * (c->head_dim + 2) * 4;
+    s.bytes = WORK_PARTS + s.slots * PR_ROWS * (c->head_dim + 2) * 4;
     return s;
   }
   s.cols = 8 * s.nt;
   s.qt = s.cols / group;
   s.blocks = s.nt == 1 ? 320 : 160;  // at most: two or one for each of 148 SMs, and some to spare
   s.items = ((uint64_t)a->requests + (uint64_t)a->rows / s.qt) * c->kv_heads;  // at most
-  s.bytes = round128(s.items * 4) + (uint64_t)s.blocks * att_parts(c->head_dim, s.nt) * s.cols * (c->head_dim + 2) * 4;
+  s.bytes = WORK_PARTS + (uint64_t)s.blocks * att_parts(c->head_dim, s.nt) * s.cols * (c->head_dim + 2) * 4;
   return s;
 }
 
@@ -1018,7 +1034,7 @@ extern "C" int cis2b_kv4_attention(const cis2b_kv4_cache *c, const cis2b_kv4_att
     p.a = k;
     p.ticket = static_cast<uint32_t *>(a->work);
     p.counter = p.ticket + 2;
-    p.part = reinterpret_cast<float *>(static_cast<uint8_t *>(a->work) + round128(8 + 4 * 2 * PR_BLOCKS));
+    p.part = reinterpret_cast<float *>(static_cast<uint8_t *>(a->work) + WORK_PARTS);
     const uint64_t tiles = ((uint64_t)a->width * c->page_size + PR_KEYS - 1) / PR_KEYS;
     const uint64_t most = s.items * ((tiles + PR_LEAST - 1) / PR_LEAST);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -1028,13 +1044,13 @@ extern "C" int cis2b_kv4_attention(const cis2b_kv4_cache *c, const cis2b_kv4_att
       return c->head_dim == 64 ? launch_prompt<64, 1, false>(p, c, most, sms, st) : launch_prompt<128, 1, false>(p, c, most, sms, st);
     return c->head_dim == 64 ? launch_prompt<64, 2, false>(p, c, most, sms, st) : launch_prompt<128, 2, false>(p, c, most, sms, st);
   }
-  k.counter = static_cast<uint32_t *>(a->work);
-  k.part = reinterpret_cast<float *>(static_cast<uint8_t *>(a->work) + round128(s.items * 4));
+  k.counter = reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(a->work) + WORK_PROMPT);
+  k.part = reinterpret_cast<float *>(static_cast<uint8_t *>(a->work) + WORK_PARTS);
   fill(k, c, a, s);
   const uint64_t recs = ((uint64_t)a->width * c->page_size + 15) / 16;
-  // The row of records is counted in 32 bits; a batch that could pass that has
-  // items enough to take them whole.
-  k.whole = (a->flags & CIS2B_KV4_WHOLE) || s.items * (recs + ATT_SETUP) > INT_MAX;
+  // The row of records is counted in 32 bits, and an item that is cut has a
+  // counter; a batch that could pass that has items enough to take them whole.
+  k.whole = (a->flags & CIS2B_KV4_WHOLE) || s.items > WORK_ITEMS || s.items * (recs + ATT_SETUP) > INT_MAX;
   const uint64_t most = std::max(s.items, (s.items * ((recs + ATT_LEAST - 1) / ATT_LEAST) + ATT_WARPS - 1) / ATT_WARPS);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   return c->head_dim == 64 ? dispatch<64>(s, k, c, std::min<uint64_t>(most, s.blocks), sms, st)

@@ -11,21 +11,28 @@
 //     S * ks_j + kz_j sum(q), p = 2^(score - M), w = p vs_j rounded to half
 //     precision and put back over S in TMEM; p and p vz_j are summed in fp32;
 //   the same thread issues O += W V^T (128 x head_dim fp32 in TMEM).
-// The two blocks of an SM fill each other's waits: per tile and block the
-// tensor cores are needed for 2 x 512 cycles of head_dim 128, the exponentials
-// take 1,024 and the instructions of all warps about 1,100.
+// The two blocks of an SM fill each other's waits.  Per tile of head_dim 128
+// the tensor cores need 1,024 cycles, the exponentials 1,024 and the warps'
+// 7,300 instructions 1,825; measured (bf16, 100 GFLOP) are 3,650, i.e. 7,300
+// per block: 4,100 for the row warps' work, whose registers leave no room to
+// load ahead, and 3,100 for the products and the hand-offs around them, which
+// cannot overlap it since the weights take the scores' place in TMEM.
+// Measured slower: the products issued by a code warp (it stalls while they
+// are queued) or by a ninth warp (96 registers), a pass of its own for the
+// row's top, polling without suspension.
 //
 // M is an integer (a power of two scales exactly) and moves only when a weight
 // could pass 2^14 (by the row's top score and the largest step of 32 keys) or p
-// 2^60; then the row's weights already written, its sums and its O are scaled.  LIMBS = 2 (fp32 rows): two
-// half-precision limbs of the query and of the weights, twice the products.
+// 2^60; then the row's weights already written, its sums and its O are scaled.
+// LIMBS = 2 (fp32 rows): two half-precision limbs of the query and of the
+// weights, twice the products.
 // The tensor cores cut off what falls below their sums, so the small limbs have
 // an O of their own, and are the first in S: that halves the cuts at full size
 // (measured 1.5e-6 of the results without it).
 //
 // Each key's four parameters cost the row warps two 16-byte broadcasts from
-// shared memory per pair of keys, 2,048 cycles a tile, more than anything else.
-// ROUNDED (bf16 rows) does without: the code warps store keys and values
+// shared memory per pair of keys, 2,048 cycles a tile (240 us where ROUNDED takes
+// 204).  ROUNDED (bf16 rows) does without: the code warps store keys and values
 // themselves, base + step * c rounded once to half precision (11 bits, where
 // the rows and the result have 8), scaled by a power of two per 32 keys that the
 // row warps take into the exponent.  A key with a NaN (or of 2^119 or more) is
@@ -59,7 +66,7 @@ __device__ __forceinline__ void bar_arrive(uint32_t b) {
 }
 __device__ __forceinline__ bool bar_poll(uint32_t b, uint32_t parity) {
   uint32_t ok;
-  asm volatile("{.reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 1000; selp.b32 %0, 1, 0, p;}"
+  asm volatile("{.reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.b32 %0, 1, 0, p;}"
                : "=r"(ok) : "r"(b), "r"(parity) : "memory");
   return ok;
 }

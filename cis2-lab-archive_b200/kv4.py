@@ -191,6 +191,8 @@ class Cache:
         bits = int(self.status.item())
         if bits:
             self.status.zero_()
+        if bits & STUCK:
+            self._work.clear()  # counters may have been left in the middle
         return bits
 
     def _rows(self, t, name: str):

@@ -440,6 +440,31 @@ def test_offsets_past_32_bits(torch, kv4):
     assert np.abs(k[0].double().cpu().numpy() - w.k[0][0]).max() < 1e-5
 
 
+def test_one_workspace_serves_calls_of_all_sizes(torch, kv4):
+    """Batches of other sizes, and both kernels, one after another on one cache: nothing that one call
+    leaves in the workspace is taken for a counter by the next."""
+    lengths, new = [3000, 2500, 40, 900, 1700, 33, 2100], [1, 60, 40, 1, 3, 33, 1]
+    w = World(torch, kv4, lengths, new, 2, 64, 16, "float32")
+    start = np.concatenate([[0], np.cumsum(new)])
+    q = w.queries(6, 64)
+
+    def part(first, last, max_new):
+        b = kv4.Batch.of(w.table[first:last].contiguous(), w.batch.length[first:last].clone(),
+                         (w.batch.row_start[first:last + 1] - int(start[first])).contiguous(), 16)
+        return w.cache.attention(q[start[first]:start[last]], b, max_new=max_new)
+
+    calls = [(0, 1, 1), (3, 5, 3), (0, 7, 60), (0, 7, 1), (1, 3, 60), (6, 7, 1), (2, 7, 40), (0, 4, 2), (0, 1, 1)]
+    first = [part(*c) for c in calls]
+    again = [part(*c) for c in calls[::-1]][::-1]
+    w.cache._work.clear()
+    for c, a, b in zip(calls, first, again):
+        fresh = part(*c)
+        w.cache._work.clear()
+        assert torch.equal(a, fresh) and torch.equal(b, fresh), c
+    w.check(q, first[2])
+    assert w.cache.errors() == 0
+
+
 def test_streams_and_graphs(torch, kv4):
     """Calls on two streams of one cache do not share a workspace; a captured step replays."""
     lengths = [2500, 1800]
