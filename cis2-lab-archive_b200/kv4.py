@@ -164,6 +164,7 @@ class Batch:
 
 class Cache:
     """One layer's keys and values in 4 bits: a pool of pages on the device.
+    Like a model handle, it belongs to one thread at a time.
 
     pool  uint8 [pages, kv_heads, page_size // 16, 16 * (head_dim + 8)];
           pass your own to place it, else it is allocated (zeroed)."""
