@@ -307,7 +307,7 @@ __global__ __launch_bounds__(ATT_THREADS, NT == 1 ? 2 : 1) void k_kv4_attention(
   {
     int st = 0, sq = 0, top = 1;
     for (int r = tid * per; r < min(tid * per + per, a.requests); ++r) {
-      const int row = __ldg(a.row_start + r), n = __ldg(a.row_start + r + 1) - row, len = __ldg(a.length + r);
+      const int row = __ldg(a.row_start + r), n = min(__ldg(a.row_start + r + 1) - row, a.rows), len = __ldg(a.length + r);
       if (per == 1) req_len[r] = len, req_row[r] = row, req_n[r] = n;
       if (n <= 0) continue;
       const int nq = n <= a.qt ? 1 : (n + a.qt - 1) / a.qt;
@@ -359,11 +359,11 @@ __global__ __launch_bounds__(ATT_THREADS, NT == 1 ? 2 : 1) void k_kv4_attention(
       seg += 31 - __clz(fine & ((1u << (ATT_THREADS / 32)) - 1));
     }
     int base = scan[seg], qbase = scan_q[seg], r = seg * per, n, len, row0, nq, vt, size;
-    for (;; ++r) {
+    for (; r < a.requests; ++r) {
       if (per == 1) {
         len = req_len[r], row0 = req_row[r], n = req_n[r];
       } else {
-        len = __ldg(a.length + r), row0 = __ldg(a.row_start + r), n = __ldg(a.row_start + r + 1) - row0;
+        len = __ldg(a.length + r), row0 = __ldg(a.row_start + r), n = min(__ldg(a.row_start + r + 1) - row0, a.rows);
       }
       if (n <= 0) continue;
       nq = n <= a.qt ? 1 : (n + a.qt - 1) / a.qt;
@@ -373,6 +373,7 @@ __global__ __launch_bounds__(ATT_THREADS, NT == 1 ? 2 : 1) void k_kv4_attention(
       if (at < next) break;
       base = next, qbase += nq * a.kv_heads;
     }
+    if (r >= a.requests) break;  // row starts that do not belong together
     const int item = (int)((uint32_t)(at - base) / (uint32_t)size);
     const int turn = nq == 1 ? 0 : (int)((uint32_t)item / (uint32_t)a.kv_heads), head = item - turn * a.kv_heads;
     // Later query tiles see more: taken from both ends in turn, so that any

@@ -206,7 +206,7 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
     int sum = 0;
     {
       for (int r = tid * per; r < min(tid * per + per, a.requests); ++r) {
-        const int row = __ldg(a.row_start + r), n = max(0, __ldg(a.row_start + r + 1) - row), len = __ldg(a.length + r);
+        const int row = __ldg(a.row_start + r), n = max(0, min(__ldg(a.row_start + r + 1) - row, a.rows)), len = __ldg(a.length + r);
         if (per == 1) req_len[r] = len, req_row[r] = row, req_n[r] = n;
         sum += (n + a.qt - 1) / a.qt;
       }
@@ -241,16 +241,19 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
       if (scan_q[seg + step] <= q) seg += step;
     int before = scan_q[seg];
     Tile t;
-    for (t.r = seg * per;; ++t.r) {
+    t.len = t.n = t.row0 = 0;
+    for (t.r = seg * per; t.r < a.requests; ++t.r) {
       if (per == 1) {
         t.len = req_len[t.r], t.row0 = req_row[t.r], t.n = req_n[t.r];
       } else {
-        t.len = __ldg(a.length + t.r), t.row0 = __ldg(a.row_start + t.r), t.n = max(0, __ldg(a.row_start + t.r + 1) - t.row0);
+        t.len = __ldg(a.length + t.r), t.row0 = __ldg(a.row_start + t.r);
+        t.n = max(0, min(__ldg(a.row_start + t.r + 1) - t.row0, a.rows));
       }
       const int nq = (t.n + a.qt - 1) / a.qt;
       if (q < before + nq) break;
       before += nq;
     }
+    if (t.r >= a.requests) t.r = 0, t.n = t.len = 0;  // row starts that do not belong together: no rows
     t.qi = q - before;
     return t;
   };

@@ -569,3 +569,22 @@ def test_refusals(torch, kv4):
     a = kv4._Attn(0, 4, 1, 1, 4, 1, 0, 0, 0.125, 0, q.data_ptr(), q.data_ptr(), 256, 64, 256, 64, batch.table.data_ptr(),
                   batch.length.data_ptr(), batch.row_start.data_ptr(), q.data_ptr(), 1)
     assert kv4._lib().cis2b_kv4_attention(cache._ref, ctypes.byref(a), None) == 1
+
+
+@pytest.mark.parametrize("max_new", [1, 64])
+def test_row_starts_and_lengths_that_do_not_belong_together(torch, kv4, max_new):
+    """Row starts that go back, leave the rows or overlap, and negative lengths: the call ends, writes only
+    inside out, and the next call is right."""
+    w = World(torch, kv4, [300, 40, 500], [1, 1, 1], 2, 64, 16, "float32")
+    q = w.queries(4, 64)
+    want = w.cache.attention(q, w.batch, max_new=1)
+    guard = torch.full((5, 4, 64), 3.0, device="cuda")
+    for starts, lengths in [([2, 1, 0, 3], [300, 40, 500]), ([0, 100, 100, 200], [300, 40, 500]),
+                            ([-50, 1, 2, 1000], [300, 40, 500]), ([0, 1, 2, 3], [-5, 40, -1])]:
+        b = kv4.Batch.of(w.table, torch.tensor(lengths, dtype=torch.int32, device="cuda"),
+                         torch.tensor(starts, dtype=torch.int32, device="cuda"), 16)
+        w.cache.attention(q, b, max_new=max_new, out=guard[1:4])
+        assert (guard[0] == 3.0).all() and (guard[4] == 3.0).all()
+    w.cache.errors()
+    w.cache._work.clear()
+    assert torch.equal(w.cache.attention(q, w.batch, max_new=1), want)
