@@ -7,7 +7,7 @@
 #include <limits.h>
 
 #include <algorithm>
-#include <mutex>
+#include <type_traits>
 
 namespace cis2b {
 
@@ -200,37 +200,77 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return d;
 }
 
-// One group's parameters and codes.  D / 8 lanes hold its elements, eight
-// each; lo and hi are already the group's, NaN if an element is.  NaN and the
-// infinities leave a step that is not finite, which poisons the group.
-//   The quotient is at most 15 (1 + 2^-21), since the step is rounded up, and
-// at least 0, since the base is rounded down: no clamp.  Adding 1.5 * 2^23
-// rounds it to a whole number, ties to even, in the low bits of the sum, and
-// eight sums times powers of 16 make the word, less the constant's own part.
-__device__ __forceinline__ uint32_t kv4_quantise(const float (&x)[8], float lo, float hi, uint32_t &step16,
-                                                 uint32_t &base16) {
-  base16 = bf16_down(lo);
+// Minimum and negated maximum of eight elements, as one pair of their own type
+// (fp32: of fp32), NaN where an element is.
+struct Range32 {
+  float lo, neg_hi;
+  __device__ void join(int d) {
+    lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, d)), neg_hi = min_nan(neg_hi, __shfl_xor_sync(0xffffffffu, neg_hi, d));
+  }
+  __device__ float2 get() const { return make_float2(lo, -neg_hi); }
+};
+template <class T2> struct Range16 {
+  T2 both;
+  __device__ void join(int d) {
+    const uint32_t other = __shfl_xor_sync(0xffffffffu, *reinterpret_cast<const uint32_t *>(&both), d);
+    both = __hmin2_nan(both, *reinterpret_cast<const T2 *>(&other));
+  }
+  __device__ float2 get() const { return make_float2(__low2float(both), -__high2float(both)); }
+};
+__device__ __forceinline__ Range32 range_of(const float (&x)[8]) {
+  Range32 r = {x[0], x[0]};
+#pragma unroll
+  for (int i = 1; i < 8; ++i) r.lo = min_nan(r.lo, x[i]), r.neg_hi = max_nan(r.neg_hi, x[i]);
+  r.neg_hi = -r.neg_hi;
+  return r;
+}
+template <class T2> __device__ __forceinline__ Range16<T2> range_of(const uint32_t (&w)[4]) {
+  T2 lo = *reinterpret_cast<const T2 *>(&w[0]), hi = lo;
+#pragma unroll
+  for (int i = 1; i < 4; ++i) {
+    const T2 x = *reinterpret_cast<const T2 *>(&w[i]);
+    lo = __hmin2_nan(lo, x), hi = __hmax2_nan(hi, x);
+  }
+  hi = __hneg2(hi);
+  // (lo.x, -hi.x) and (lo.y, -hi.y)
+  const uint32_t l = *reinterpret_cast<const uint32_t *>(&lo), h = *reinterpret_cast<const uint32_t *>(&hi);
+  const uint32_t a = __byte_perm(l, h, 0x5410), b = __byte_perm(l, h, 0x7632);
+  return {__hmin2_nan(*reinterpret_cast<const T2 *>(&a), *reinterpret_cast<const T2 *>(&b))};
+}
+
+// A group's step (low 16 bits) and base (high) as bfloat16, and the factor of
+// its elements; NaN in both for a group with a NaN, an infinity, or too wide.
+__device__ __forceinline__ uint32_t kv4_params(float lo, float hi, float &inv) {
+  const uint32_t base16 = bf16_down(lo);
   const float base = __uint_as_float(base16 << 16);
   const float q = __fdiv_rn(__fsub_rn(hi, base), 15.0f);
-  if (!(q <= 3.3e38f) || !(fabsf(base) <= 3.3e38f)) {  // bfloat16's largest is 3.39e38
-    step16 = base16 = 0x7fc0u;
-    return 0;
-  }
-  step16 = bf16_up(q);
+  const bool fine = q <= 3.3e38f && fabsf(base) <= 3.3e38f;  // bfloat16's largest is 3.39e38
+  uint32_t step16 = bf16_up(q);
   float step = __uint_as_float(step16 << 16);
   if (step < 0x1p-100f) step = 0.0f, step16 = 0;
-  const float inv = step > 0.0f ? __frcp_rn(step) : 0.0f;
+  inv = step > 0.0f ? __frcp_rn(step) : 0.0f;
+  return fine ? step16 | base16 << 16 : 0x7fc07fc0u;
+}
+
+// Eight codes.  The quotient is at most 15 (1 + 2^-21), since the step is
+// rounded up, and at least 0, since the base is rounded down: no clamp.  Adding
+// 1.5 * 2^23 rounds it to a whole number, ties to even, in the low bits of the
+// sum, and eight sums times powers of 16 make the word, less the constant's own
+// part.
+__device__ __forceinline__ uint32_t kv4_codes(const float (&x)[8], uint32_t params, float inv) {
+  const float base = bf16_hi(params);
   uint32_t word = 0;
 #pragma unroll
   for (int i = 7; i >= 0; --i)
     word = word * 16 + __float_as_uint(__fadd_rn(__fmul_rn(__fsub_rn(x[i], base), inv), 12582912.0f));
-  return word - 0x4b400000u * 0x11111111u;
+  return base == base ? word - 0x4b400000u * 0x11111111u : 0u;
 }
 
 // Rows to codes: D / 8 lanes take one (row, head), eight key and eight value
 // elements each, so one warp instruction reads whole 128-byte lines and a
-// group's minimum and maximum are log2(D / 8) shuffles away.  Bytes bound it:
-// each element is read once and each code written once.
+// group's range is log2(D / 8) shuffles away.  Half of the lanes then find the
+// key's parameters and half the value's.  Each element is read once and each
+// code written once; instructions bound it (fp16, 40,009 rows of 8 x 128).
 template <int HD, int DT>
 __global__ __launch_bounds__(ROW_THREADS) void k_kv4_append(RowArgs a, const void *k, const void *v, bool wide) {
   constexpr int LANES = HD / 8;
@@ -244,34 +284,45 @@ __global__ __launch_bounds__(ROW_THREADS) void k_kv4_append(RowArgs a, const voi
     if (a.status && part == 0) atomicOr(a.status, CIS2B_KV4_BAD_SLOT);
     slot = -1;
   }
+  const bool on = slot >= 0;
   float x[8], y[8];
-  float xl, xh, yl, yh;
-  if (slot >= 0) {
-    load8<DT>(k, row * a.ks + head * a.kh + part * 8, wide, x);
-    load8<DT>(v, row * a.vs + head * a.vh + part * 8, wide, y);
+  float2 xr, yr;
+  if constexpr (DT == KV4_F32) {
+    load_query<true, 8>(k, false, row * a.ks + head * a.kh + part * 8, wide, on, x);
+    load_query<true, 8>(v, false, row * a.vs + head * a.vh + part * 8, wide, on, y);
+    Range32 p = range_of(x), q = range_of(y);
+#pragma unroll
+    for (int d = 1; d < LANES; d <<= 1) p.join(d), q.join(d);
+    xr = p.get(), yr = q.get();
   } else {
+    using T2 = std::conditional_t<DT == KV4_F16, __half2, __nv_bfloat162>;
+    uint32_t xw[4], yw[4];
+    load_words(k, row * a.ks + head * a.kh + part * 8, wide, on, xw);
+    load_words(v, row * a.vs + head * a.vh + part * 8, wide, on, yw);
+    Range16<T2> p = range_of<T2>(xw), q = range_of<T2>(yw);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = y[i] = 0.0f;
-  }
-  xl = xh = x[0], yl = yh = y[0];
+    for (int d = 1; d < LANES; d <<= 1) p.join(d), q.join(d);
+    xr = p.get(), yr = q.get();
 #pragma unroll
-  for (int i = 1; i < 8; ++i) {
-    xl = min_nan(xl, x[i]), xh = max_nan(xh, x[i]), yl = min_nan(yl, y[i]), yh = max_nan(yh, y[i]);
+    for (int i = 0; i < 4; ++i) {
+      const T2 u = *reinterpret_cast<const T2 *>(&xw[i]), w = *reinterpret_cast<const T2 *>(&yw[i]);
+      x[2 * i] = __low2float(u), x[2 * i + 1] = __high2float(u), y[2 * i] = __low2float(w), y[2 * i + 1] = __high2float(w);
+    }
   }
-#pragma unroll
-  for (int d = 1; d < LANES; d <<= 1) {
-    xl = min_nan(xl, __shfl_xor_sync(0xffffffffu, xl, d)), xh = max_nan(xh, __shfl_xor_sync(0xffffffffu, xh, d));
-    yl = min_nan(yl, __shfl_xor_sync(0xffffffffu, yl, d)), yh = max_nan(yh, __shfl_xor_sync(0xffffffffu, yh, d));
-  }
-  if (slot < 0) return;
-  uint32_t ks, kb, vs, vb;
-  const uint32_t kc = kv4_quantise(x, xl, xh, ks, kb), vc = kv4_quantise(y, yl, yh, vs, vb);
+  const bool of_value = part >= LANES / 2;
+  float inv;
+  const uint32_t params = kv4_params(of_value ? yr.x : xr.x, of_value ? yr.y : xr.y, inv);
+  const uint32_t other = __shfl_xor_sync(0xffffffffu, params, LANES / 2);
+  const float other_inv = __shfl_xor_sync(0xffffffffu, inv, LANES / 2);
+  if (!on) return;
+  const uint32_t kp = of_value ? other : params, vp = of_value ? params : other;
+  const uint32_t kc = kv4_codes(x, kp, of_value ? other_inv : inv), vc = kv4_codes(y, vp, of_value ? inv : other_inv);
   const int page = slot >> a.shift, off = slot & ((1 << a.shift) - 1), r = off & 15;
   uint8_t *rec = const_cast<uint8_t *>(a.pool) +
                  ((((int64_t)page * a.kv_heads + head) << (a.shift - 4)) + (off >> 4)) * kv4_rec_bytes(HD);
   reinterpret_cast<uint32_t *>(rec + r * (HD / 2))[part] = kc;
   reinterpret_cast<uint32_t *>(rec + (16 + r) * (HD / 2))[part] = vc;
-  if (part == 0) *reinterpret_cast<uint2 *>(rec + 16 * HD + r * 8) = make_uint2(ks | kb << 16, vs | vb << 16);
+  if (part == 0) *reinterpret_cast<uint2 *>(rec + 16 * HD + r * 8) = make_uint2(kp, vp);
 }
 
 // base + step * code: the product is exact (12 bits), so one rounding.  A code
@@ -282,37 +333,48 @@ __device__ __forceinline__ void kv4_values(uint32_t word, uint32_t params, float
   for (int i = 0; i < 8; ++i) x[i] = fmaf(step, __uint_as_float(((word >> (4 * i)) & 15) | 0x4b000000u) - 8388608.0f, base);
 }
 
-// Codes to rows, the same split.
+// Codes to rows, the same split, two rows per lane: what bounds it is the wait
+// for the slot and then for the codes.
 template <int HD>
 __global__ __launch_bounds__(ROW_THREADS) void k_kv4_gather(RowArgs a, void *k, void *v, int dt, bool wide) {
-  constexpr int LANES = HD / 8;
-  const uint32_t item = (uint32_t)blockIdx.x * (ROW_THREADS / LANES) + threadIdx.x / LANES;
+  constexpr int LANES = HD / 8, PER = ROW_THREADS / LANES;
+  const uint32_t items = (uint32_t)a.rows * a.kv_heads;
   const int part = threadIdx.x & (LANES - 1);
-  const int64_t row = item / (uint32_t)a.kv_heads;
-  const int head = (int)(item - (uint32_t)row * a.kv_heads);
-  if (row >= a.rows) return;
-  int slot = __ldg(a.slot + row);
-  if (slot >= a.slots) {
-    if (a.status && part == 0) atomicOr(a.status, CIS2B_KV4_BAD_SLOT);
-    slot = -1;
-  }
-  float x[8], y[8];
-  if (slot >= 0) {
-    const int page = slot >> a.shift, off = slot & ((1 << a.shift) - 1), r = off & 15;
-    const uint8_t *rec =
-        a.pool + ((((int64_t)page * a.kv_heads + head) << (a.shift - 4)) + (off >> 4)) * kv4_rec_bytes(HD);
-    const uint32_t kc = reinterpret_cast<const uint32_t *>(rec + r * (HD / 2))[part];
-    const uint32_t vc = reinterpret_cast<const uint32_t *>(rec + (16 + r) * (HD / 2))[part];
-    const uint2 p = *reinterpret_cast<const uint2 *>(rec + 16 * HD + r * 8);
-    kv4_values(kc, p.x, x);
-    kv4_values(vc, p.y, y);
-  } else {
+  uint32_t item[2], kc[2], vc[2];
+  uint2 p[2];
+  int slot[2], head[2];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = y[i] = 0.0f;
+  for (int i = 0; i < 2; ++i) {
+    item[i] = (uint32_t)blockIdx.x * (2 * PER) + i * PER + threadIdx.x / LANES;
+    const uint32_t row = item[i] / (uint32_t)a.kv_heads;
+    head[i] = (int)(item[i] - row * a.kv_heads);
+    slot[i] = item[i] < items ? __ldg(a.slot + row) : -1;
   }
-  const int64_t at = (int64_t)item * HD + part * 8;
-  store8(k, dt, at, wide, x);
-  store8(v, dt, at, wide, y);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if (slot[i] >= a.slots) {
+      if (a.status && part == 0) atomicOr(a.status, CIS2B_KV4_BAD_SLOT);
+      slot[i] = -1;
+    }
+    kc[i] = vc[i] = 0, p[i] = make_uint2(0, 0);
+    if (slot[i] < 0) continue;
+    const int page = slot[i] >> a.shift, off = slot[i] & ((1 << a.shift) - 1), r = off & 15;
+    const uint8_t *rec =
+        a.pool + ((((int64_t)page * a.kv_heads + head[i]) << (a.shift - 4)) + (off >> 4)) * kv4_rec_bytes(HD);
+    kc[i] = reinterpret_cast<const uint32_t *>(rec + r * (HD / 2))[part];
+    vc[i] = reinterpret_cast<const uint32_t *>(rec + (16 + r) * (HD / 2))[part];
+    p[i] = *reinterpret_cast<const uint2 *>(rec + 16 * HD + r * 8);
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if (item[i] >= items) continue;
+    float x[8], y[8];  // step and base 0 where there is nothing
+    kv4_values(kc[i], p[i].x, x);
+    kv4_values(vc[i], p[i].y, y);
+    const int64_t at = (int64_t)item[i] * HD + part * 8;
+    store8(k, dt, at, wide, x);
+    store8(v, dt, at, wide, y);
+  }
 }
 
 template <int HD>
@@ -403,6 +465,7 @@ extern "C" int cis2b_kv4_gather(const cis2b_kv4_cache *c, int32_t dtype, void *k
   if (!grid) return CIS2B_OK;
   const bool wide = !((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  grid = (grid + 1) / 2;  // two rows per lane
   if (c->head_dim == 64) k_kv4_gather<64><<<grid, ROW_THREADS, 0, s>>>(a, k, v, dtype, wide);
   else k_kv4_gather<128><<<grid, ROW_THREADS, 0, s>>>(a, k, v, dtype, wide);
   return kv4_cuda(cudaGetLastError());

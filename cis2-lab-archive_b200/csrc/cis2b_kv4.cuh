@@ -39,43 +39,21 @@ __device__ __forceinline__ uint32_t bf16_down(float x) {
 // The bfloat16 value at or above x, x >= 0.
 __device__ __forceinline__ uint32_t bf16_up(float x) { return (__float_as_uint(x) + 0xffffu) >> 16; }
 
-// Eight consecutive elements as float32.  `wide`: the address is 16-byte
-// aligned (the host checks base and strides once).
-template <int DT>
-__device__ __forceinline__ void load8(const void *base, int64_t at, bool wide, float (&x)[8]) {
-  if constexpr (DT == KV4_F32) {
-    const float *p = static_cast<const float *>(base) + at;
-    if (wide) {
-      const float4 a = __ldg(reinterpret_cast<const float4 *>(p));
-      const float4 b = __ldg(reinterpret_cast<const float4 *>(p) + 1);
-      x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-    } else {
+// Eight consecutive 16-bit elements, zeros where `on` is not set.  `wide`: the
+// address is 16-byte aligned (the host checks base and strides once).
+__device__ __forceinline__ void load_words(const void *base, int64_t at, bool wide, bool on, uint32_t (&w)[4]) {
+  const uint16_t *p = static_cast<const uint16_t *>(base) + at;
+  w[0] = w[1] = w[2] = w[3] = 0;
+  if (on && wide) {
+    const uint4 a = __ldg(reinterpret_cast<const uint4 *>(p));
+    w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
+  } else if (on) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = __ldg(p + i);
-    }
-  } else {
-    const uint16_t *p = static_cast<const uint16_t *>(base) + at;
-    uint32_t w[4];
-    if (wide) {
-      const uint4 a = __ldg(reinterpret_cast<const uint4 *>(p));
-      w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = __ldg(p + 2 * i) | (uint32_t)__ldg(p + 2 * i + 1) << 16;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (DT == KV4_BF16) {
-        x[2 * i] = bf16_lo(w[i]), x[2 * i + 1] = bf16_hi(w[i]);
-      } else {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
-        x[2 * i] = f.x, x[2 * i + 1] = f.y;
-      }
-    }
+    for (int i = 0; i < 4; ++i) w[i] = __ldg(p + 2 * i) | (uint32_t)__ldg(p + 2 * i + 1) << 16;
   }
 }
 
-// N consecutive query elements as float32, zeros where `on` is not set: fp32,
+// N consecutive elements as float32, zeros where `on` is not set: fp32,
 // or 16-bit elements of a type known at run time.  All loads are issued before
 // anything is done with them.
 template <bool F32, int N>
