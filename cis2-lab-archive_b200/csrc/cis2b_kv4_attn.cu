@@ -886,6 +886,7 @@ constexpr int PR_BLOCKS = 320;  // of k_kv4_prompt at most: two for each of 148 
 // counters, then k_kv4_attention's counters.  Parts follow; nothing reads a
 // part that its own call has not written.
 constexpr uint64_t WORK_PROMPT = 4096, WORK_ITEMS = 65536, WORK_PARTS = WORK_PROMPT + 4 * WORK_ITEMS;
+static_assert(WORK_PARTS == CIS2B_KV4_WORK_ZERO, "as include/cis2b.h says");
 static_assert(8 + 4 * 2 * PR_BLOCKS <= WORK_PROMPT, "tickets and counters of k_kv4_prompt");
 
 // Query columns per item: the fewest groups of 8 that hold one request's rows,

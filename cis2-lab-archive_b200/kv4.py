@@ -26,6 +26,7 @@ Cis2Error = _pkg.Cis2Error
 _I32, _I64, _U64, _P = ctypes.c_int32, ctypes.c_int64, ctypes.c_uint64, ctypes.c_void_p
 
 BAD_SLOT, BAD_PAGE, STUCK = 1, 2, 4  # CIS2B_KV4_*
+_WORK_ZERO = 266240  # CIS2B_KV4_WORK_ZERO
 PLAN_FREE, PLAN_WIDTH, PLAN_ROWS, PLAN_NEGATIVE = 1, 2, 4, 8  # CIS2B_KV4_PLAN_*
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # CIS2B_F32, _F16, _BF16
 
@@ -185,6 +186,7 @@ class Cache:
         self.status = torch.zeros(1, dtype=torch.int32, device=f"cuda:{self.device}")
         self._c.pool, self._c.status = self.pool.data_ptr(), self.status.data_ptr()
         self._work = {}   # by stream: calls on one stream follow one another
+        self._kept = []   # outgrown ones, which a captured graph may still hold
         self._calls = {}  # by shape: filled-in arguments
 
     def errors(self) -> int:
@@ -192,8 +194,11 @@ class Cache:
         bits = int(self.status.item())
         if bits:
             self.status.zero_()
-        if bits & STUCK:
-            self._work.clear()  # counters may have been left in the middle
+        if bits & STUCK:  # counters may have been left in the middle, on any stream
+            torch.cuda.synchronize(self.device)
+            for work in [*self._work.values(), *self._kept]:
+                work[:_WORK_ZERO].zero_()
+            torch.cuda.synchronize(self.device)
         return bits
 
     def _rows(self, t, name: str):
@@ -256,11 +261,21 @@ class Cache:
         stream = _raw_stream(dev)
         work = self._work.get(stream)
         if work is None or work.numel() < need:
-            work = self._work[stream] = torch.zeros(need, dtype=torch.uint8, device=q.device)
+            work = self._new_work(stream, need)
         a.q, a.out, a.work, a.work_bytes = q.data_ptr(), out.data_ptr(), work.data_ptr(), work.numel()
         a.table, a.length, a.row_start = batch.table.data_ptr(), batch.length.data_ptr(), batch.row_start.data_ptr()
         _call(dev, _lib().cis2b_kv4_attention, self._ref, ref)
         return out
+
+    def _new_work(self, stream: int, need: int):
+        work = torch.empty(need, dtype=torch.uint8, device=f"cuda:{self.device}")
+        work[:_WORK_ZERO].zero_()
+        if torch.cuda.is_current_stream_capturing():
+            return work  # the graph's own, zeroed by each replay; not for calls outside it
+        if stream in self._work:
+            self._kept.append(self._work[stream])
+        self._work[stream] = work
+        return work
 
     def _prepare(self, q, out, batch, scale, window, sinks, max_new, whole):
         if q.dim() != 3 or q.shape[2] != self.head_dim:
@@ -280,4 +295,4 @@ class Cache:
                   out.stride(0), out.stride(1), None, None, None, None, 0)
         need = _U64()
         _check(_lib().cis2b_kv4_workspace(self._ref, ctypes.byref(a), ctypes.byref(need)))
-        return a, ctypes.byref(a), max(16, need.value)
+        return a, ctypes.byref(a), need.value

@@ -362,13 +362,15 @@ int cis2b_kv4_gather(const cis2b_kv4_cache *c, int32_t dtype, void *k, void *v, 
  *              alone, and a request's result does not depend on the others
  *              (given the same max_new), at the cost of parallelism over long
  *              requests
- *   work       cis2b_kv4_workspace() bytes or more, zeroed once before the
- *              first call and then left alone: calls of other sizes may use
+ *   work       cis2b_kv4_workspace() bytes or more, of which the first
+ *              CIS2B_KV4_WORK_ZERO are zeroed once before the first call;
+ *              then left alone: calls of other sizes may use
  *              it too, but calls that may overlap on the GPU need one each.
  *              Zero it again after CIS2B_KV4_STUCK
  * Softmax statistics and sums are held in fp32; fp32 rows keep 22 bits of
  * every product's operands, 16-bit rows at least 11. */
 #define CIS2B_KV4_WHOLE 1
+#define CIS2B_KV4_WORK_ZERO 266240
 typedef struct {
   int32_t dtype;    /* CIS2B_F32, _F16 or _BF16: q and out */
   int32_t heads;    /* a multiple of kv_heads, at most 32 times as many */

@@ -491,6 +491,35 @@ def test_streams_and_graphs(torch, kv4):
         assert torch.equal(out, want)
 
 
+def test_a_first_call_inside_a_graph(torch, kv4):
+    """A call that makes its workspace while a graph is captured leaves nothing unzeroed to others, and a
+    workspace that is outgrown stays with the graph that holds it."""
+    w = World(torch, kv4, [2500, 1800], [1, 1], 2, 64, 16, "float32")
+    q = w.queries(4, 64)
+    out = torch.zeros_like(q)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        w.cache.attention(q, w.batch, max_new=1, out=out)
+    with torch.cuda.stream(side):  # before any replay
+        want = w.cache.attention(q, w.batch, max_new=1)
+        w.check(q, want)
+        second = torch.cuda.CUDAGraph()
+    out2 = torch.zeros_like(q)
+    with torch.cuda.graph(second, stream=side):
+        w.cache.attention(q, w.batch, max_new=1, out=out2)
+    with torch.cuda.stream(side):  # a larger workspace on the same stream
+        w.cache.attention(q, w.batch, max_new=16)
+    torch.cuda.synchronize()
+    for _ in range(2):
+        for g, o in ((graph, out), (second, out2)):
+            o.zero_()
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(o, want)
+
+
 def test_a_step_through_all_operators(torch, kv4):
     """plan, append and attention as a serving loop calls them, against the restatements: a prompt chunk,
     then decode steps, pages taken from a free list."""
