@@ -681,6 +681,7 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
             }
             // What stands in TMEM: this tile's earlier weights, and O.
             const __half2 f16 = __half2half2(__float2half_rn(f));
+            tc_wait_st();  // the weights that are read back were stored asynchronously
 #pragma unroll 1
             for (int k = 0; k < 2 * c; ++k) {
               uint32_t w[8 * LIMBS];

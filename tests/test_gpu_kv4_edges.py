@@ -1,0 +1,66 @@
+"""The 4-bit cache at its edges: jumps of the running maximum, what stands in
+places that no row sees, the ends of the number range, arguments that do not
+belong together, streams and graphs.
+
+Tolerances are those of test_gpu_kv4.py (errors relative to the largest
+|value| that the rows see); where a test needs another one its comment derives it."""
+from __future__ import annotations
+
+import importlib
+
+import numpy as np
+import pytest
+
+from test_gpu_kv4 import TOL, World, plain_attention, stands_for
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = ["float32", "float16", "bfloat16"]
+
+
+@pytest.fixture(scope="module")
+def torch():
+    return importlib.import_module("torch")
+
+
+@pytest.fixture(scope="module")
+def kv4():
+    return importlib.import_module("cis2-lab-archive_b200.kv4")
+
+
+def write(torch, w, x, y, request=0, first=0):
+    """Keys x and values y [n, kv_heads, head_dim] into the request's tokens first .. of a World."""
+    at = np.arange(first, first + len(x))
+    slots = (w.table[request].cpu().numpy()[at // w.page] * w.page + at % w.page).astype(np.int32)
+    w.cache.append(torch.from_numpy(x.astype(np.float32)).cuda(), torch.from_numpy(y.astype(np.float32)).cuda(),
+                   torch.from_numpy(slots).cuda())
+    if first + len(x) <= len(w.k[request]):
+        w.k[request][at], w.v[request][at] = stands_for(x), stands_for(y)
+
+
+def along(t, d, kv_heads=1):
+    """Keys whose product with a query of ones is t (log2 units where the scale is ln 2)."""
+    return np.broadcast_to((np.asarray(t, np.float64) / d)[:, None, None], (len(t), kv_heads, d)).astype(np.float32)
+
+
+LN2 = float(np.log(2.0))
+
+
+# ---------------------------------------------------------------- the running maximum
+
+@pytest.mark.parametrize("rise", [5.0, 12.0, 18.0])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_the_maximum_rises_inside_a_tile(torch, kv4, dtype, rise):
+    """The scores of every 32 keys stand `rise` above those before them (and start again with each 128),
+    so the weights of a tile that are already written have to be scaled, several times over."""
+    d, n, m = 64, 600, 70
+    w = World(torch, kv4, [n], [m], 1, d, 16, dtype)
+    g = np.random.default_rng(2)
+    j = np.arange(n)
+    x = along((j % 128 // 32) * rise + (j // 128) * rise * 2, d)
+    write(torch, w, x, g.standard_normal((n, 1, d)))
+    q = torch.ones((m, 2, d), device="cuda").to(w.dtype)
+    for _ in range(20):
+        out = w.cache.attention(q, w.batch, scale=LN2, max_new=m)
+    w.check(q, out, scale=LN2)
+    assert w.cache.errors() == 0
