@@ -169,7 +169,7 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
   constexpr int KB = HD / 64;                  // 64-element column blocks of Q and K
   constexpr uint32_t QB = PR_ROWS * 128, VB = HD * 128;  // bytes of a block of Q or K; of V
   extern __shared__ uint8_t pr_smem[];
-  __shared__ __align__(8) uint64_t bars[6];
+  __shared__ __align__(8) uint64_t bars[7];
   __shared__ int scan_q[256], req_len[256], req_row[256], req_n[256], warp_sum[8];
   __shared__ uint16_t order[PR_MAX_SORT], tiles_of[PR_MAX_SORT];
   __shared__ int part0[PR_MAX_SORT + 1];       // parts before each query tile, in order
@@ -186,10 +186,15 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
   uint8_t *base = pr_smem + ((1024 - (smem_of(pr_smem) & 1023)) & 1023);
   uint8_t *sq = base, *sk = sq + LIMBS * KB * QB, *sv = sk + KB * QB;
   float4 *sp = reinterpret_cast<float4 *>(sv + 2 * VB);  // [2][64 key pairs][2]: (ks, ks, kz, kz), (vs, vs, vz, vz)
-  const uint32_t b_k = smem_of(&bars[0]), b_v = smem_of(&bars[1]), b_s = smem_of(&bars[2]), b_p = smem_of(&bars[3]),
+  const uint32_t b_v = smem_of(&bars[1]), b_s = smem_of(&bars[2]), b_p = smem_of(&bars[3]),
                  b_o = smem_of(&bars[4]), b_c = smem_of(&bars[5]);
+  // Keys and parameters have a barrier for each parity of the tile: the code
+  // warps may be through with the next tile's before a row warp has seen this
+  // one's.  They are not through with those of the tile after: that waits for
+  // the next tile's scores, which wait for every row warp's weights of this one.
+  auto b_k = [&](uint32_t now) { return smem_of(&bars[now & 1 ? 6 : 0]); };
   if (tid == 0) {
-    bar_init(b_k, 128), bar_init(b_v, 128), bar_init(b_s, 1), bar_init(b_p, 128), bar_init(b_o, 1);
+    bar_init(b_k(0), 128), bar_init(b_k(1), 128), bar_init(b_v, 128), bar_init(b_s, 1), bar_init(b_p, 128), bar_init(b_o, 1);
     bar_init(b_c, 128);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     dead = 0;
@@ -308,7 +313,7 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
     units = all_q * a.kv_heads;
   }
 
-  uint32_t phase = 0;  // key tiles that this block has been through: one phase of every barrier each
+  uint32_t phase = 0;  // key tiles that this block has been through: one phase of every barrier each (of b_k's two in turn)
   int unit = blockIdx.x;
   while (unit < units) {
     // ---- the unit
@@ -510,7 +515,7 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
           }
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        bar_arrive(b_k);
+        bar_arrive(b_k(now));
       };
       auto store_values = [&](uint32_t now) {
 #pragma unroll
@@ -593,7 +598,7 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
         if (warp == 0) {
           // the scores take the place of the last tile's weights
           if (j > j0 && !bar_wait(b_o, parity ^ 1, &dead)) break;
-          if (!bar_wait(b_k, parity, &dead)) break;
+          if (!bar_wait(b_k(now), now >> 1 & 1, &dead)) break;
           if (lane == 0) {
             tc_after();
 #pragma unroll
@@ -607,7 +612,7 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
           __syncwarp();
         }
         // the parameters come from the code warps, the scores from the products
-        if (!bar_wait(b_k, parity, &dead) || !bar_wait(b_s, parity, &dead)) break;
+        if (!bar_wait(b_k(now), now >> 1 & 1, &dead) || !bar_wait(b_s, parity, &dead)) break;
         tc_after();
         const int rec0 = j * PR_RECS;
         // Every row sees every key of the tile: no mask.

@@ -64,3 +64,22 @@ def test_the_maximum_rises_inside_a_tile(torch, kv4, dtype, rise):
         out = w.cache.attention(q, w.batch, scale=LN2, max_new=m)
     w.check(q, out, scale=LN2)
     assert w.cache.errors() == 0
+
+
+# ---------------------------------------------------------------- hand-offs between warps
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("head_dim", [64, 128])
+def test_many_tiles_hand_over(torch, kv4, dtype, head_dim):
+    """Requests of one to many key tiles behind one another in each block, many times over: no wait runs out
+    and every call has the same bits."""
+    new = [40, 33, 300, 1, 129]
+    w = World(torch, kv4, [9000, 300, 700, 129, 129], new, 2, head_dim, 64, dtype)
+    q = w.queries(4, head_dim)
+    want = w.cache.attention(q, w.batch, max_new=300)
+    whole = w.cache.attention(q, w.batch, max_new=300, whole=True)
+    for _ in range(100):
+        assert torch.equal(w.cache.attention(q, w.batch, max_new=300), want)
+        assert torch.equal(w.cache.attention(q, w.batch, max_new=300, whole=True), whole)
+    assert w.cache.errors() == 0
+    w.check(q, want), w.check(q, whole)
