@@ -71,11 +71,12 @@ __device__ __forceinline__ bool bar_poll(uint32_t b, uint32_t parity) {
   return ok;
 }
 // Waits for the phase of that parity to complete; gives up after PR_WAIT
-// polls, or when another thread has.  A warp waits and gives up as one.
+// polls, or when another thread has.  A warp waits and gives up as one; every
+// lane has seen the phase by its own poll, which is what orders its reads.
 __device__ __forceinline__ bool bar_wait(uint32_t b, uint32_t parity, volatile int *dead) {
   for (int i = 0; i < PR_WAIT; ++i) {
     const bool ok = bar_poll(b, parity), stop = (i & 63) == 63 && *dead;
-    if (__any_sync(0xffffffffu, ok)) return true;
+    if (__all_sync(0xffffffffu, ok)) return true;
     if (__any_sync(0xffffffffu, stop)) return false;
   }
   *dead = 1;
