@@ -43,6 +43,16 @@ struct AttArgs {
   float per_warp;     // 1 / warps of the grid, rounded up
 };
 
+// A request's first row and its new tokens; 0 where its row starts do not belong
+// to this call.  Tokens past the call's rows count for its positions (the step
+// had too few rows for them), but have no row: rows_of().
+__device__ __forceinline__ int tokens_of(const AttArgs &a, int r, int &row0) {
+  row0 = __ldg(a.row_start + r);
+  const int row1 = __ldg(a.row_start + r + 1);
+  return row0 >= 0 && row0 < a.rows && row1 > row0 ? row1 - row0 : 0;
+}
+__device__ __forceinline__ int rows_of(const AttArgs &a, int row0, int n) { return n ? min(n, a.rows - row0) : 0; }
+
 // The keys that one query tile sees, as 16-key records 0 .. sink-1 and
 // lo .. hi-1.
 struct Span {
@@ -51,11 +61,12 @@ struct Span {
   int tiles;      // records in all
 };
 
-__device__ __forceinline__ Span span_of(const AttArgs &a, int len, int n, int qt_index) {
+// `n` new tokens, of which `rows` have a row.
+__device__ __forceinline__ Span span_of(const AttArgs &a, int len, int n, int rows, int qt_index) {
   Span s;
   const int first = len - n;
   s.p0 = first + qt_index * a.qt;
-  s.p1 = min(first + min((qt_index + 1) * a.qt, n), len) - 1;
+  s.p1 = min(first + min((qt_index + 1) * a.qt, rows), len) - 1;
   s.sink = s.lo = s.tiles = 0;
   if (s.p1 < 0) return s;
   const int hi = (s.p1 >> 4) + 1;
@@ -307,10 +318,11 @@ __global__ __launch_bounds__(ATT_THREADS, NT == 1 ? 2 : 1) void k_kv4_attention(
   {
     int st = 0, sq = 0, top = 1;
     for (int r = tid * per; r < min(tid * per + per, a.requests); ++r) {
-      const int row = __ldg(a.row_start + r), n = min(__ldg(a.row_start + r + 1) - row, a.rows), len = __ldg(a.length + r);
+      int row;
+      const int n = tokens_of(a, r, row), on = rows_of(a, row, n), len = __ldg(a.length + r);
       if (per == 1) req_len[r] = len, req_row[r] = row, req_n[r] = n;
-      if (n <= 0) continue;
-      const int nq = n <= a.qt ? 1 : (n + a.qt - 1) / a.qt;
+      if (n == 0) continue;
+      const int nq = on <= a.qt ? 1 : (on + a.qt - 1) / a.qt;
       const int vt = tiles_bound(a, len);
       st += nq * (vt + ATT_SETUP), sq += nq, top = max(top, vt);
     }
@@ -358,15 +370,16 @@ __global__ __launch_bounds__(ATT_THREADS, NT == 1 ? 2 : 1) void k_kv4_attention(
       const uint32_t fine = __ballot_sync(0xffffffffu, scan[seg + (lane & (ATT_THREADS / 32 - 1))] <= at);
       seg += 31 - __clz(fine & ((1u << (ATT_THREADS / 32)) - 1));
     }
-    int base = scan[seg], qbase = scan_q[seg], r = seg * per, n, len, row0, nq, vt, size;
+    int base = scan[seg], qbase = scan_q[seg], r = seg * per, n, on, len, row0, nq, vt, size;
     for (; r < a.requests; ++r) {
       if (per == 1) {
         len = req_len[r], row0 = req_row[r], n = req_n[r];
       } else {
-        len = __ldg(a.length + r), row0 = __ldg(a.row_start + r), n = min(__ldg(a.row_start + r + 1) - row0, a.rows);
+        len = __ldg(a.length + r), n = tokens_of(a, r, row0);
       }
-      if (n <= 0) continue;
-      nq = n <= a.qt ? 1 : (n + a.qt - 1) / a.qt;
+      if (n == 0) continue;
+      on = rows_of(a, row0, n);
+      nq = on <= a.qt ? 1 : (on + a.qt - 1) / a.qt;
       vt = tiles_bound(a, len);
       size = whole ? 1 : vt + ATT_SETUP;  // of one item in the row
       const int next = base + nq * a.kv_heads * size;
@@ -379,7 +392,7 @@ __global__ __launch_bounds__(ATT_THREADS, NT == 1 ? 2 : 1) void k_kv4_attention(
     // Later query tiles see more: taken from both ends in turn, so that any
     // stretch of them is about average.
     const int qi = turn & 1 ? nq - 1 - turn / 2 : turn / 2;
-    const Span s = span_of(a, len, n, qi);
+    const Span s = span_of(a, len, n, on, qi);
     int from, to, begin = 0;  // records of the item; where it begins in the row
     if (whole) {
       const int share = max((s.tiles + ATT_WARPS - 1) / ATT_WARPS, 1);
@@ -393,7 +406,7 @@ __global__ __launch_bounds__(ATT_THREADS, NT == 1 ? 2 : 1) void k_kv4_attention(
     }
     const int t_begin = min(from, s.tiles), t_end = min(to, s.tiles);
     row0 += qi * a.qt;
-    const int ncol = min(a.qt, n - qi * a.qt) * a.group;
+    const int ncol = min(a.qt, on - qi * a.qt) * a.group;
 
     // ---- this warp's records
     const int32_t *row_table = a.table + (int64_t)r * a.width;

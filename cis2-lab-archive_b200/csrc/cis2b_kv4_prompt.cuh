@@ -212,9 +212,10 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
     int sum = 0;
     {
       for (int r = tid * per; r < min(tid * per + per, a.requests); ++r) {
-        const int row = __ldg(a.row_start + r), n = max(0, min(__ldg(a.row_start + r + 1) - row, a.rows)), len = __ldg(a.length + r);
-        if (per == 1) req_len[r] = len, req_row[r] = row, req_n[r] = n;
-        sum += (n + a.qt - 1) / a.qt;
+        int row;
+        const int n = tokens_of(a, r, row);
+        if (per == 1) req_len[r] = __ldg(a.length + r), req_row[r] = row, req_n[r] = n;
+        sum += (rows_of(a, row, n) + a.qt - 1) / a.qt;
       }
       const int own = sum;
 #pragma unroll
@@ -238,7 +239,7 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(&tmem_base);
 
   struct Tile {
-    int r, len, n, row0, qi;
+    int r, len, n, rows, row0, qi;  // n new tokens, of which `rows` have a row
   };
   auto find = [&](int q) {  // query tile q of the batch
     int seg = 0;
@@ -247,23 +248,23 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
       if (scan_q[seg + step] <= q) seg += step;
     int before = scan_q[seg];
     Tile t;
-    t.len = t.n = t.row0 = 0;
+    t.len = t.n = t.rows = t.row0 = 0;
     for (t.r = seg * per; t.r < a.requests; ++t.r) {
       if (per == 1) {
         t.len = req_len[t.r], t.row0 = req_row[t.r], t.n = req_n[t.r];
       } else {
-        t.len = __ldg(a.length + t.r), t.row0 = __ldg(a.row_start + t.r);
-        t.n = max(0, min(__ldg(a.row_start + t.r + 1) - t.row0, a.rows));
+        t.len = __ldg(a.length + t.r), t.n = tokens_of(a, t.r, t.row0);
       }
-      const int nq = (t.n + a.qt - 1) / a.qt;
+      t.rows = rows_of(a, t.row0, t.n);
+      const int nq = (t.rows + a.qt - 1) / a.qt;
       if (q < before + nq) break;
       before += nq;
     }
-    if (t.r >= a.requests) t.r = 0, t.n = t.len = 0;  // row starts that do not belong together: no rows
+    if (t.r >= a.requests) t.r = 0, t.n = t.rows = t.len = 0;  // row starts that do not belong together: no rows
     t.qi = q - before;
     return t;
   };
-  auto key_tiles = [&](const Tile &t) { return (span_of(a, t.len, t.n, t.qi).tiles + PR_RECS - 1) / PR_RECS; };
+  auto key_tiles = [&](const Tile &t) { return (span_of(a, t.len, t.n, t.rows, t.qi).tiles + PR_RECS - 1) / PR_RECS; };
 
   // Up to PR_MAX_SORT query tiles are taken longest first, and the longest are
   // cut into parts of `each` key tiles where there are too few to go round.
@@ -331,10 +332,10 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
       q = all_q - 1 - ui;
     }
     const Tile t = find(q);
-    const Span s = span_of(a, t.len, t.n, t.qi);
+    const Span s = span_of(a, t.len, t.n, t.rows, t.qi);
     const int all_tiles = (s.tiles + PR_RECS - 1) / PR_RECS, share = (all_tiles + parts - 1) / parts;
     const int j0 = min(part * share, all_tiles), j1 = min(j0 + share, all_tiles);
-    const int row0 = t.row0 + t.qi * a.qt, nrow = min(a.qt, t.n - t.qi * a.qt) * a.group;
+    const int row0 = t.row0 + t.qi * a.qt, nrow = min(a.qt, t.rows - t.qi * a.qt) * a.group;
     auto key_rec = [&](int rec) { return rec < s.sink ? rec : rec - s.sink + s.lo; };
 
     // ---- queries: row = token x group + head of the group

@@ -83,3 +83,20 @@ def test_many_tiles_hand_over(torch, kv4, dtype, head_dim):
         assert torch.equal(w.cache.attention(q, w.batch, max_new=300, whole=True), whole)
     assert w.cache.errors() == 0
     w.check(q, want), w.check(q, whole)
+
+
+# ---------------------------------------------------------------- lengths and row starts
+
+@pytest.mark.parametrize("heads", [2, 16])  # one kernel or the other for the 20 rows below
+def test_a_request_that_reaches_past_the_rows(torch, kv4, heads):
+    """A step with more new tokens than rows (PLAN_ROWS): the rows that there are stand at their own
+    positions, p = length - (row_start[r + 1] - row_start[r]) + i."""
+    lengths, new = [30, 100, 9], [4, 80, 9]
+    w = World(torch, kv4, lengths, new, 1, 64, 16, "float32", rows=20)
+    q = w.queries(heads, 64)
+    for max_new in (1, 16):
+        out = w.cache.attention(q, w.batch, max_new=max_new)
+        # request 1's first 16 rows are the last of a request of 36 tokens
+        cut = plain_attention(q.double().cpu().numpy(), [w.k[0], w.k[1][:36]], [w.v[0], w.v[1][:36]], [30, 36], [4, 16], 0.125, 0, 0)
+        assert np.abs(out.double().cpu().numpy() - cut).max() <= TOL["float32"] * np.abs(w.v[1]).max()
+    assert w.cache.errors() == 0
