@@ -38,7 +38,7 @@ struct AttArgs {
   int dtype, requests, rows, width, kv_heads, group, shift, pages, window, sinks;
   int q_wide, o_wide;
   int qt;             // tokens per query tile
-  int items, whole;   // a bound on the items that may be cut; whole items per block
+  int items, whole;   // a bound on the items (query tiles x KV heads); whole items per block
   float scale;
   float per_warp;     // 1 / warps of the grid, rounded up
 };
@@ -52,6 +52,12 @@ __device__ __forceinline__ int tokens_of(const AttArgs &a, int r, int &row0) {
   return row0 >= 0 && row0 < a.rows && row1 > row0 ? row1 - row0 : 0;
 }
 __device__ __forceinline__ int rows_of(const AttArgs &a, int row0, int n) { return n ? min(n, a.rows - row0) : 0; }
+
+// Records of `keys` tokens of a request, and of all pages in its table.  A
+// length past the table counts as one record more, whose page is missing, so
+// that no caller's length can pass the 32-bit sums below or the workspace.
+__device__ __forceinline__ int records(uint32_t keys) { return (int)((keys + 15) >> 4); }
+__device__ __forceinline__ int table_records(const AttArgs &a) { return (int)((uint32_t)a.width << (a.shift - 4)); }
 
 // The keys that one query tile sees, as 16-key records 0 .. sink-1 and
 // lo .. hi-1.
@@ -69,10 +75,10 @@ __device__ __forceinline__ Span span_of(const AttArgs &a, int len, int n, int ro
   s.p1 = min(first + min((qt_index + 1) * a.qt, rows), len) - 1;
   s.sink = s.lo = s.tiles = 0;
   if (s.p1 < 0) return s;
-  const int hi = (s.p1 >> 4) + 1;
+  const int hi = min((s.p1 >> 4) + 1, table_records(a) + 1);
   if (a.window) {
-    const int lo = max(0, s.p0 - a.window + 1) >> 4;
-    const int sink = (min(a.sinks, s.p1 + 1) + 15) >> 4;
+    const int lo = min(max(0, s.p0 - a.window + 1) >> 4, hi - 1);
+    const int sink = records(min(a.sinks, s.p1 + 1));
     if (sink < lo) s.sink = sink, s.lo = lo;
   }
   s.tiles = s.sink + hi - s.lo;
@@ -82,10 +88,11 @@ __device__ __forceinline__ Span span_of(const AttArgs &a, int len, int n, int ro
 // A bound on span_of().tiles over the query tiles of a request: what each of
 // them counts as when the work is shared out.
 __device__ __forceinline__ int tiles_bound(const AttArgs &a, int len) {
-  const int all = (len + 15) >> 4;
-  if (!a.window) return max(all, 1);
-  const int some = ((min(a.sinks, len) + 15) >> 4) + ((min(a.window, len) + a.qt - 2) >> 4) + 2;
-  return max(min(all, some), 1);
+  const int all = min(records((uint32_t)max(len, 1)), table_records(a) + 1);
+  if (!a.window) return all;
+  const uint32_t keys = (uint32_t)all * 16;
+  const int some = records(min((uint32_t)a.sinks, keys)) + (int)((min((uint32_t)a.window, keys) + a.qt - 2) >> 4) + 2;
+  return min(all, some);
 }
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                          uint32_t b0, uint32_t b1) {
@@ -293,7 +300,8 @@ __global__ __launch_bounds__(ATT_THREADS, NT == 1 ? 2 : 1) void k_kv4_attention(
   // A code's operand is the code over this, of even and odd elements.
   constexpr float EVEN = EXACT ? 1.0f / 16.0f : 16777216.0f, ODD = EXACT ? 1.0f / 16.0f : 1048576.0f;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ int scan_t[ATT_THREADS], scan_q[ATT_THREADS], warp_t[ATT_WARPS], warp_q[ATT_WARPS], warp_top[ATT_WARPS];
+  __shared__ int scan_t[ATT_THREADS], scan_q[ATT_THREADS], warp_t[ATT_WARPS], warp_top[ATT_WARPS];
+  __shared__ int64_t warp_q[ATT_WARPS];
   __shared__ int req_len[ATT_THREADS], req_row[ATT_THREADS], req_n[ATT_THREADS];  // of up to as many requests
   // Each warp's cut items: one that ends in it, one that goes on after it.
   struct Cut {
@@ -314,9 +322,11 @@ __global__ __launch_bounds__(ATT_THREADS, NT == 1 ? 2 : 1) void k_kv4_attention(
   // Records (with the gaps) and items before each request: thread i sums
   // requests i * per .. of its own.
   const int per = (a.requests + ATT_THREADS - 1) / ATT_THREADS;
-  int all_tiles = 0, all_q = 0, top_tiles = 1;
+  int all_tiles = 0, top_tiles = 1;
+  int64_t all_q = 0;
   {
-    int st = 0, sq = 0, top = 1;
+    int st = 0, top = 1;
+    int64_t sq = 0;
     for (int r = tid * per; r < min(tid * per + per, a.requests); ++r) {
       int row;
       const int n = tokens_of(a, r, row), on = rows_of(a, row, n), len = __ldg(a.length + r);
@@ -326,27 +336,33 @@ __global__ __launch_bounds__(ATT_THREADS, NT == 1 ? 2 : 1) void k_kv4_attention(
       const int vt = tiles_bound(a, len);
       st += nq * (vt + ATT_SETUP), sq += nq, top = max(top, vt);
     }
-    const int own_t = st, own_q = sq;
+    const int own_t = st;
+    const int64_t own_q = sq;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-      const int x = __shfl_up_sync(0xffffffffu, st, d), y = __shfl_up_sync(0xffffffffu, sq, d);
+      const int x = __shfl_up_sync(0xffffffffu, st, d);
+      const int64_t y = __shfl_up_sync(0xffffffffu, sq, d);
       if (lane >= d) st += x, sq += y;
     }
     top = __reduce_max_sync(0xffffffffu, top);
     if (lane == 31) warp_t[warp] = st, warp_q[warp] = sq, warp_top[warp] = top;
     __syncthreads();
-    int before_t = 0, before_q = 0;
+    int before_t = 0;
+    int64_t before_q = 0;
 #pragma unroll
     for (int w = 0; w < ATT_WARPS; ++w) {
       if (w < warp) before_t += warp_t[w], before_q += warp_q[w];
       all_tiles += warp_t[w], all_q += warp_q[w], top_tiles = max(top_tiles, warp_top[w]);
     }
     scan_t[tid] = (before_t + st - own_t) * a.kv_heads;
-    scan_q[tid] = (before_q + sq - own_q) * a.kv_heads;
+    scan_q[tid] = (int)(before_q + sq - own_q) * a.kv_heads;
     __syncthreads();
   }
-  all_tiles *= a.kv_heads;
-  const int items = all_q * a.kv_heads;
+  // Requests that overlap in their rows can have more query tiles than the host
+  // counted with: such row starts have no items.
+  const bool fits = all_q * a.kv_heads <= a.items;
+  all_tiles = fits ? all_tiles * a.kv_heads : 0;
+  const int items = fits ? (int)all_q * a.kv_heads : 0;
   // A range's records: an equal share, but not so few that the joins outweigh them.
   const int range = (int)blockIdx.x * ATT_WARPS + warp;
   const int each = max(__float2int_ru(__fmul_ru(__int2float_ru(all_tiles), a.per_warp)), ATT_LEAST);
@@ -416,7 +432,7 @@ __global__ __launch_bounds__(ATT_THREADS, NT == 1 ? 2 : 1) void k_kv4_attention(
     // and all_lo .. all_hi-1.
     const int shiftr = s.sink - s.lo;
     const int all_hi = ((s.p0 + 1) >> 4) + shiftr;
-    const int all_lo = a.window ? max(s.sink, ((max(0, s.p1 - a.window + 1) + 15) >> 4) + shiftr) : 0;
+    const int all_lo = a.window ? max(s.sink, records(max(0, s.p1 - a.window + 1)) + shiftr) : 0;
     const int all_sink = min(a.window ? a.sinks >> 4 : 0, min((s.p0 + 1) >> 4, s.sink));
     // Lane i looks up record i of the next 32: its index in the pool, or NONE.
     constexpr uint32_t NONE = 0xffffffffu;
@@ -824,7 +840,7 @@ __global__ __launch_bounds__(ATT_THREADS, NT == 1 ? 2 : 1) void k_kv4_attention(
       first = (int)((uint32_t)cut.begin / (uint32_t)each) / ATT_WARPS;
       return (int)((uint32_t)(cut.begin + cut.size - 1) / (uint32_t)each) / ATT_WARPS - first + 1;
     };
-    if (tid < 2 && edge_last[tid] && edge[tid].item < a.items) {
+    if (tid < 2 && edge_last[tid]) {
       int first;
       const int parts = blocks_of(edge[tid], first);
       // One thread's fence covers the block's writes: the barrier orders them before it.
@@ -904,6 +920,7 @@ static_assert(8 + 4 * 2 * PR_BLOCKS <= WORK_PROMPT, "tickets and counters of k_k
 
 // Query columns per item: the fewest groups of 8 that hold one request's rows,
 // up to 32.
+constexpr uint64_t ITEMS_MOST = 1u << 30;  // a block's next item, its number plus the grid's, stays in 32 bits
 Shape shape_of(const cis2b_kv4_cache *c, const cis2b_kv4_attn *a) {
   Shape s;
   const int group = a->heads / c->kv_heads;
@@ -943,6 +960,8 @@ int check_attn(const cis2b_kv4_cache *c, const cis2b_kv4_attn *a) {
     return kv4_fail(CIS2B_ERR_ARG, "attention: width * page_size must be < 2^31");
   if (a->window < 0 || a->sinks < 0) return kv4_fail(CIS2B_ERR_ARG, "attention: window and sinks must be >= 0");
   if (!isfinite(a->scale)) return kv4_fail(CIS2B_ERR_ARG, "attention: scale must be finite");
+  if (shape_of(c, a).items > ITEMS_MOST)
+    return kv4_fail(CIS2B_ERR_ARG, "attention: (requests + rows) * kv_heads must be at most 2^30");
   return CIS2B_OK;
 }
 
@@ -997,7 +1016,7 @@ void fill(AttArgs &k, const cis2b_kv4_cache *c, const cis2b_kv4_attn *a, const S
   k.group = a->heads / c->kv_heads, k.pages = c->pages, k.window = a->window, k.sinks = a->sinks;
   k.shift = __builtin_ctz(c->page_size);
   k.qt = s.qt;
-  k.items = (int)std::min<uint64_t>(s.items, INT_MAX);
+  k.items = (int)s.items;
   k.scale = a->scale;
 }
 
@@ -1062,7 +1081,7 @@ extern "C" int cis2b_kv4_attention(const cis2b_kv4_cache *c, const cis2b_kv4_att
   k.counter = reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(a->work) + WORK_PROMPT);
   k.part = reinterpret_cast<float *>(static_cast<uint8_t *>(a->work) + WORK_PARTS);
   fill(k, c, a, s);
-  const uint64_t recs = ((uint64_t)a->width * c->page_size + 15) / 16;
+  const uint64_t recs = (uint64_t)a->width * c->page_size / 16 + 1;  // as tiles_bound()
   // The row of records is counted in 32 bits, and an item that is cut has a
   // counter; a batch that could pass that has items enough to take them whole.
   k.whole = (a->flags & CIS2B_KV4_WHOLE) || s.items > WORK_ITEMS || s.items * (recs + ATT_SETUP) > INT_MAX;

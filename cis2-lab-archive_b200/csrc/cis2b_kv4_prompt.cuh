@@ -171,7 +171,9 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
   constexpr uint32_t QB = PR_ROWS * 128, VB = HD * 128;  // bytes of a block of Q or K; of V
   extern __shared__ uint8_t pr_smem[];
   __shared__ __align__(8) uint64_t bars[7];
-  __shared__ int scan_q[256], req_len[256], req_row[256], req_n[256], warp_sum[8];
+  __shared__ int scan_q[256], req_len[256], req_row[256], req_n[256];
+  __shared__ int64_t warp_sum[8];
+  __shared__ unsigned long long tile_sum;
   __shared__ uint16_t order[PR_MAX_SORT], tiles_of[PR_MAX_SORT];
   __shared__ int part0[PR_MAX_SORT + 1];       // parts before each query tile, in order
   __shared__ float row_top[4];
@@ -207,9 +209,9 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
 
   // ---- query tiles before each request; what the units are
   const int per = (a.requests + 255) / 256;
-  int all_q = 0;
+  int all_q;
   {
-    int sum = 0;
+    int64_t sum = 0, all = 0;
     {
       for (int r = tid * per; r < min(tid * per + per, a.requests); ++r) {
         int row;
@@ -217,22 +219,23 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
         if (per == 1) req_len[r] = __ldg(a.length + r), req_row[r] = row, req_n[r] = n;
         sum += (rows_of(a, row, n) + a.qt - 1) / a.qt;
       }
-      const int own = sum;
+      const int64_t own = sum;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
-        const int x = __shfl_up_sync(0xffffffffu, sum, d);
+        const int64_t x = __shfl_up_sync(0xffffffffu, sum, d);
         if (lane >= d) sum += x;
       }
       if (lane == 31) warp_sum[warp] = sum;
-      scan_q[tid] = sum - own;
+      sum -= own;
     }
     __syncthreads();
-    int before = 0;
+    int64_t before = 0;
     for (int w = 0; w < 8; ++w) {
       if (w < warp) before += warp_sum[w];
-      all_q += warp_sum[w];
+      all += warp_sum[w];
     }
-    scan_q[tid] += before;
+    scan_q[tid] = (int)(before + sum);
+    all_q = all * a.kv_heads <= a.items ? (int)all : 0;  // else requests overlap in their rows: no units
     __syncthreads();
   }
   tc_after();
@@ -273,19 +276,19 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
   const bool sorted = all_q <= PR_MAX_SORT;
   int each, units;
   if (sorted) {
-    int sum = 0;
+    int sum = 0;  // two query tiles of at most 2^24 key tiles
     for (int q = tid; q < all_q; q += PR_THREADS) {
       const int n = key_tiles(find(q));
       tiles_of[q] = (uint16_t)min(n, 65535);
       sum += n;
     }
     sum = __reduce_add_sync(0xffffffffu, sum);
-    if (tid == 0) part0[0] = 0;
+    if (tid == 0) tile_sum = 0;
     __syncthreads();
-    if (lane == 0) atomicAdd(&part0[0], sum);
+    if (lane == 0) atomicAdd(&tile_sum, (unsigned long long)sum);
     __syncthreads();
-    const int64_t all = (int64_t)part0[0] * a.kv_heads;
-    each = a.whole ? INT_MAX / 2 : (int)max((int64_t)PR_LEAST, (all + gridDim.x - 1) / gridDim.x);
+    const int64_t all = (int64_t)tile_sum * a.kv_heads;
+    each = a.whole ? INT_MAX / 2 : (int)min(max((int64_t)PR_LEAST, (all + gridDim.x - 1) / gridDim.x), (int64_t)INT_MAX / 2);
     for (int q = tid; q < all_q; q += PR_THREADS) {
       int rank = 0;
       const int mine = tiles_of[q];

@@ -374,7 +374,7 @@ int cis2b_kv4_gather(const cis2b_kv4_cache *c, int32_t dtype, void *k, void *v, 
 typedef struct {
   int32_t dtype;    /* CIS2B_F32, _F16 or _BF16: q and out */
   int32_t heads;    /* a multiple of kv_heads, at most 32 times as many */
-  int32_t requests; /* >= 1 */
+  int32_t requests; /* >= 1; (requests + rows) * kv_heads <= 2^30 */
   int32_t rows;     /* rows of q and out */
   int32_t width;    /* entries per row of table */
   int32_t max_new;  /* >= 1 */

@@ -100,3 +100,57 @@ def test_a_request_that_reaches_past_the_rows(torch, kv4, heads):
         cut = plain_attention(q.double().cpu().numpy(), [w.k[0], w.k[1][:36]], [w.v[0], w.v[1][:36]], [30, 36], [4, 16], 0.125, 0, 0)
         assert np.abs(out.double().cpu().numpy() - cut).max() <= TOL["float32"] * np.abs(w.v[1]).max()
     assert w.cache.errors() == 0
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("max_new,new", [(1, [1, 1]), (3, [3, 2]), (600, [600, 500])])
+@pytest.mark.parametrize("length", [2 ** 31 - 1, 2 ** 31 - 16, 2 ** 31 - 700, 10 ** 6])
+def test_a_length_past_the_table(torch, kv4, dtype, max_new, new, length):
+    """Every key of the table is seen by every row, what is past it is reported, and with a window that
+    lies past the table nothing is seen.  The sums over so many tiles stay in range."""
+    w = World(torch, kv4, [64, 48], [1, 1], 2, 64, 16, dtype)
+    table = torch.cat([w.table[:, :3], w.table[:, :3]]).contiguous()[:2]  # three full pages each
+    n = sum(new)
+    start = torch.tensor([0, new[0], n], dtype=torch.int32, device="cuda")
+    b = kv4.Batch.of(table, torch.tensor([length, 48 + new[1]], dtype=torch.int32, device="cuda"), start, 16)
+    q = torch.randn(n, 4, 64, device="cuda", generator=torch.Generator("cuda").manual_seed(1)).to(w.dtype)
+    k, v = [w.k[0][:48], w.k[1]], [w.v[0][:48], w.v[1]]
+    out = w.cache.attention(q, b, max_new=max_new)
+    assert w.cache.errors() == kv4.BAD_PAGE
+    # all 48 keys before every row: the same as one row of a request of 48 tokens, row by row
+    rows = [0, 1, new[0] - 1, new[0], n - 1]
+    for i in rows:
+        r = int(i >= new[0])
+        want = plain_attention(q[i:i + 1].double().cpu().numpy(), [k[r]], [v[r]], [48], [1], 0.125, 0, 0)
+        assert np.abs(out[i].double().cpu().numpy() - want).max() <= TOL[dtype] * np.abs(v[r]).max(), i
+    out = w.cache.attention(q, b, max_new=max_new, window=40, sinks=0)
+    assert not out[:new[0]].any() and w.cache.errors() == kv4.BAD_PAGE
+    assert torch.equal(out, w.cache.attention(q, b, max_new=max_new, window=40, sinks=0))
+    w.cache.errors()
+    # the counters of the workspace are as they were
+    w2 = World(torch, kv4, [3000, 900], [40, 1], 2, 64, 16, dtype)
+    w2.cache._work = w.cache._work
+    q2 = w2.queries(4, 64)
+    for m in (1, 40):
+        w2.check(q2, w2.cache.attention(q2, w2.batch, max_new=m))
+
+
+@pytest.mark.parametrize("max_new", [1, 64])
+def test_requests_that_overlap_in_their_rows(torch, kv4, max_new):
+    """More query tiles than the host counts with: nothing is written outside out, and the workspace's
+    counters are as they were."""
+    n, rows = 300, 257
+    w = World(torch, kv4, [3000, 900], [40, 1], 2, 64, 16, "float32")
+    q = torch.randn(rows, 4, 64, device="cuda")
+    guard = torch.full((rows + 2, 4, 64), 3.0, device="cuda")
+    start = torch.tensor([0, 2 ** 31 - 1] * (n // 2) + [2 ** 31 - 1], dtype=torch.int32, device="cuda")
+    b = kv4.Batch.of(w.table[:1].expand(n, -1).contiguous(), torch.full((n,), 2 ** 31 - 1, dtype=torch.int32, device="cuda"), start, 16)
+    w.cache.attention(q, b, max_new=max_new, out=guard[1:-1])
+    assert (guard[0] == 3.0).all() and (guard[-1] == 3.0).all()
+    w.cache.errors()
+    q = w.queries(4, 64)
+    for m in (1, 40):
+        w.check(q, w.cache.attention(q, w.batch, max_new=m))
+    with pytest.raises(kv4.Cis2Error):  # more query tiles than can be counted
+        a = kv4._Attn(0, 2, 2 ** 30, 2 ** 30, 4, 1, 0, 0, 0.125, 0, *([256] * 2), 256, 64, 256, 64, *([256] * 4), 2 ** 60)
+        kv4._check(kv4._lib().cis2b_kv4_attention(kv4.ctypes.byref(kv4._Cache(0, 4, 16, 2, 64, 0, 256, None)), kv4.ctypes.byref(a), None))
