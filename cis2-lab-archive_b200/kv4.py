@@ -10,7 +10,9 @@ include/cis2b.h, where the format and every rule is written down).
     out = cache.attention(q, batch, window=0, sinks=0, max_new=1)
 
 Everything runs on torch's current stream and returns without waiting for
-it.  Nothing here has a gradient.  This module needs torch for its tensors;
+it.  attention keeps a workspace per stream; each call captured in a CUDA
+graph has its own, so graphs may be replayed on any streams, and beside other
+calls (not one graph beside itself).  Nothing here has a gradient.  This module needs torch for its tensors;
 the rest of the package does not.
 """
 from __future__ import annotations
@@ -74,6 +76,7 @@ def _check(rc: int) -> None:
 
 _raw_stream = torch._C._cuda_getCurrentRawStream
 _current_device = torch._C._cuda_getDevice
+_capturing = torch._C._cuda_isCurrentStreamCapturing
 
 
 def _call(device: int, fn, *args) -> None:
@@ -186,7 +189,6 @@ class Cache:
         self.status = torch.zeros(1, dtype=torch.int32, device=f"cuda:{self.device}")
         self._c.pool, self._c.status = self.pool.data_ptr(), self.status.data_ptr()
         self._work = {}   # by stream: calls on one stream follow one another
-        self._kept = []   # outgrown ones, which a captured graph may still hold
         self._calls = {}  # by shape: filled-in arguments
 
     def errors(self) -> int:
@@ -196,7 +198,7 @@ class Cache:
             self.status.zero_()
         if bits & STUCK:  # counters may have been left in the middle, on any stream
             torch.cuda.synchronize(self.device)
-            for work in [*self._work.values(), *self._kept]:
+            for work in self._work.values():
                 work[:_WORK_ZERO].zero_()
             torch.cuda.synchronize(self.device)
         return bits
@@ -258,23 +260,26 @@ class Cache:
         dev = self.device
         if q.get_device() != dev or out.get_device() != dev or batch.device != dev:
             raise ValueError(f"q, out and the batch must be on cuda:{dev}")
-        stream = _raw_stream(dev)
-        work = self._work.get(stream)
-        if work is None or work.numel() < need:
-            work = self._new_work(stream, need)
+        work = self._workspace(need)
         a.q, a.out, a.work, a.work_bytes = q.data_ptr(), out.data_ptr(), work.data_ptr(), work.numel()
         a.table, a.length, a.row_start = batch.table.data_ptr(), batch.length.data_ptr(), batch.row_start.data_ptr()
         _call(dev, _lib().cis2b_kv4_attention, self._ref, ref)
         return out
 
-    def _new_work(self, stream: int, need: int):
-        work = torch.empty(need, dtype=torch.uint8, device=f"cuda:{self.device}")
-        work[:_WORK_ZERO].zero_()
-        if torch.cuda.is_current_stream_capturing():
-            return work  # the graph's own, zeroed by each replay; not for calls outside it
-        if stream in self._work:
-            self._kept.append(self._work[stream])
-        self._work[stream] = work
+    def _workspace(self, need: int):
+        """The current stream's workspace.  A call that is captured gets one of
+        its own, zeroed by each replay: a graph may run beside this stream."""
+        dev = self.device
+        if _current_device() != dev:
+            with torch.cuda.device(dev):
+                return self._workspace(need)
+        capturing, stream = _capturing(), _raw_stream(dev)
+        work = None if capturing else self._work.get(stream)
+        if work is None or work.numel() < need:
+            work = torch.empty(need, dtype=torch.uint8, device=f"cuda:{dev}")
+            work[:_WORK_ZERO].zero_()
+            if not capturing:
+                self._work[stream] = work  # an outgrown one is free for what follows on this stream
         return work
 
     def _prepare(self, q, out, batch, scale, window, sinks, max_new, whole):

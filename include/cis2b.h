@@ -365,7 +365,8 @@ int cis2b_kv4_gather(const cis2b_kv4_cache *c, int32_t dtype, void *k, void *v, 
  *   work       cis2b_kv4_workspace() bytes or more, of which the first
  *              CIS2B_KV4_WORK_ZERO are zeroed once before the first call;
  *              then left alone: calls of other sizes may use
- *              it too, but calls that may overlap on the GPU need one each.
+ *              it too, but calls that may overlap on the GPU (replays of
+ *              captured ones among them) need one each.
  *              Zero it again after CIS2B_KV4_STUCK
  * Softmax statistics and sums are held in fp32; fp32 rows keep 22 bits of
  * every product's operands, 16-bit rows at least 11. */

@@ -154,3 +154,40 @@ def test_requests_that_overlap_in_their_rows(torch, kv4, max_new):
     with pytest.raises(kv4.Cis2Error):  # more query tiles than can be counted
         a = kv4._Attn(0, 2, 2 ** 30, 2 ** 30, 4, 1, 0, 0, 0.125, 0, *([256] * 2), 256, 64, 256, 64, *([256] * 4), 2 ** 60)
         kv4._check(kv4._lib().cis2b_kv4_attention(kv4.ctypes.byref(kv4._Cache(0, 4, 16, 2, 64, 0, 256, None)), kv4.ctypes.byref(a), None))
+
+
+# ---------------------------------------------------------------- streams and graphs
+
+@pytest.mark.parametrize("max_new", [1, 40])
+def test_graphs_run_beside_their_capture_stream(torch, kv4, max_new):
+    """Two graphs captured on a stream that has called before, replayed on two other streams beside calls
+    on the first: each has a workspace of its own."""
+    w = World(torch, kv4, [9000, 7000], [max_new, 1], 2, 64, 16, "float32")
+    q = w.queries(4, 64)
+    side, one, two = (torch.cuda.Stream() for _ in range(3))
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        want = w.cache.attention(q, w.batch, max_new=max_new)
+    torch.cuda.synchronize()
+    w.check(q, want)
+    graphs, outs = [], []
+    for _ in range(2):
+        out = torch.zeros_like(q)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            w.cache.attention(q, w.batch, max_new=max_new, out=out)
+            w.cache.attention(q, w.batch, max_new=max_new, out=out)
+        graphs.append(graph), outs.append(out)
+    torch.cuda.synchronize()
+    for _ in range(20):
+        got = []
+        for stream, graph in zip((one, two), graphs):
+            with torch.cuda.stream(stream):
+                for _ in range(5):
+                    graph.replay()
+        with torch.cuda.stream(side):
+            for _ in range(10):
+                got.append(w.cache.attention(q, w.batch, max_new=max_new))
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, want) for o in [*got, *outs])
+    assert w.cache.errors() == 0
