@@ -1020,18 +1020,18 @@ void fill(AttArgs &k, const cis2b_kv4_cache *c, const cis2b_kv4_attn *a, const S
   k.scale = a->scale;
 }
 
-template <int HD, int LIMBS, bool ROUNDED>
+template <int HD, int LIMBS>
 int launch_prompt(const PromptArgs &args, const cis2b_kv4_cache *c, uint64_t most, int sms, cudaStream_t stream) {
   static std::atomic<bool> ready[64];  // by device: the attribute is set
   const int smem = pr_smem_bytes(HD, LIMBS);
   if (!ready[c->device].load(std::memory_order_relaxed)) {
-    if (int rc = kv4_cuda(cudaFuncSetAttribute(k_kv4_prompt<HD, LIMBS, ROUNDED>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)))
+    if (int rc = kv4_cuda(cudaFuncSetAttribute(k_kv4_prompt<HD, LIMBS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)))
       return rc;
     ready[c->device].store(true, std::memory_order_relaxed);
   }
   const int per_sm = HD == 128 && LIMBS == 2 ? 1 : 2;  // as its launch bounds and shared memory allow
   const int grid = (int)std::max<uint64_t>(1, std::min<uint64_t>(most, std::min(sms * per_sm, PR_BLOCKS)));
-  k_kv4_prompt<HD, LIMBS, ROUNDED><<<grid, PR_THREADS, smem, stream>>>(args);
+  k_kv4_prompt<HD, LIMBS><<<grid, PR_THREADS, smem, stream>>>(args);
   return kv4_cuda(cudaGetLastError());
 }
 
@@ -1072,11 +1072,9 @@ extern "C" int cis2b_kv4_attention(const cis2b_kv4_cache *c, const cis2b_kv4_att
     const uint64_t tiles = ((uint64_t)a->width * c->page_size + PR_KEYS - 1) / PR_KEYS;
     const uint64_t most = s.items * ((tiles + PR_LEAST - 1) / PR_LEAST);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (a->dtype == CIS2B_BF16)
-      return c->head_dim == 64 ? launch_prompt<64, 1, true>(p, c, most, sms, st) : launch_prompt<128, 1, true>(p, c, most, sms, st);
-    if (a->dtype == CIS2B_F16)
-      return c->head_dim == 64 ? launch_prompt<64, 1, false>(p, c, most, sms, st) : launch_prompt<128, 1, false>(p, c, most, sms, st);
-    return c->head_dim == 64 ? launch_prompt<64, 2, false>(p, c, most, sms, st) : launch_prompt<128, 2, false>(p, c, most, sms, st);
+    if (a->dtype == CIS2B_F32)
+      return c->head_dim == 64 ? launch_prompt<64, 2>(p, c, most, sms, st) : launch_prompt<128, 2>(p, c, most, sms, st);
+    return c->head_dim == 64 ? launch_prompt<64, 1>(p, c, most, sms, st) : launch_prompt<128, 1>(p, c, most, sms, st);
   }
   k.counter = reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(a->work) + WORK_PROMPT);
   k.part = reinterpret_cast<float *>(static_cast<uint8_t *>(a->work) + WORK_PARTS);

@@ -31,12 +31,11 @@
 // (measured 1.5e-6 of the results without it).
 //
 // Each key's four parameters cost the row warps two 16-byte broadcasts from
-// shared memory per pair of keys, 2,048 cycles a tile (240 us where ROUNDED takes
-// 204).  ROUNDED (bf16 rows) does without: the code warps store keys and values
-// themselves, base + step * c rounded once to half precision (11 bits, where
-// the rows and the result have 8), scaled by a power of two per 32 keys that the
-// row warps take into the exponent.  A key with a NaN (or of 2^119 or more) is
-// stored as zero and noted; rows that see it become NaN.
+// shared memory per pair of keys, 2,048 cycles a tile.  bf16 rows could do
+// without where keys and values are rounded to half precision as operands
+// (measured 15 percent faster), but then a chunk of 32 keys shares one exponent:
+// a token of large values takes its neighbours' bits, and a row's result would
+// depend on tokens that it does not see.
 #pragma once
 
 constexpr int PR_ROWS = 128, PR_KEYS = 128, PR_RECS = PR_KEYS / KV4_REC;
@@ -132,17 +131,6 @@ __device__ __forceinline__ void tc_st8(uint32_t at, const uint32_t (&r)[8]) {
                "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                : "memory");
 }
-// Two codes (bits 0-3, or 4-7, of each 16-bit half) as base + step * c.
-__device__ __forceinline__ uint32_t value_low(uint32_t x, __half2 step, __half2 base) {
-  const uint32_t y = x & 0x000f000fu;
-  const __half2 v = __hfma2(*reinterpret_cast<const __half2 *>(&y), step, base);
-  return *reinterpret_cast<const uint32_t *>(&v);
-}
-__device__ __forceinline__ uint32_t value_high(uint32_t x, __half2 step16, __half2 base) {
-  const uint32_t y = x & 0x00f000f0u;
-  const __half2 v = __hfma2(*reinterpret_cast<const __half2 *>(&y), step16, base);
-  return *reinterpret_cast<const uint32_t *>(&v);
-}
 // Shared-memory operand with rows of 128 bytes in the 128-byte swizzle (16-byte
 // piece p of row r at p ^ (r & 7)), groups of 8 rows 1,024 bytes apart.
 __device__ __forceinline__ uint64_t tc_desc(uint32_t at) {
@@ -161,16 +149,15 @@ __device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, ui
                "r"(a), "l"(b), "r"(idesc), "r"((int)add) : "memory");
 }
 
-template <int HD, int LIMBS, bool ROUNDED>
+template <int HD, int LIMBS>
 __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k_kv4_prompt(PromptArgs pa) {
   const AttArgs &a = pa.a;
   constexpr int REC = kv4_rec_bytes(HD);
   constexpr int TMEM = 128 + LIMBS * HD <= 256 ? 256 : 512;  // columns: S, O of each limb
-  constexpr float P_TOP = ROUNDED ? 90.0f : 54.0f;  // log2 of the largest p that M rises to
   constexpr int KB = HD / 64;                  // 64-element column blocks of Q and K
   constexpr uint32_t QB = PR_ROWS * 128, VB = HD * 128;  // bytes of a block of Q or K; of V
   extern __shared__ uint8_t pr_smem[];
-  __shared__ __align__(8) uint64_t bars[7];
+  __shared__ __align__(8) uint64_t bars[6];
   __shared__ int scan_q[256], req_len[256], req_row[256], req_n[256];
   __shared__ int64_t warp_sum[8];
   __shared__ unsigned long long tile_sum;
@@ -181,24 +168,19 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
   __shared__ int next_unit, dead, last;
   __shared__ uint32_t held[2][PR_RECS];        // records of each tile that the pool holds
   __shared__ float value_part[2][4];           // log2 of the largest value step of each 32 keys
-  // ROUNDED: each chunk's factor of the scores and exponent of the values, and
-  // the keys with a NaN, by record.
-  __shared__ float2 chunk_scale[2][4];
-  __shared__ uint32_t bad[2][PR_RECS];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   uint8_t *base = pr_smem + ((1024 - (smem_of(pr_smem) & 1023)) & 1023);
   uint8_t *sq = base, *sk = sq + LIMBS * KB * QB, *sv = sk + KB * QB;
   float4 *sp = reinterpret_cast<float4 *>(sv + 2 * VB);  // [2][64 key pairs][2]: (ks, ks, kz, kz), (vs, vs, vz, vz)
   const uint32_t b_v = smem_of(&bars[1]), b_s = smem_of(&bars[2]), b_p = smem_of(&bars[3]),
-                 b_o = smem_of(&bars[4]), b_c = smem_of(&bars[5]);
+                 b_o = smem_of(&bars[4]);
   // Keys and parameters have a barrier for each parity of the tile: the code
   // warps may be through with the next tile's before a row warp has seen this
   // one's.  They are not through with those of the tile after: that waits for
   // the next tile's scores, which wait for every row warp's weights of this one.
-  auto b_k = [&](uint32_t now) { return smem_of(&bars[now & 1 ? 6 : 0]); };
+  auto b_k = [&](uint32_t now) { return smem_of(&bars[now & 1 ? 5 : 0]); };
   if (tid == 0) {
     bar_init(b_k(0), 128), bar_init(b_k(1), 128), bar_init(b_v, 128), bar_init(b_s, 1), bar_init(b_p, 128), bar_init(b_o, 1);
-    bar_init(b_c, 128);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     dead = 0;
   }
@@ -369,14 +351,8 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
       const float top = fmaxf(fmaxf(row_top[0], row_top[1]), fmaxf(row_top[2], row_top[3]));
       const int e2 = (int)(__float_as_uint(top) >> 23);
       const int up = e2 == 0 || e2 == 255 ? 0 : min(max(13 - (e2 - 127), -100), 100);
-      float f = __uint_as_float((uint32_t)(127 + up) << 23);
-      code_scale = sl * __uint_as_float((uint32_t)(127 - up) << 23);
-      if constexpr (ROUNDED) {  // a positive factor of the scores
-        if (!(code_scale > 0.0f)) f = code_scale < 0.0f ? -f : code_scale == 0.0f ? 0.0f : f;
-        code_scale = code_scale == 0.0f ? 1.0f : fabsf(code_scale);
-      } else {
-        code_scale *= 0.0625f;  // the codes' operands are 16 times as large
-      }
+      const float f = __uint_as_float((uint32_t)(127 + up) << 23);
+      code_scale = sl * __uint_as_float((uint32_t)(127 - up) << 23) * 0.0625f;  // the codes' operands are 16 times as large
       if (warp < 4) {
 #pragma unroll 1
         for (int d0 = 0; d0 < HD; d0 += 32) {
@@ -460,33 +436,8 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
             vw[i][k] = id == NONE ? 0u : __ldg(reinterpret_cast<const uint32_t *>(p + k * (HD / 2)));
         }
       };
-      // ROUNDED: the power of two of this warp's 32 keys (the row warps' chunk),
-      // and each key's constants as halves: step * 2^24 (a code in bits 0-3 is
-      // c 2^-24) and base of keys, of values.
-      __half *consts = reinterpret_cast<__half *>(sp);  // [2][4][128 keys]
-      auto prepare = [&](uint32_t now) {
-        const float ks = bf16_lo(par.x), kb = bf16_hi(par.x), vs = bf16_lo(par.y), vb = bf16_hi(par.y);
-        const float k_top = fmaxf(fabsf(kb), fabsf(fmaf(15.0f, ks, kb))), v_top = fmaxf(fabsf(vb), fabsf(fmaf(15.0f, vs, vb)));
-        const bool fine = ks + vs == ks + vs && k_top < 0x1p119f && v_top < 0x1p119f;
-        const uint32_t not_fine = __ballot_sync(0xffffffffu, !fine);
-        const uint32_t mk = __reduce_max_sync(0xffffffffu, fine ? __float_as_uint(k_top) : 0u);
-        const uint32_t mv = __reduce_max_sync(0xffffffffu, fine ? __float_as_uint(v_top) : 0u);
-        // The largest comes to 2^-7 .. 2^-6, so that step * 2^24 fits.
-        const int ek = mk ? max((int)(mk >> 23) - 120, -100) : 0, ev = mv ? max((int)(mv >> 23) - 120, -100) : 0;
-        const float fk = fine ? __uint_as_float((uint32_t)(127 - ek) << 23) : 0.0f;
-        const float fv = fine ? __uint_as_float((uint32_t)(127 - ev) << 23) : 0.0f;
-        __half *c = consts + (now & 1) * 512 + pt;
-        c[0] = __float2half_rn(fine ? ks * fk * 0x1p24f : 0.0f), c[128] = __float2half_rn(fine ? kb * fk : 0.0f);
-        c[256] = __float2half_rn(fine ? vs * fv * 0x1p24f : 0.0f), c[384] = __float2half_rn(fine ? vb * fv : 0.0f);
-        if (lane == 0) {
-          chunk_scale[now & 1][pw] = make_float2(code_scale * __uint_as_float((uint32_t)(127 + ek) << 23), (float)ev);
-          bad[now & 1][2 * pw] = not_fine & 0xffffu, bad[now & 1][2 * pw + 1] = not_fine >> 16;
-        }
-        bar_arrive(b_c);
-      };
       auto store_keys = [&](uint32_t now) {
         if (pw == 0 && lane < PR_RECS) held[now & 1][lane] = ids != NONE;
-        if constexpr (!ROUNDED) {
         float *dst = reinterpret_cast<float *>(sp + (now & 1) * 128 + (pt >> 1) * 2) + (pt & 1);
         const float ks = bf16_lo(par.x), vs = bf16_lo(par.y);
         dst[0] = ks * code_scale, dst[2] = fmaf(7.5f, ks, bf16_hi(par.x));
@@ -494,27 +445,15 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
         // (a step that is not a number, or zero, bounds nothing)
         const uint32_t most = __reduce_max_sync(0xffffffffu, vs == vs ? __float_as_uint(vs) : 0u);
         if (lane == 0) value_part[now & 1][pw] = lg2(__uint_as_float(most));
-        }
 #pragma unroll
         for (int i = 0; i < KN; ++i) {
           const int key = HD == 128 ? i * 32 + pw * 8 + (lane & 7) : i * 64 + pw * 16 + (lane >> 4) * 8 + (lane & 7);
           const int c = HD == 128 ? lane >> 3 : (lane >> 3) & 1;
           const uint32_t w[4] = {kw[i].x, kw[i].y, kw[i].z, kw[i].w};
-          __half2 step, step16, at_zero;
-          if constexpr (ROUNDED) {
-            step = __half2half2(consts[(now & 1) * 512 + key]), at_zero = __half2half2(consts[(now & 1) * 512 + 128 + key]);
-            step16 = __hmul2(step, __half2half2(__ushort_as_half(0x2c00)));  // 1/16
-          }
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             uint32_t v[4];  // elements 0 and 4, 1 and 5, 2 and 6, 3 and 7 of the word
-            if constexpr (ROUNDED) {
-              const uint32_t x = w[k], y = x >> 8;
-              v[0] = value_low(x, step, at_zero), v[1] = value_high(x, step16, at_zero);
-              v[2] = value_low(y, step, at_zero), v[3] = value_high(y, step16, at_zero);
-            } else {
-              codes_of<true>(w[k], v);
-            }
+            codes_of<true>(w[k], v);
             const int piece = (c & 1) * 4 + k;
             *reinterpret_cast<uint4 *>(sk + (c >> 1) * QB + key * 128 + (piece ^ (key & 7)) * 16) = make_uint4(v[0], v[1], v[2], v[3]);
           }
@@ -526,18 +465,6 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
 #pragma unroll
         for (int i = 0; i < VN; ++i) {
           const int kg = HD == 128 ? i * 8 + pw * 2 + (lane >> 4) : pw * 4 + (lane >> 3), word = lane & (HD / 8 - 1);
-          uint4 steps, bases;
-          __half2 step[4], step16[4], at_zero[4];  // of keys 2 k and 2 k + 1
-          if constexpr (ROUNDED) {
-            steps = *reinterpret_cast<const uint4 *>(consts + (now & 1) * 512 + 256 + kg * 8);
-            bases = *reinterpret_cast<const uint4 *>(consts + (now & 1) * 512 + 384 + kg * 8);
-            const uint32_t st[4] = {steps.x, steps.y, steps.z, steps.w}, ba[4] = {bases.x, bases.y, bases.z, bases.w};
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              step[k] = *reinterpret_cast<const __half2 *>(&st[k]), at_zero[k] = *reinterpret_cast<const __half2 *>(&ba[k]);
-              step16[k] = __hmul2(step[k], __half2half2(__ushort_as_half(0x2c00)));
-            }
-          }
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             uint32_t x[4];
@@ -546,15 +473,9 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
             uint32_t y[4][4];  // [element 8 word + 4 h + e][keys 2 k and 2 k + 1]
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              if constexpr (ROUNDED) {
-                const uint32_t u = x[k] >> 8;
-                y[0][k] = value_low(x[k], step[k], at_zero[k]), y[1][k] = value_high(x[k], step16[k], at_zero[k]);
-                y[2][k] = value_low(u, step[k], at_zero[k]), y[3][k] = value_high(u, step16[k], at_zero[k]);
-              } else {
-                uint32_t v[4];
-                codes_of<true>(x[k], v);
-                y[0][k] = v[0], y[1][k] = v[1], y[2][k] = v[2], y[3][k] = v[3];
-              }
+              uint32_t v[4];
+              codes_of<true>(x[k], v);
+              y[0][k] = v[0], y[1][k] = v[1], y[2][k] = v[2], y[3][k] = v[3];
             }
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -570,8 +491,7 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
       if (j0 < j1) {
         load_keys();
         load_values();
-        if constexpr (ROUNDED) prepare(phase);
-        if (!ROUNDED || bar_wait(b_c, phase & 1, &dead)) store_keys(phase);
+        store_keys(phase);
       }
       for (int j = j0; j < j1; ++j) {
         const uint32_t now = phase + (j - j0), parity = now & 1;
@@ -581,15 +501,13 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
           page_next = page_of(j + 2);
           load_keys();
         }
-        // The last tile's products are done: the values' place is free, and
-        // every warp has read the constants before last.
+        // The last tile's products are done: the values' place is free.
         if (j > j0 && !bar_wait(b_o, parity ^ 1, &dead)) break;
         store_values(now);
         if (j + 1 < j1) {
-          if constexpr (ROUNDED) prepare(now + 1);
           load_values();
           // The scores are done: the keys' place is free.
-          if (!bar_wait(b_s, parity, &dead) || (ROUNDED && !bar_wait(b_c, parity ^ 1, &dead))) break;
+          if (!bar_wait(b_s, parity, &dead)) break;
           store_keys(now + 1);
         }
       }
@@ -626,27 +544,20 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
           const int lo = key_rec(rec0) * 16, hi = key_rec(rec0 + PR_RECS - 1) * 16 + 15;
           unmasked = hi <= s.p0 && (a.window == 0 || lo > s.p1 - a.window || hi < a.sinks);
 #pragma unroll
-          for (int k = 0; k < PR_RECS; ++k) unmasked = unmasked && held[parity][k] && !(ROUNDED && bad[parity][k]);
+          for (int k = 0; k < PR_RECS; ++k) unmasked = unmasked && held[parity][k];
         }
         const float4 *params = sp + parity * 128;
         // A chunk is two records: 32 scores in; 8 words of weights (and 8 of
         // the second limb) per record out, over the record's scores.
 #pragma unroll 1
         for (int c = 0; c < PR_RECS / 2; ++c) {
-          // log2 of the chunk's largest value step (ROUNDED: the exponent of
-          // its values; its scores are `factor` times S)
-          const float lv_top = ROUNDED ? chunk_scale[parity][c].y : value_part[parity][c];
-          const float factor = ROUNDED ? chunk_scale[parity][c].x : 1.0f;
+          const float lv_top = value_part[parity][c];  // log2 of the chunk's largest value step
           uint32_t raw[32];
           tc_ld32(raw, mine + c * 32);
           tc_wait_ld32(raw);
           float2 u[16];  // scores in units of log2
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            if constexpr (ROUNDED) {
-              u[i] = make_float2(__uint_as_float(raw[2 * i]), __uint_as_float(raw[2 * i + 1]));
-              continue;
-            }
             const float4 kp = params[(c * 16 + i) * 2];
             u[i] = fma2(make_float2(__uint_as_float(raw[2 * i]), __uint_as_float(raw[2 * i + 1])), make_float2(kp.x, kp.y),
                         mul2(make_float2(kp.z, kp.w), make_float2(sum_s, sum_s)));
@@ -666,7 +577,6 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
                 const uint32_t sink = sink_i <= 0 ? 0u : sink_i > 15 ? 0xffffu : (1u << sink_i) - 1;
                 bits &= late | sink;
               }
-              if (ROUNDED && (bits & bad[parity][c * 2 + h])) l = __int_as_float(0x7fffffff);
               see |= bits << (16 * h);
             }
 #pragma unroll
@@ -678,14 +588,12 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
           float top = -INFINITY;
 #pragma unroll
           for (int i = 0; i < 16; i += 2) top = fmaxf(top, fmaxf(fmaxf(u[i].x, u[i].y), fmaxf(u[i + 1].x, u[i + 1].y)));
-          top *= factor;
-          // Weights stay below 2^14, p below 2^60 (ROUNDED, where it is only
-          // summed: 2^96); if not, M rises to 2^8 below the top.
-          const bool raise = top - M > fminf(14.0f - lv_top, P_TOP + 6.0f);
+          // Weights stay below 2^14 and p below 2^60; if not, M rises to 2^8 below the top.
+          const bool raise = top - M > fminf(14.0f - lv_top, 60.0f);
           if (__any_sync(0xffffffffu, raise)) {
             float f = 1.0f;
             if (raise) {
-              const float m = ceilf(top + fmaxf(lv_top - 8.0f, -P_TOP));
+              const float m = ceilf(top + fmaxf(lv_top - 8.0f, -54.0f));
               f = ex2(M - m);
               M = m, l *= f, z *= f;
             }
@@ -720,7 +628,7 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
             tc_wait_st();
           }
           float2 l2 = make_float2(0.0f, 0.0f), z2 = l2;
-          const float2 minus = make_float2(ROUNDED ? lv_top - M : -M, ROUNDED ? lv_top - M : -M);
+          const float2 minus = make_float2(-M, -M);
           auto weigh = [&](auto masked) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -728,12 +636,6 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
               [[maybe_unused]] uint32_t lo[8];
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
-                if constexpr (ROUNDED) {
-                  const float2 e = fma2(u[8 * h + i], make_float2(factor, factor), minus), w = make_float2(ex2(e.x), ex2(e.y));
-                  l2 = add2(l2, w);
-                  hi[i] = pack_half(w.x, w.y);
-                  continue;
-                }
                 const float2 e = add2(u[8 * h + i], minus), p = make_float2(ex2(e.x), ex2(e.y));
                 const float4 vp = params[(c * 16 + 8 * h + i) * 2 + 1];
                 float2 vs = make_float2(vp.x, vp.y), vz = make_float2(vp.z, vp.w);
@@ -753,9 +655,8 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
               if constexpr (LIMBS == 2) tc_st8(mine + c * 32 + h * 16 + 8, lo);
             }
           };
-          if (ROUNDED || unmasked) weigh(std::false_type()); else weigh(std::true_type());
-          if constexpr (ROUNDED) l += (l2.x + l2.y) * ex2(-lv_top);
-          else l += l2.x + l2.y, z += z2.x + z2.y;
+          if (unmasked) weigh(std::false_type()); else weigh(std::true_type());
+          l += l2.x + l2.y, z += z2.x + z2.y;
         }
         tc_wait_st();
         tc_before();
@@ -819,7 +720,7 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const float v = __uint_as_float(i < 4 ? x0[i * 8 + word] : x1[(i - 4) * 8 + word]);
-            y[i] = ROUNDED ? v : fmaf(v, 0.0625f, z);
+            y[i] = fmaf(v, 0.0625f, z);
           }
           const int d = 8 * (8 * b + word);
           if (parts > 1) {

@@ -191,3 +191,36 @@ def test_graphs_run_beside_their_capture_stream(torch, kv4, max_new):
         torch.cuda.synchronize()
         assert all(torch.equal(o, want) for o in [*got, *outs])
     assert w.cache.errors() == 0
+
+
+# ---------------------------------------------------------------- numbers of very different sizes
+
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_scores_that_underflow(torch, kv4, dtype, new):
+    """Queries and keys around 1e-25: every score is 0 in 32 bits, every row the mean of what it sees."""
+    w = World(torch, kv4, [150, 40], [new, 40], 1, 64, 16, dtype)
+    g = np.random.default_rng(3)
+    for r, n in enumerate(w.lengths):
+        write(torch, w, 1e-25 * g.standard_normal((n, 1, 64)), w.y[r], request=r)
+    q = (w.queries(2, 64).float() * 1e-25).to(w.dtype)
+    w.check(q, w.cache.attention(q, w.batch, max_new=40 if new > 1 else 1))
+
+
+@pytest.mark.parametrize("size", [2.0 ** 14, 2.0 ** 22])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_an_outlier_does_not_coarsen_its_neighbours(torch, kv4, dtype, size):
+    """One token in every 32 has values `size` times the others' and a score 80 powers of two below them:
+    its share of a result is at most 20 * 2^(22 - 80), so errors are relative to the others' values."""
+    d, n, m = 64, 600, 70
+    w = World(torch, kv4, [n], [m], 1, d, 16, dtype)
+    g = np.random.default_rng(4)
+    y = g.standard_normal((n, 1, d))
+    top = np.abs(stands_for(y.astype(np.float32))).max()
+    big = np.arange(n) % 32 == 9
+    y[big] *= size
+    write(torch, w, along(np.where(big, -80.0, 0.0), d), y)
+    q = torch.ones((m, 2, d), device="cuda").to(w.dtype)
+    out = w.cache.attention(q, w.batch, scale=LN2, max_new=m)
+    want = plain_attention(q.double().cpu().numpy(), w.k, w.v, [n], [m], LN2, 0, 0)
+    assert np.abs(out.double().cpu().numpy() - want).max() <= TOL[dtype] * top
