@@ -22,8 +22,10 @@
 // row's top, polling without suspension.
 //
 // M is an integer (a power of two scales exactly) and moves only when a weight
-// could pass 2^14 (by the row's top score and the largest step of 32 keys) or p
-// 2^60; then the row's weights already written, its sums and its O are scaled.
+// passes 2^14 or p 2^60; then the row's weights already written, its sums and
+// its O are scaled.  Whether one might is asked per 32 keys, by the row's top
+// score and the largest step, of tokens that it does not see too; whether and
+// how far M moves goes by the weights of the keys that it sees.
 // LIMBS = 2 (fp32 rows): two half-precision limbs of the query and of the
 // weights, twice the products.
 // The tensor cores cut off what falls below their sums, so the small limbs have
@@ -168,6 +170,7 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
   __shared__ int next_unit, dead, last;
   __shared__ uint32_t held[2][PR_RECS];        // records of each tile that the pool holds
   __shared__ float value_part[2][4];           // log2 of the largest value step of each 32 keys
+  __shared__ float4 value_log[2][PR_KEYS / 4];  // log2 of each key's
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   uint8_t *base = pr_smem + ((1024 - (smem_of(pr_smem) & 1023)) & 1023);
   uint8_t *sq = base, *sk = sq + LIMBS * KB * QB, *sv = sk + KB * QB;
@@ -442,9 +445,14 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
         const float ks = bf16_lo(par.x), vs = bf16_lo(par.y);
         dst[0] = ks * code_scale, dst[2] = fmaf(7.5f, ks, bf16_hi(par.x));
         dst[4] = vs, dst[6] = fmaf(7.5f, vs, bf16_hi(par.y));
-        // (a step that is not a number, or zero, bounds nothing)
-        const uint32_t most = __reduce_max_sync(0xffffffffu, vs == vs ? __float_as_uint(vs) : 0u);
-        if (lane == 0) value_part[now & 1][pw] = lg2(__uint_as_float(most));
+        // The largest logarithm, not that of the largest, bounds what the row
+        // warps add for each key.  Unseen keys may hold anything: NaN and
+        // negative numbers bound nothing.
+        const float log_vs = vs > 0.0f ? lg2(vs) : -INFINITY;
+        reinterpret_cast<float *>(value_log[now & 1])[pt] = log_vs;
+        int most = __float_as_int(log_vs);
+        most = __reduce_max_sync(0xffffffffu, most ^ (most >> 31 & 0x7fffffff));  // whole numbers in the order of the floats
+        if (lane == 0) value_part[now & 1][pw] = __int_as_float(most ^ (most >> 31 & 0x7fffffff));
 #pragma unroll
         for (int i = 0; i < KN; ++i) {
           const int key = HD == 128 ? i * 32 + pw * 8 + (lane & 7) : i * 64 + pw * 16 + (lane >> 4) * 8 + (lane & 7);
@@ -589,11 +597,20 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
 #pragma unroll
           for (int i = 0; i < 16; i += 2) top = fmaxf(top, fmaxf(fmaxf(u[i].x, u[i].y), fmaxf(u[i + 1].x, u[i + 1].y)));
           // Weights stay below 2^14 and p below 2^60; if not, M rises to 2^8 below the top.
-          const bool raise = top - M > fminf(14.0f - lv_top, 60.0f);
+          bool raise = fmaxf(top + lv_top - 14.0f, top - 60.0f) > M;  // might it have to
+          float w_top = -INFINITY;
+          if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+              const float4 lv = value_log[parity][c * 8 + i / 2];
+              w_top = fmaxf(fmaxf(w_top, fmaxf(u[i].x + lv.x, u[i].y + lv.y)), fmaxf(u[i + 1].x + lv.z, u[i + 1].y + lv.w));
+            }
+            raise = fmaxf(w_top - 14.0f, top - 60.0f) > M;
+          }
           if (__any_sync(0xffffffffu, raise)) {
             float f = 1.0f;
             if (raise) {
-              const float m = ceilf(top + fmaxf(lv_top - 8.0f, -54.0f));
+              const float m = ceilf(fmaxf(w_top - 8.0f, top - 54.0f));
               f = ex2(M - m);
               M = m, l *= f, z *= f;
             }

@@ -224,3 +224,76 @@ def test_an_outlier_does_not_coarsen_its_neighbours(torch, kv4, dtype, size):
     out = w.cache.attention(q, w.batch, scale=LN2, max_new=m)
     want = plain_attention(q.double().cpu().numpy(), w.k, w.v, [n], [m], LN2, 0, 0)
     assert np.abs(out.double().cpu().numpy() - want).max() <= TOL[dtype] * top
+
+
+def junk(torch, w, request, first, last, kind, seed=7):
+    """Other contents, all finite, for the tokens first .. last - 1 (slots of the request's pages)."""
+    n, (kv, d) = last - first, (w.cache.kv_heads, w.cache.head_dim)
+    if n <= 0:
+        return
+    if kind == "append":  # what an earlier request of large values leaves
+        g = np.random.default_rng(seed)
+        x = (g.standard_normal((2, n, kv, d)) * 10.0 ** g.integers(-30, 31, (2, n, 1, 1))).astype(np.float32)
+        saved = w.k[request].copy(), w.v[request].copy()
+        write(torch, w, x[0], x[1], request, first)
+        w.k[request], w.v[request] = saved
+        return
+    g = torch.Generator("cuda").manual_seed(seed)  # any bytes, as in a pool that was never set
+    pool = w.cache.pool.view(*w.cache.pool.shape[:3], 16 * (d + 8))
+    for p in range(first, last):
+        page, rec, row = int(w.table[request, p // w.page]), p % w.page // 16, p % 16
+        at = pool[page, :, rec]
+        for a, b in ((row * d // 2, d // 2), (8 * d + row * d // 2, d // 2), (16 * d + 8 * row, 8)):
+            at[:, a:a + b] = torch.randint(0, 256, (kv, b), dtype=torch.uint8, device="cuda", generator=g)
+
+
+@pytest.mark.parametrize("kind", ["append", "bytes"])
+@pytest.mark.parametrize("new", [1, 5, 90])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_what_stands_in_unseen_places_changes_no_bit(torch, kv4, dtype, new, kind):
+    """The rest of the last page, tokens before the window, and tokens after a row: whatever finite numbers
+    (or bytes) stand there, every row has the bits that it has without them."""
+    d, page, n = 64, 64, 333
+    w = World(torch, kv4, [n, 70], [new, 1], 2, d, page, dtype)
+    q = w.queries(4, d)
+    clean = w.cache.attention(q, w.batch, max_new=new)
+    w.check(q, clean)
+    windowed = w.cache.attention(q, w.batch, max_new=new, window=40, sinks=20)
+    w.check(q, windowed, window=40, sinks=20)
+    for seed in range(4):
+        junk(torch, w, 0, n, 384, kind, seed), junk(torch, w, 1, 70, 128, kind, seed)
+        assert torch.equal(w.cache.attention(q, w.batch, max_new=new), clean)
+        junk(torch, w, 0, 20, n - new - 39, kind, seed)  # the first row is at n - new
+        assert torch.equal(w.cache.attention(q, w.batch, max_new=new, window=40, sinks=20), windowed)
+        for r in range(2):  # as it was
+            write(torch, w, w.x[r], w.y[r], r)
+        if new > 1:
+            cut = new // 2  # tokens from here on are changed: the rows before are not
+            junk(torch, w, 0, n - new + cut, n, kind, seed)
+            assert torch.equal(w.cache.attention(q, w.batch, max_new=new)[:cut], clean[:cut])
+            assert torch.equal(w.cache.attention(q, w.batch, max_new=new, window=40, sinks=20)[:cut], windowed[:cut])
+            write(torch, w, w.x[0], w.y[0])
+    assert w.cache.errors() == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_later_and_lighter_tokens_of_any_size(torch, kv4, dtype):
+    """The last token of a prompt is 10^12 times the others: the rows before it are as they are without it.
+    And a token of that size that is seen, with 2^-150 of the weight, costs the rows nothing either."""
+    d, n, m = 64, 300, 120
+    w = World(torch, kv4, [n], [m], 1, d, 16, dtype)
+    y = w.y[0].copy()
+    y[n - 1] *= 1e12
+    write(torch, w, w.x[0], y)
+    q = w.queries(2, d)
+    out = w.cache.attention(q, w.batch, max_new=m)
+    want = plain_attention(q.double().cpu().numpy(), w.k, w.v, [n], [m], d ** -0.5, 0, 0)
+    top = np.abs(w.v[0][:n - 1]).max()
+    assert np.abs(out[:-1].double().cpu().numpy() - want[:-1]).max() <= TOL[dtype] * top
+    y = np.random.default_rng(8).standard_normal((n, 1, d))
+    y[7::40] *= 1e12
+    write(torch, w, along(np.where(np.arange(n) % 40 == 7, -150.0, 0.0), d), y)
+    q = torch.ones((m, 2, d), device="cuda").to(w.dtype)
+    out = w.cache.attention(q, w.batch, scale=LN2, max_new=m)
+    want = plain_attention(q.double().cpu().numpy(), w.k, w.v, [n], [m], LN2, 0, 0)
+    assert np.abs(out.double().cpu().numpy() - want).max() <= TOL[dtype] * 5
