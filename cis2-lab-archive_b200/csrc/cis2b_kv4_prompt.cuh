@@ -614,8 +614,8 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
               f = ex2(M - m);
               M = m, l *= f, z *= f;
             }
-            // What stands in TMEM: this tile's earlier weights, and O.
-            const __half2 f16 = __half2half2(__float2half_rn(f));
+            // What stands in TMEM: this tile's earlier weights, and O.  The factor
+            // may be below half precision's least where the products are not.
             tc_wait_st();  // the weights that are read back were stored asynchronously
 #pragma unroll 1
             for (int k = 0; k < 2 * c; ++k) {
@@ -623,9 +623,15 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
               if constexpr (LIMBS == 2) tc_ld16(w, mine + k * 16); else tc_ld8(w, mine + k * 16);
               tc_wait_ld();
 #pragma unroll
-              for (int i = 0; i < 8 * LIMBS; ++i) {
-                const __half2 y = __hmul2(*reinterpret_cast<const __half2 *>(&w[i]), f16);
-                w[i] = *reinterpret_cast<const uint32_t *>(&y);
+              for (int i = 0; i < 8; ++i) {
+                float2 y = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+                if constexpr (LIMBS == 2) y = add2(y, __half22float2(*reinterpret_cast<const __half2 *>(&w[8 + i])));
+                y = mul2(y, make_float2(f, f));
+                w[i] = pack_half(y.x, y.y);
+                if constexpr (LIMBS == 2) {
+                  const float2 back = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+                  w[8 + i] = pack_half(y.x - back.x, y.y - back.y);
+                }
               }
               if constexpr (LIMBS == 2) tc_st16(mine + k * 16, w); else tc_st8(mine + k * 16, w);
             }

@@ -297,3 +297,23 @@ def test_later_and_lighter_tokens_of_any_size(torch, kv4, dtype):
     out = w.cache.attention(q, w.batch, scale=LN2, max_new=m)
     want = plain_attention(q.double().cpu().numpy(), w.k, w.v, [n], [m], LN2, 0, 0)
     assert np.abs(out.double().cpu().numpy() - want).max() <= TOL[dtype] * 5
+
+
+@pytest.mark.parametrize("jump", [17.0, 19.2, 20.3, 21.0, 25.0, 33.0])
+def test_the_maximum_jumps_inside_a_tile(torch, kv4, jump):
+    """96 keys just below the bound of their weights, then one of the same tile `jump` powers of two above
+    them, where the factor for what is written is below half precision's least: their share, 96 * 2^-jump
+    of values of +-1 beside one of +-1/2, is not lost (it is up to 1.8 times the tolerance)."""
+    d, n, m = 64, 326, 70
+    w = World(torch, kv4, [n], [m], 1, d, 16, "float32")
+    t = np.full(n, -100.0)
+    t[:128] = 0.0
+    t[128:224] = 6.5
+    t[224] = 6.5 + jump
+    y = np.broadcast_to(np.where(np.arange(d) % 3 > 0, 1.0, -1.0), (n, 1, d)).astype(np.float32).copy()
+    y[224] = np.where(np.arange(d) % 2 > 0, 0.5, -0.5)
+    write(torch, w, along(t, d), y)
+    q = torch.ones((m, 2, d), device="cuda")
+    out = w.cache.attention(q, w.batch, scale=LN2, max_new=m)
+    want = plain_attention(q.double().cpu().numpy(), w.k, w.v, [n], [m], LN2, 0, 0)
+    assert np.abs(out.double().cpu().numpy() - want).max() <= TOL["float32"]
