@@ -299,6 +299,9 @@ __global__ __launch_bounds__(ATT_THREADS, NT == 1 ? 2 : 1) void k_kv4_attention(
   constexpr int PARTS = att_parts(HD, NT);
   // A code's operand is the code over this, of even and odd elements.
   constexpr float EVEN = EXACT ? 1.0f / 16.0f : 16777216.0f, ODD = EXACT ? 1.0f / 16.0f : 1048576.0f;
+  // Of the scores, it goes to the queries' factors and the keys' steps in equal
+  // shares where it is large, so that neither leaves fp32's range before the other.
+  constexpr float OF_Q = EXACT ? EVEN : 4096.0f, OF_K = EXACT ? 1.0f : 4096.0f;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int scan_t[ATT_THREADS], scan_q[ATT_THREADS], warp_t[ATT_WARPS], warp_top[ATT_WARPS];
   __shared__ int64_t warp_q[ATT_WARPS];
@@ -468,11 +471,10 @@ __global__ __launch_bounds__(ATT_THREADS, NT == 1 ? 2 : 1) void k_kv4_attention(
     // ---- query operands: lane (g, t) holds elements t HD/4 .. of column g
     uint32_t bq[NT == 1 ? LIMBS : 1][NT == 1 ? KS : 1][2];
     float2 sum_s[NT];  // sum(q) * scale * log2 e of this lane's two columns
+    float2 code_scale[NT];  // of the same columns
     int pos[NT][2];
-    float code_scale;
     {
-      float x[NT][4 * W][2];
-      float top = 0.0f;
+      float x[NT][4 * W][2], top[NT];
       const float sl = a.scale * 1.4426950408889634f;
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
@@ -491,14 +493,19 @@ __global__ __launch_bounds__(ATT_THREADS, NT == 1 ? 2 : 1) void k_kv4_attention(
             cp_async_commit();
           }
         }
+        top[j] = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8 * W; ++i) top = fmaxf(top, fabsf(e[i])), sum += e[i];
+        for (int i = 0; i < 8 * W; ++i) top[j] = fmaxf(top[j], fabsf(e[i])), sum += e[i];
         // Word w's `and`s give the code pairs (0,4) (1,5) (2,6) (3,7).
 #pragma unroll
         for (int i = 0; i < 4 * W; ++i) x[j][i][0] = e[(i & ~3) * 2 + (i & 3)], x[j][i][1] = e[(i & ~3) * 2 + (i & 3) + 4];
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        sum *= sl;
+        top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], 1));
+        top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], 2));
+        // A column with an infinity has NaN for every key that it sees (an
+        // infinite sum could be -infinity for each, which is a mask's).
+        sum = top[j] == INFINITY ? __int_as_float(0x7fffffff) : sum * sl;
         sum_s[j] = make_float2(__shfl_sync(0xffffffffu, sum, 8 * t), __shfl_sync(0xffffffffu, sum, 8 * t + 4));
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
@@ -506,16 +513,15 @@ __global__ __launch_bounds__(ATT_THREADS, NT == 1 ? 2 : 1) void k_kv4_attention(
           pos[j][c] = cc < ncol ? s.p0 + cc / a.group : -1;
         }
       }
+      // A power of two per column brings its largest element to 2^13 .. 2^14:
+      // 16-bit elements down to 2^-24 of it stay exact.
 #pragma unroll
-      for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-      // A power of two brings the largest element to 2^13 .. 2^14: 16-bit
-      // elements down to 2^-24 of it stay exact.
-      const int e = (int)(__float_as_uint(top) >> 23);  // biased exponent
-      const int up = e == 0 || e == 255 ? 0 : min(max(13 - (e - 127), -100), 100);
-      const float f = __uint_as_float((uint32_t)(127 + up) << 23), back = __uint_as_float((uint32_t)(127 - up) << 23);
-      code_scale = sl * EVEN * back;
-#pragma unroll
-      for (int j = 0; j < NT; ++j)
+      for (int j = 0; j < NT; ++j) {
+        const int e = (int)(__float_as_uint(top[j]) >> 23);  // biased exponent
+        const int up = e == 0 || e == 255 ? 0 : min(13 - (e - 127), 100);
+        const float f = __uint_as_float((uint32_t)(127 + up) << 23);
+        const float own = sl * OF_Q * __uint_as_float((uint32_t)(127 - up) << 23);
+        code_scale[j] = make_float2(__shfl_sync(0xffffffffu, own, 8 * t), __shfl_sync(0xffffffffu, own, 8 * t + 4));
 #pragma unroll
         for (int w = 0; w < W; ++w) {
           uint32_t v[LIMBS][4];
@@ -539,6 +545,7 @@ __global__ __launch_bounds__(ATT_THREADS, NT == 1 ? 2 : 1) void k_kv4_attention(
             }
           }
         }
+      }
     }
     if constexpr (NT > 1) __syncwarp();
 
@@ -620,7 +627,7 @@ __global__ __launch_bounds__(ATT_THREADS, NT == 1 ? 2 : 1) void k_kv4_attention(
       for (int i = 0; i < 2 * RP; ++i) {
         const uint8_t *rec = ring + (stage * RP + (i >> 1)) * REC;
         const uint2 p = *reinterpret_cast<const uint2 *>(rec + 16 * HD + (g + 8 * (i & 1)) * 8);
-        ks[i] = bf16_lo(p.x) * code_scale;
+        ks[i] = bf16_lo(p.x) * OF_K;
         kz[i] = EXACT ? fmaf(7.5f, bf16_lo(p.x), bf16_hi(p.x)) : bf16_hi(p.x);
         vs[i] = bf16_lo(p.y), vz[i] = fmaf(7.5f, vs[i], bf16_hi(p.y));
       }
@@ -632,7 +639,7 @@ __global__ __launch_bounds__(ATT_THREADS, NT == 1 ? 2 : 1) void k_kv4_attention(
 #pragma unroll
         for (int i = 0; i < E; ++i) {
           const float2 raw = make_float2(sc[i >> 1][j][2 * (i & 1)], sc[i >> 1][j][2 * (i & 1) + 1]);
-          tt[i] = fma2(raw, make_float2(ks[i], ks[i]), mul2(make_float2(kz[i], kz[i]), sum_s[j]));
+          tt[i] = fma2(mul2(raw, code_scale[j]), make_float2(ks[i], ks[i]), mul2(make_float2(kz[i], kz[i]), sum_s[j]));
           vse[i] = make_float2(vs[i], vs[i]), vze[i] = make_float2(vz[i], vz[i]);
         }
         if (!unmasked) {

@@ -45,6 +45,7 @@ constexpr int PR_THREADS = 256;      // warps 0-3 rows, 4-7 codes; warp 0 also i
 constexpr int PR_MAX_SORT = 512;     // query tiles whose order is chosen (longest first)
 constexpr int PR_LEAST = 16;         // least key tiles of a part
 constexpr int PR_WAIT = 1 << 20;     // polls of a barrier before the kernel gives up
+constexpr float PR_K = 0x1p-14f;     // of the keys' parameters: products with queries' operands (2^28 at most) stay in range
 
 struct PromptArgs {
   AttArgs a;
@@ -165,7 +166,6 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
   __shared__ unsigned long long tile_sum;
   __shared__ uint16_t order[PR_MAX_SORT], tiles_of[PR_MAX_SORT];
   __shared__ int part0[PR_MAX_SORT + 1];       // parts before each query tile, in order
-  __shared__ float row_top[4];
   __shared__ uint32_t tmem_base;
   __shared__ int next_unit, dead, last;
   __shared__ uint32_t held[2][PR_RECS];        // records of each tile that the pool holds
@@ -327,62 +327,65 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
     auto key_rec = [&](int rec) { return rec < s.sink ? rec : rec - s.sink + s.lo; };
 
     // ---- queries: row = token x group + head of the group
-    float sum_s = 0.0f, code_scale;
+    // A power of two per row brings its largest element to 2^13 .. 2^14.  It is
+    // divided out in the exponent: a row's scores are `factor` times S * ks +
+    // kz * sum_s.  With the scale's sign in the query and its mantissa in the keys'
+    // parameters, factor is a positive power of two, so that a score times it is
+    // the same number wherever it is formed, and -infinity stays that.
+    float sum_s = 0.0f, factor = 1.0f;
     int pos = -1;
     const float sl = a.scale * 1.4426950408889634f;
-    {
+    const uint32_t sl_bits = __float_as_uint(fabsf(sl));
+    const float key_factor = PR_K * (sl_bits >> 23 ? __uint_as_float((sl_bits & 0x7fffffu) | 0x3f800000u) : 1.0f);
+    if (warp < 4) {
       const int tok = tid / a.group;
       const int64_t row = (int64_t)row0 + tok;
       const bool on = tid < nrow && row >= 0 && row < a.rows;
       const int64_t from = row * a.q_row + (int64_t)(head * a.group + tid - tok * a.group) * a.q_head;
-      if (warp < 4) {
-        if (tid < nrow) pos = s.p0 + tok;
-        float top = 0.0f;
+      if (tid < nrow) pos = s.p0 + tok;
+      float top = 0.0f;
 #pragma unroll 1
-        for (int d = 0; d < HD; d += 32) {
-          float e[32];
-          load_query<LIMBS == 2, 32>(a.q, a.dtype == KV4_BF16, from + d, a.q_wide, on, e);
+      for (int d = 0; d < HD; d += 32) {
+        float e[32];
+        load_query<LIMBS == 2, 32>(a.q, a.dtype == KV4_BF16, from + d, a.q_wide, on, e);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) top = fmaxf(top, fabsf(e[i])), sum_s += e[i];
-        }
-        sum_s *= sl;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-        if (lane == 0) row_top[warp] = top;
+        for (int i = 0; i < 32; ++i) top = fmaxf(top, fabsf(e[i])), sum_s += e[i];
       }
-      __syncthreads();
-      const float top = fmaxf(fmaxf(row_top[0], row_top[1]), fmaxf(row_top[2], row_top[3]));
       const int e2 = (int)(__float_as_uint(top) >> 23);
-      const int up = e2 == 0 || e2 == 255 ? 0 : min(max(13 - (e2 - 127), -100), 100);
-      const float f = __uint_as_float((uint32_t)(127 + up) << 23);
-      code_scale = sl * __uint_as_float((uint32_t)(127 - up) << 23) * 0.0625f;  // the codes' operands are 16 times as large
-      if (warp < 4) {
+      const int up = e2 == 0 || e2 == 255 ? 0 : min(13 - (e2 - 127), 100);
+      float f = __uint_as_float((uint32_t)(127 + up) << 23);
+      // (codes' operands are 16 times as large)
+      factor = __uint_as_float(sl_bits & 0x7f800000u) * __uint_as_float((uint32_t)(127 - up) << 23) * (0.0625f / PR_K);
+      factor = sl == 0.0f ? 1.0f : fminf(fmaxf(factor, 0x1p-126f), 0x1p126f);
+      f = sl > 0.0f ? f : sl < 0.0f ? -f : 0.0f;
+      // A row with an infinity has NaN for every key that it sees (an infinite
+      // sum could be -infinity for each, which is a mask's).
+      sum_s = top == INFINITY ? __int_as_float(0x7fffffff) : sum_s * f * 16.0f;
 #pragma unroll 1
-        for (int d0 = 0; d0 < HD; d0 += 32) {
-          float e[32];
-          load_query<LIMBS == 2, 32>(a.q, a.dtype == KV4_BF16, from + d0, a.q_wide, on, e);
+      for (int d0 = 0; d0 < HD; d0 += 32) {
+        float e[32];
+        load_query<LIMBS == 2, 32>(a.q, a.dtype == KV4_BF16, from + d0, a.q_wide, on, e);
 #pragma unroll
-          for (int d = d0; d < d0 + 32; d += 8) {
-            uint32_t v[LIMBS][4];
+        for (int d = d0; d < d0 + 32; d += 8) {
+          uint32_t v[LIMBS][4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {  // elements i and i + 4, as a word's codes come out
-              const float y0 = e[d - d0 + i] * f, y1 = e[d - d0 + i + 4] * f;
-              v[0][i] = pack_half(y0, y1);
-              if constexpr (LIMBS == 2) {
-                const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&v[0][i]));
-                v[1][i] = pack_half(y0 - h.x, y1 - h.y);
-              }
+          for (int i = 0; i < 4; ++i) {  // elements i and i + 4, as a word's codes come out
+            const float y0 = e[d - d0 + i] * f, y1 = e[d - d0 + i + 4] * f;
+            v[0][i] = pack_half(y0, y1);
+            if constexpr (LIMBS == 2) {
+              const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&v[0][i]));
+              v[1][i] = pack_half(y0 - h.x, y1 - h.y);
             }
-#pragma unroll
-            for (int l = 0; l < LIMBS; ++l)
-              *reinterpret_cast<uint4 *>(sq + (l * KB + d / 64) * QB + tid * 128 + (((d / 8) & 7) ^ (tid & 7)) * 16) =
-                  make_uint4(v[l][0], v[l][1], v[l][2], v[l][3]);
           }
+#pragma unroll
+          for (int l = 0; l < LIMBS; ++l)
+            *reinterpret_cast<uint4 *>(sq + (l * KB + d / 64) * QB + tid * 128 + (((d / 8) & 7) ^ (tid & 7)) * 16) =
+                make_uint4(v[l][0], v[l][1], v[l][2], v[l][3]);
         }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       }
-      __syncthreads();
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
+    __syncthreads();
 
     float M = -1e30f, l = 0.0f, z = 0.0f;
     if (warp >= 4) {
@@ -443,7 +446,7 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
         if (pw == 0 && lane < PR_RECS) held[now & 1][lane] = ids != NONE;
         float *dst = reinterpret_cast<float *>(sp + (now & 1) * 128 + (pt >> 1) * 2) + (pt & 1);
         const float ks = bf16_lo(par.x), vs = bf16_lo(par.y);
-        dst[0] = ks * code_scale, dst[2] = fmaf(7.5f, ks, bf16_hi(par.x));
+        dst[0] = ks * key_factor, dst[2] = fmaf(7.5f, ks, bf16_hi(par.x)) * key_factor;
         dst[4] = vs, dst[6] = fmaf(7.5f, vs, bf16_hi(par.y));
         // The largest logarithm, not that of the largest, bounds what the row
         // warps add for each key.  Unseen keys may hold anything: NaN and
@@ -563,7 +566,7 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
           uint32_t raw[32];
           tc_ld32(raw, mine + c * 32);
           tc_wait_ld32(raw);
-          float2 u[16];  // scores in units of log2
+          float2 u[16];  // times factor: scores in units of log2
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const float4 kp = params[(c * 16 + i) * 2];
@@ -596,6 +599,7 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
           float top = -INFINITY;
 #pragma unroll
           for (int i = 0; i < 16; i += 2) top = fmaxf(top, fmaxf(fmaxf(u[i].x, u[i].y), fmaxf(u[i + 1].x, u[i + 1].y)));
+          top *= factor;
           // Weights stay below 2^14 and p below 2^60; if not, M rises to 2^8 below the top.
           bool raise = fmaxf(top + lv_top - 14.0f, top - 60.0f) > M;  // might it have to
           float w_top = -INFINITY;
@@ -603,7 +607,9 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
 #pragma unroll
             for (int i = 0; i < 16; i += 2) {
               const float4 lv = value_log[parity][c * 8 + i / 2];
-              w_top = fmaxf(fmaxf(w_top, fmaxf(u[i].x + lv.x, u[i].y + lv.y)), fmaxf(u[i + 1].x + lv.z, u[i + 1].y + lv.w));
+              const float2 fact = make_float2(factor, factor);
+              const float2 y0 = add2(mul2(u[i], fact), make_float2(lv.x, lv.y)), y1 = add2(mul2(u[i + 1], fact), make_float2(lv.z, lv.w));
+              w_top = fmaxf(fmaxf(w_top, fmaxf(y0.x, y0.y)), fmaxf(y1.x, y1.y));
             }
             raise = fmaxf(w_top - 14.0f, top - 60.0f) > M;
           }
@@ -659,7 +665,7 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
               [[maybe_unused]] uint32_t lo[8];
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
-                const float2 e = add2(u[8 * h + i], minus), p = make_float2(ex2(e.x), ex2(e.y));
+                const float2 e = fma2(u[8 * h + i], make_float2(factor, factor), minus), p = make_float2(ex2(e.x), ex2(e.y));
                 const float4 vp = params[(c * 16 + 8 * h + i) * 2 + 1];
                 float2 vs = make_float2(vp.x, vp.y), vz = make_float2(vp.z, vp.w);
                 if constexpr (decltype(masked)::value) {  // whatever the cache holds there

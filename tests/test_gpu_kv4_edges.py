@@ -317,3 +317,62 @@ def test_the_maximum_jumps_inside_a_tile(torch, kv4, jump):
     out = w.cache.attention(q, w.batch, scale=LN2, max_new=m)
     want = plain_attention(q.double().cpu().numpy(), w.k, w.v, [n], [m], LN2, 0, 0)
     assert np.abs(out.double().cpu().numpy() - want).max() <= TOL["float32"]
+
+
+@pytest.mark.parametrize("new", [1, 5, 60])
+@pytest.mark.parametrize("gain", [1e-4, 1e-5, 1e6])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_an_infinite_query_stays_in_its_row(torch, kv4, dtype, gain, new):
+    """Rows with an infinity or a NaN are NaN; the other heads and tokens of their tile, 1 / gain in size,
+    are as they are without them."""
+    if dtype == "float16" and gain == 1e-5:
+        pytest.skip("queries of 1e5 are outside half precision")
+    d = 64
+    w = World(torch, kv4, [200, 90], [new, 1], 1, d, 16, dtype)
+    for r, x in enumerate(w.x):
+        write(torch, w, x * gain, w.y[r], r)
+    q = (w.queries(4, d).float() / gain).to(w.dtype)
+    clean = w.cache.attention(q, w.batch, max_new=new)
+    w.check(q, clean)
+    bad = torch.zeros(q.shape[:2], dtype=torch.bool, device="cuda")
+    bad[0, 1] = bad[new // 2, 3] = bad[new, 0] = True
+    q[0, 1, 5], q[new // 2, 3, 60], q[new, 0, 0] = float("inf"), float("nan"), -float("inf")
+    got = w.cache.attention(q, w.batch, max_new=new)
+    assert torch.isnan(got[bad]).all() and torch.equal(got[~bad], clean[~bad])
+    # rows that see nothing are zero whatever their query is
+    got = w.cache.attention(q, kv4.Batch.of(torch.full_like(w.table, -1), w.batch.length, w.batch.row_start, 16), max_new=new)
+    assert not got.any() and w.cache.errors() == kv4.BAD_PAGE
+
+
+@pytest.mark.parametrize("new", [1, 5, 60])
+@pytest.mark.parametrize("size", [1e-30, 1e-12, 1e12, 1e30])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_a_query_of_another_size_changes_no_other_row(torch, kv4, dtype, size, new):
+    d = 64
+    w = World(torch, kv4, [200, 90], [new, 1], 1, d, 16, dtype)
+    q = w.queries(4, d)
+    clean = w.cache.attention(q, w.batch, max_new=new)
+    w.check(q, clean)
+    other = torch.zeros(q.shape[:2], dtype=torch.bool, device="cuda")
+    other[0, 1] = other[new // 2, 3] = True
+    q[other] = (q[other].float() * size).to(w.dtype)
+    got = w.cache.attention(q, w.batch, max_new=new)
+    assert torch.equal(got[~other], clean[~other]) and torch.isfinite(got).all()
+    # and the rows of that size alone, over keys that bring their scores back
+    q[~other] = 0
+    w.cache.append(*(torch.from_numpy(a).cuda() for a in ((w.x[0] / size).astype(np.float32), w.y[0])),
+                   (w.table[0, torch.arange(200, device="cuda") // 16] * 16 + torch.arange(200, device="cuda") % 16).int())
+    w.k[0] = stands_for((w.x[0] / size).astype(np.float32))
+    w.check(q, w.cache.attention(q, w.batch, max_new=new))
+
+
+@pytest.mark.parametrize("new", [1, 60])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_the_largest_queries(torch, kv4, dtype, new):
+    """Queries up to 2^121 over keys that bring their scores back."""
+    d, size = 64, 2.0 ** 119
+    w = World(torch, kv4, [200], [new], 1, d, 16, dtype)
+    write(torch, w, w.x[0] / np.float32(size), w.y[0])
+    q = (w.queries(4, d).float() * size).to(w.dtype)
+    assert torch.isfinite(q).all()
+    w.check(q, w.cache.attention(q, w.batch, max_new=new))
