@@ -148,6 +148,12 @@ __device__ __forceinline__ float lg2(float x) {
   return y;
 }
 
+// What a value's weight is bounded by: its step, and, where that is smaller by
+// OF_BASE, its base (at code 7.5).  Numbers that no caller's group has, negative
+// steps and NaN, bound nothing.
+constexpr float OF_BASE = 0x1p-80f;
+__device__ __forceinline__ float size_of(float step, float base) { return fmaxf(fmaxf(step, 0.0f), fabsf(base) * OF_BASE); }
+
 // Four elements of a column's result: numerators over the denominator (zero
 // where nothing was seen).
 __device__ __forceinline__ void emit(const AttArgs &a, int row0, int head, int col, int d, float4 x, float den) {
@@ -280,8 +286,10 @@ __host__ __device__ constexpr int att_parts(int hd, int nt) { return ATT_WARPS +
 // to the second's operand layout by an 8 x 8 register transpose.
 //
 // M is a lazy maximum per column: it moves only when a weight p * vs (the
-// number that is rounded to half precision) passes 2^14, or p passes 2^60,
-// and then to 2^8 below the top.  Weights keep 11 bits down to 2^-22 of the
+// number that is rounded to half precision) passes 2^14, or p 2^60, or p |vz|
+// 2^94 (whose sum stays in fp32: of groups of one large number, with step 0),
+// and then to 2^8 below the top.  Whether one might is asked per lane, unseen
+// keys' parameters included; the move goes by the keys that the column sees.  Weights keep 11 bits down to 2^-22 of the
 // largest; LIMBS = 2 (fp32 rows) adds a second half-precision limb to the
 // weights and the query, 22 bits.  Codes are centred at 7.5, which halves the
 // rounding's effect: directly where EXACT, else by the sum of the rounded
@@ -631,6 +639,10 @@ __global__ __launch_bounds__(ATT_THREADS, NT == 1 ? 2 : 1) void k_kv4_attention(
         kz[i] = EXACT ? fmaf(7.5f, bf16_lo(p.x), bf16_hi(p.x)) : bf16_hi(p.x);
         vs[i] = bf16_lo(p.y), vz[i] = fmaf(7.5f, vs[i], bf16_hi(p.y));
       }
+      float z_most = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 2 * RP; ++i) z_most = fmaxf(z_most, fabsf(vz[i]));
+      const float p_bound = fmaxf(0x1p-46f, z_most * OF_BASE);
       uint32_t bw[RP][NT][LIMBS][2];
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
@@ -666,27 +678,26 @@ __global__ __launch_bounds__(ATT_THREADS, NT == 1 ? 2 : 1) void k_kv4_attention(
           chk.x = fmaxf(chk.x, w[i].x), chk.y = fmaxf(chk.y, w[i].y);
           big.x = fmaxf(big.x, p[i].x), big.y = fmaxf(big.y, p[i].y);
         }
-        chk.x = fmaxf(chk.x, big.x * 0x1p-46f), chk.y = fmaxf(chk.y, big.y * 0x1p-46f);
+        chk.x = fmaxf(chk.x, big.x * p_bound), chk.y = fmaxf(chk.y, big.y * p_bound);
         if (__any_sync(0xffffffffu, fmaxf(chk.x, chk.y) > 0x1p14f)) {
           float2 tw = make_float2(-INFINITY, -INFINITY), ts = tw;
 #pragma unroll
           for (int i = 0; i < E; ++i) {
-            tw.x = fmaxf(tw.x, tt[i].x + lg2(vse[i].x)), tw.y = fmaxf(tw.y, tt[i].y + lg2(vse[i].y));
+            tw.x = fmaxf(tw.x, tt[i].x + lg2(size_of(vse[i].x, vze[i].x))), tw.y = fmaxf(tw.y, tt[i].y + lg2(size_of(vse[i].y, vze[i].y)));
             ts.x = fmaxf(ts.x, tt[i].x), ts.y = fmaxf(ts.y, tt[i].y);
           }
-          auto raise = [&](float &m, float ck, float w_top, float t_top) {  // the factor for what was summed
+          auto raise = [&](float &m, float w_top, float t_top) {  // the factor for what was summed
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) {
-              ck = fmaxf(ck, __shfl_xor_sync(0xffffffffu, ck, d));
               w_top = fmaxf(w_top, __shfl_xor_sync(0xffffffffu, w_top, d));
               t_top = fmaxf(t_top, __shfl_xor_sync(0xffffffffu, t_top, d));
             }
-            if (!(ck > 0x1p14f)) return 1.0f;
+            if (!(fmaxf(w_top - 14.0f, t_top - 60.0f) > m)) return 1.0f;
             const float before = m;
             m = fmaxf(w_top - 8.0f, t_top - 54.0f);
             return ex2(before - m);
           };
-          const float2 f = make_float2(raise(M[j].x, chk.x, tw.x, ts.x), raise(M[j].y, chk.y, tw.y, ts.y));
+          const float2 f = make_float2(raise(M[j].x, tw.x, ts.x), raise(M[j].y, tw.y, ts.y));
           l[j] = mul2(l[j], f), z[j] = mul2(z[j], f);
           ones[j][0] *= f.x, ones[j][1] *= f.y;
 #pragma unroll

@@ -22,9 +22,9 @@
 // row's top, polling without suspension.
 //
 // M is an integer (a power of two scales exactly) and moves only when a weight
-// passes 2^14 or p 2^60; then the row's weights already written, its sums and
+// passes 2^14, p 2^60 or p |vz_j| 2^94 (whose sum stays in fp32); then the row's weights already written, its sums and
 // its O are scaled.  Whether one might is asked per 32 keys, by the row's top
-// score and the largest step, of tokens that it does not see too; whether and
+// score and the largest step or base, of tokens that it does not see too; whether and
 // how far M moves goes by the weights of the keys that it sees.
 // LIMBS = 2 (fp32 rows): two half-precision limbs of the query and of the
 // weights, twice the products.
@@ -169,7 +169,7 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
   __shared__ uint32_t tmem_base;
   __shared__ int next_unit, dead, last;
   __shared__ uint32_t held[2][PR_RECS];        // records of each tile that the pool holds
-  __shared__ float value_part[2][4];           // log2 of the largest value step of each 32 keys
+  __shared__ float value_part[2][4];           // log2 of the largest value size (size_of()) of each 32 keys
   __shared__ float4 value_log[2][PR_KEYS / 4];  // log2 of each key's
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   uint8_t *base = pr_smem + ((1024 - (smem_of(pr_smem) & 1023)) & 1023);
@@ -445,15 +445,14 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
       auto store_keys = [&](uint32_t now) {
         if (pw == 0 && lane < PR_RECS) held[now & 1][lane] = ids != NONE;
         float *dst = reinterpret_cast<float *>(sp + (now & 1) * 128 + (pt >> 1) * 2) + (pt & 1);
-        const float ks = bf16_lo(par.x), vs = bf16_lo(par.y);
+        const float ks = bf16_lo(par.x), vs = bf16_lo(par.y), vz = fmaf(7.5f, vs, bf16_hi(par.y));
         dst[0] = ks * key_factor, dst[2] = fmaf(7.5f, ks, bf16_hi(par.x)) * key_factor;
-        dst[4] = vs, dst[6] = fmaf(7.5f, vs, bf16_hi(par.y));
+        dst[4] = vs, dst[6] = vz;
         // The largest logarithm, not that of the largest, bounds what the row
-        // warps add for each key.  Unseen keys may hold anything: NaN and
-        // negative numbers bound nothing.
-        const float log_vs = vs > 0.0f ? lg2(vs) : -INFINITY;
-        reinterpret_cast<float *>(value_log[now & 1])[pt] = log_vs;
-        int most = __float_as_int(log_vs);
+        // warps add for each key.
+        const float log_size = lg2(size_of(vs, vz));
+        reinterpret_cast<float *>(value_log[now & 1])[pt] = log_size;
+        int most = __float_as_int(log_size);
         most = __reduce_max_sync(0xffffffffu, most ^ (most >> 31 & 0x7fffffff));  // whole numbers in the order of the floats
         if (lane == 0) value_part[now & 1][pw] = __int_as_float(most ^ (most >> 31 & 0x7fffffff));
 #pragma unroll
@@ -562,7 +561,7 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
         // the second limb) per record out, over the record's scores.
 #pragma unroll 1
         for (int c = 0; c < PR_RECS / 2; ++c) {
-          const float lv_top = value_part[parity][c];  // log2 of the chunk's largest value step
+          const float lv_top = value_part[parity][c];  // log2 of the chunk's largest value size
           uint32_t raw[32];
           tc_ld32(raw, mine + c * 32);
           tc_wait_ld32(raw);
@@ -600,7 +599,7 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
 #pragma unroll
           for (int i = 0; i < 16; i += 2) top = fmaxf(top, fmaxf(fmaxf(u[i].x, u[i].y), fmaxf(u[i + 1].x, u[i + 1].y)));
           top *= factor;
-          // Weights stay below 2^14 and p below 2^60; if not, M rises to 2^8 below the top.
+          // Weights stay below 2^14, p below 2^60; if not, M rises to 2^8 below the top.
           bool raise = fmaxf(top + lv_top - 14.0f, top - 60.0f) > M;  // might it have to
           float w_top = -INFINITY;
           if (__any_sync(0xffffffffu, raise)) {

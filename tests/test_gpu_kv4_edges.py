@@ -376,3 +376,23 @@ def test_the_largest_queries(torch, kv4, dtype, new):
     q = (w.queries(4, d).float() * size).to(w.dtype)
     assert torch.isfinite(q).all()
     w.check(q, w.cache.attention(q, w.batch, max_new=new))
+
+
+@pytest.mark.parametrize("new", [1, 5, 60])
+@pytest.mark.parametrize("size", [1e20, 2e22, 1e27, 1e33, 2e37])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_constant_groups_of_any_size(torch, kv4, dtype, size, new):
+    """Values that are the same number in a whole group have a step of 0 and no weight but p itself; with
+    others, or alone, they come out as they are."""
+    d = 64
+    w = World(torch, kv4, [200, 90], [new, 1], 1, d, 16, dtype)
+    g = np.random.default_rng(6)
+    for every in (1, 2):  # all of them, or every other one
+        for r, n in enumerate(w.lengths):
+            y = w.y[r] * np.float32(size if every == 1 else size * 2.0 ** -60)
+            # bfloat16 numbers, so that a group's base is the value
+            y[::every] = np.float32(size) * (g.integers(1, 128, (len(range(0, n, every)), 1, 1)) / np.float32(64))
+            y = (y.view(np.uint32) & 0xffff0000).view(np.float32)
+            write(torch, w, w.x[r], y, r)
+        q = w.queries(4, d)
+        w.check(q, w.cache.attention(q, w.batch, max_new=new))
