@@ -11,6 +11,7 @@
 #include "cis2b_kv4.h"
 #include "cis2b_kv4.cuh"
 
+#include <float.h>
 #include <limits.h>
 #include <math.h>
 
@@ -25,6 +26,8 @@ constexpr int ATT_THREADS = 32 * ATT_WARPS;
 constexpr int ATT_LEAST = 8;   // least records (of 16 keys) that a warp is given
 constexpr int ATT_SETUP = 6;   // what an item's fixed costs come to, in records
 constexpr int ATT_MEET = 8;    // what joining the parts of several blocks comes to, in records
+
+constexpr float LOWEST = -FLT_MAX;  // a maximum before anything is seen: below every finite score
 
 struct AttArgs {
   const void *q;
@@ -173,7 +176,7 @@ struct Joined {
   float m, den;
 };
 __device__ __forceinline__ Joined join_parts(const float *p, int64_t stride, int n, const float *extra, int col_at, int ml_at) {
-  Joined s = {make_float4(0, 0, 0, 0), -1e30f, 0.0f};
+  Joined s = {make_float4(0, 0, 0, 0), LOWEST, 0.0f};
   const int all = n + (extra != nullptr);
   constexpr int AT_ONCE = 4;
   for (int k = 0; k < all; k += AT_ONCE) {
@@ -183,7 +186,7 @@ __device__ __forceinline__ Joined join_parts(const float *p, int64_t stride, int
 #pragma unroll
     for (int e = 0; e < AT_ONCE; ++e) {
       const float *q = k + e < n ? p + (k + e) * stride : extra;
-      ml[e] = make_float2(-1e30f, 0.0f), y[e] = make_float4(0, 0, 0, 0);
+      ml[e] = make_float2(LOWEST, 0.0f), y[e] = make_float4(0, 0, 0, 0);
       if (k + e < all) ml[e] = *reinterpret_cast<const float2 *>(q + ml_at), y[e] = *reinterpret_cast<const float4 *>(q + col_at);
     }
 #pragma unroll
@@ -567,7 +570,7 @@ __global__ __launch_bounds__(ATT_THREADS, NT == 1 ? 2 : 1) void k_kv4_attention(
         for (int i = 0; i < 4; ++i) o[j][m][i] = 0.0f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) ones[j][i] = 0.0f;
-      M[j] = make_float2(-1e30f, -1e30f), l[j] = z[j] = make_float2(0.0f, 0.0f);
+      M[j] = make_float2(LOWEST, LOWEST), l[j] = z[j] = make_float2(0.0f, 0.0f);
     }
     int stage = 0;
     for (int tile = t_begin; tile < t_end; tile += RP) {

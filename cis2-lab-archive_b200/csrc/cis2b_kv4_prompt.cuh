@@ -387,7 +387,7 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
     }
     __syncthreads();
 
-    float M = -1e30f, l = 0.0f, z = 0.0f;
+    float M = LOWEST, l = 0.0f, z = 0.0f;
     if (warp >= 4) {
       // ---- codes
       const int pt = tid - 128, pw = warp - 4;

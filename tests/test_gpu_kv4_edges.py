@@ -396,3 +396,15 @@ def test_constant_groups_of_any_size(torch, kv4, dtype, size, new):
             write(torch, w, w.x[r], y, r)
         q = w.queries(4, d)
         w.check(q, w.cache.attention(q, w.batch, max_new=new))
+
+
+@pytest.mark.parametrize("lengths,new", [([200], 1), ([6000], 1), ([200], 60), ([6000], 60)])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_scores_far_below_zero(torch, kv4, dtype, lengths, new):
+    """Every score below -10^31: the first key, whose score is the largest by far, has all the weight."""
+    d, n = 64, lengths[0]
+    w = World(torch, kv4, lengths, [new], 1, d, 16, dtype)
+    write(torch, w, along(-1e31 * (1 + np.arange(n)), d), w.y[0])
+    q = torch.ones((new, 4, d), device="cuda").to(w.dtype)
+    for whole in (False, True):
+        w.check(q, w.cache.attention(q, w.batch, scale=LN2, max_new=new, whole=whole), scale=LN2)
