@@ -80,7 +80,7 @@ __device__ __forceinline__ Span span_of(const AttArgs &a, int len, int n, int ro
   if (s.p1 < 0) return s;
   const int hi = min((s.p1 >> 4) + 1, table_records(a) + 1);
   if (a.window) {
-    const int lo = min(max(0, s.p0 - a.window + 1) >> 4, hi - 1);
+    const int lo = s.p0 < a.window ? 0 : min((s.p0 - a.window + 1) >> 4, hi - 1);
     const int sink = records(min(a.sinks, s.p1 + 1));
     if (sink < lo) s.sink = sink, s.lo = lo;
   }

@@ -408,3 +408,15 @@ def test_scores_far_below_zero(torch, kv4, dtype, lengths, new):
     q = torch.ones((new, 4, d), device="cuda").to(w.dtype)
     for whole in (False, True):
         w.check(q, w.cache.attention(q, w.batch, scale=LN2, max_new=new, whole=whole), scale=LN2)
+
+
+@pytest.mark.parametrize("max_new", [1, 4, 80])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 30, 41, 40])
+def test_windows_of_any_length_with_rows_before_the_first_token(torch, kv4, max_new, window):
+    """More new rows than tokens, so that the first stand before position 0, and a window up to the largest."""
+    w = World(torch, kv4, [40], [80], 2, 64, 16, "float32")
+    q = w.queries(4, 64)
+    out = w.cache.attention(q, w.batch, window=window, max_new=max_new)
+    assert not out[:40].any()
+    want = plain_attention(q[40:].double().cpu().numpy(), w.k, w.v, [40], [40], 0.125, 0, 0)
+    assert np.abs(out[40:].double().cpu().numpy() - want).max() <= TOL["float32"] * np.abs(w.v[0]).max()
