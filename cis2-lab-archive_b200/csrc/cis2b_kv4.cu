@@ -430,9 +430,14 @@ extern "C" int cis2b_kv4_plan(const cis2b_kv4_step *s, void *stream) {
   const PlanArgs a{s->requests, s->rows,      s->width,  shift,        s->free_count, s->cached,  s->new_tokens,
                    s->free_pages, s->table,   s->length, s->row_start, s->slot,       s->position, s->request, s->counts};
   const size_t smem = sizeof(int32_t) * 2 * ((size_t)s->requests + 1);
-  if (smem > 47 * 1024)
-    if (int rc = kv4_cuda(cudaFuncSetAttribute(k_kv4_plan, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)))
-      return rc;
+  // The limit is the kernel's, not the call's: set once, to the most that any
+  // call needs, so that no thread lowers it under another.
+  static std::atomic<bool> ready[64];  // by device
+  if (smem > 47 * 1024 && !ready[s->device].load(std::memory_order_relaxed)) {
+    const int most = (int)(sizeof(int32_t) * 2 * (PLAN_MAX_REQUESTS + 1));
+    if (int rc = kv4_cuda(cudaFuncSetAttribute(k_kv4_plan, cudaFuncAttributeMaxDynamicSharedMemorySize, most))) return rc;
+    ready[s->device].store(true, std::memory_order_relaxed);
+  }
   const int grid = std::max(1, std::min(sms, (s->rows + PLAN_THREADS - 1) / PLAN_THREADS));
   k_kv4_plan<<<grid, PLAN_THREADS, smem, static_cast<cudaStream_t>(stream)>>>(a);
   return kv4_cuda(cudaGetLastError());

@@ -420,3 +420,57 @@ def test_windows_of_any_length_with_rows_before_the_first_token(torch, kv4, max_
     assert not out[:40].any()
     want = plain_attention(q[40:].double().cpu().numpy(), w.k, w.v, [40], [40], 0.125, 0, 0)
     assert np.abs(out[40:].double().cpu().numpy() - want).max() <= TOL["float32"] * np.abs(w.v[0]).max()
+
+
+# ---------------------------------------------------------------- planning
+
+def plan_case(torch, kv4, requests):
+    """A batch of many requests, its inputs, and what it has to give (by prefix sums)."""
+    g = np.random.default_rng(requests)
+    page, width = 16, 4
+    cached, new = g.integers(0, 40, requests), g.integers(0, 3, requests)
+    have, need = -(-cached // page), -(-(cached + new) // page)
+    i32 = lambda x: torch.tensor(np.asarray(x), dtype=torch.int32, device="cuda")  # noqa: E731
+    batch = kv4.Batch(requests, int(new.sum()), width, page, table=i32(np.arange(requests * width).reshape(-1, width)))
+    row = np.concatenate([[0], np.cumsum(new)])
+    first = np.concatenate([[0], np.cumsum(need - have)])
+    req = np.repeat(np.arange(requests), new)
+    pos = cached[req] + np.arange(row[-1]) - row[req]
+    col = pos // page
+    fresh = col >= have[req]
+    page_of = np.where(fresh, 10 ** 6 + first[req] + col - have[req], req * width + col)
+    want = dict(row_start=row, request=req, position=pos, slot=page_of * page + pos % page)
+    free = i32(10 ** 6 + np.arange(first[-1]))
+    return batch, (i32(cached), i32(new), free), want, [int(row[-1]), int(first[-1]), 0, 0]
+
+
+@pytest.mark.parametrize("requests", [6013, 6014, 6016, 12000, 16384])
+def test_plan_of_many_requests(torch, kv4, requests):
+    batch, args, want, counts = plan_case(torch, kv4, requests)
+    batch.plan(*args)
+    assert batch.counts.tolist() == counts
+    for name, x in want.items():
+        assert np.array_equal(getattr(batch, name).cpu().numpy(), x), name
+
+
+def test_plans_of_two_threads(torch, kv4):
+    """Batches of different sizes planned by two threads at once: neither takes the other's shared memory away."""
+    import threading
+    errors = []
+
+    def plan(requests, stream):
+        try:
+            with torch.cuda.stream(stream):
+                batch, args, want, _ = plan_case(torch, kv4, requests)
+                for _ in range(4000):
+                    batch.plan(*args)
+                assert np.array_equal(batch.slot.cpu().numpy(), want["slot"])
+        except Exception as e:  # noqa: BLE001 -- of another thread
+            errors.append(e)
+
+    threads = [threading.Thread(target=plan, args=(n, torch.cuda.Stream())) for n in (16384, 6100, 9000)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
