@@ -10,15 +10,17 @@ include/cis2b.h, where the format and every rule is written down).
     out = cache.attention(q, batch, window=0, sinks=0, max_new=1)
 
 Everything runs on torch's current stream and returns without waiting for
-it.  attention keeps a workspace per stream; each call captured in a CUDA
-graph has its own, so graphs may be replayed on any streams, and beside other
-calls (not one graph beside itself).  Nothing here has a gradient.  This module needs torch for its tensors;
-the rest of the package does not.
+it.  attention keeps a workspace per stream, which the caches of a device
+share; each call captured in a CUDA graph has its own, so graphs may be
+replayed on any streams, and beside other calls (not one graph beside itself).
+Nothing here has a gradient.  This module needs torch for its tensors; the
+rest of the package does not.
 """
 from __future__ import annotations
 
 import ctypes
 import importlib
+import weakref
 
 import torch
 
@@ -166,6 +168,14 @@ class Batch:
         return int(self.counts[2].item())
 
 
+class _Workspaces(dict):
+    """A device's workspaces, by stream: calls on one stream follow one another,
+    whichever layer's cache they are of.  Kept by the caches of the device."""
+
+
+_workspaces = weakref.WeakValueDictionary()  # by device
+
+
 class Cache:
     """One layer's keys and values in 4 bits: a pool of pages on the device.
     Like a model handle, it belongs to one thread at a time.
@@ -188,7 +198,7 @@ class Cache:
         self.page_size, self.kv_heads, self.head_dim = page_size, kv_heads, head_dim
         self.status = torch.zeros(1, dtype=torch.int32, device=f"cuda:{self.device}")
         self._c.pool, self._c.status = self.pool.data_ptr(), self.status.data_ptr()
-        self._work = {}   # by stream: calls on one stream follow one another
+        self._work = _workspaces.setdefault(self.device, _Workspaces())
         self._calls = {}  # by shape: filled-in arguments
 
     def errors(self) -> int:
@@ -198,7 +208,7 @@ class Cache:
             self.status.zero_()
         if bits & STUCK:  # counters may have been left in the middle, on any stream
             torch.cuda.synchronize(self.device)
-            for work in self._work.values():
+            for work in list(self._work.values()):
                 work[:_WORK_ZERO].zero_()
             torch.cuda.synchronize(self.device)
         return bits

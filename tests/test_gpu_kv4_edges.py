@@ -474,3 +474,31 @@ def test_plans_of_two_threads(torch, kv4):
     for t in threads:
         t.join()
     assert not errors
+
+
+# ---------------------------------------------------------------- what a user holds
+
+def test_layers_share_a_workspace(torch, kv4):
+    """The caches of a model's layers hold one workspace per stream between them, and none once they are gone."""
+    import gc
+    n = 12
+    worlds = [World(torch, kv4, [2000 + 100 * i], [40], 2, 128, 64, "bfloat16", seed=i) for i in range(n)]
+    qs = [w.queries(8, 128) for w in worlds]
+    torch.cuda.synchronize()
+    gc.collect()
+    before = torch.cuda.memory_allocated()
+    outs = [[torch.empty_like(q) for q in qs] for _ in range(2)]
+    held = sum(o.numel() * o.element_size() for o in outs[0] + outs[1])
+    for m, some in zip((1, 40), outs):  # each kernel, the layers one after another
+        for w, q, out in zip(worlds, qs, some):
+            w.cache.attention(q, w.batch, max_new=m, out=out)
+    after = torch.cuda.memory_allocated()
+    assert len({id(w.cache._work) for w in worlds}) == 1
+    largest = max(work.numel() for work in worlds[0].cache._work.values())
+    assert after - before <= held + 1.1 * largest + (1 << 20)
+    for w, q, a, b in zip(worlds, qs, *outs):
+        w.check(q, a), w.check(q, b)
+        assert w.cache.errors() == 0
+    del w, worlds
+    gc.collect()
+    assert not kv4._workspaces.get(torch.cuda.current_device())
