@@ -251,8 +251,10 @@ class Cache:
         the cache; their own keys and values are appended before.  With
         window > 0 a row sees its last `window` keys and the first `sinks`.
         max_new is the most rows that one request has in this step (a bound
-        will do; it only chooses the kernel).  whole: a request's result does
-        not depend on the rest of the batch (slower over long requests).
+        will do; it only chooses the kernel).  If None, a batch with no more
+        rows than requests is taken to have one each, any other may have all
+        rows in one request.  whole: a request's result does not depend on the
+        rest of the batch, given the same max_new (slower over long requests).
         Returns out (made if None)."""
         if q.requires_grad and torch.is_grad_enabled():
             raise ValueError("attention over the 4-bit cache has no gradient")
@@ -304,8 +306,10 @@ class Cache:
         if batch.page_size != self.page_size:
             raise ValueError(f"the batch was made for pages of {batch.page_size} tokens, not {self.page_size}")
         rows, heads = q.shape[0], q.shape[1]
+        if max_new is None:
+            max_new = 1 if rows <= batch.table.shape[0] else rows
         a = _Attn(_DTYPES[q.dtype], heads, batch.table.shape[0], rows, batch.table.shape[1],
-                  max(1, rows if max_new is None else max_new), window, sinks,
+                  max(1, max_new), window, sinks,
                   self.head_dim ** -0.5 if scale is None else scale, int(whole), None, None, q.stride(0), q.stride(1),
                   out.stride(0), out.stride(1), None, None, None, None, 0)
         need = _U64()

@@ -502,3 +502,22 @@ def test_layers_share_a_workspace(torch, kv4):
     del w, worlds
     gc.collect()
     assert not kv4._workspaces.get(torch.cuda.current_device())
+
+
+# ---------------------------------------------------------------- arguments
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_decode_batch_takes_the_one_row_kernel_by_itself(torch, kv4, dtype):
+    """Without max_new, a batch with no more rows than requests is taken for decode: the bits of max_new=1."""
+    lengths = list(range(20, 660, 40))
+    w = World(torch, kv4, lengths, [1] * len(lengths), 2, 64, 16, dtype)
+    q = w.queries(16, 64)
+    out = w.cache.attention(q, w.batch)
+    w.check(q, out)
+    assert torch.equal(out, w.cache.attention(q, w.batch, max_new=1))
+    assert not torch.equal(out, w.cache.attention(q, w.batch, max_new=len(lengths)))  # the other kernel's
+    # and one request with all the rows of such a batch is still right
+    w = World(torch, kv4, [500, 9, 9, 9], [4, 0, 0, 0], 2, 64, 16, dtype)
+    q = w.queries(16, 64)
+    w.check(q, w.cache.attention(q, w.batch))
+    assert torch.equal(w.cache.attention(q, w.batch, max_new=0), w.cache.attention(q, w.batch, max_new=1))
