@@ -108,6 +108,13 @@ def _ints(t, name: str, device: int, shape: tuple | None = None):
     return t
 
 
+def _int32(*named) -> None:
+    """Refuses numbers that a field of 32 bits would cut: (name, number) pairs."""
+    for name, x in named:
+        if not -2 ** 31 <= x < 2 ** 31:
+            raise ValueError(f"{name} must fit in 32 bits, not {x}")
+
+
 class Batch:
     """One step's block tables and slot maps, shared by every layer's cache.
 
@@ -119,6 +126,7 @@ class Batch:
     def __init__(self, requests: int, tokens: int, width: int, page_size: int, table=None, device="cuda"):
         if requests < 1 or tokens < 0 or width < 1:
             raise ValueError("requests and width must be >= 1 and tokens >= 0")
+        _int32(("requests", requests), ("tokens", tokens), ("width", width), ("page_size", page_size))
         self.device = _device_index(device if table is None else table.device)
         self.page_size = page_size
 
@@ -160,6 +168,7 @@ class Batch:
         dev, n = self.device, s.requests
         _ints(cached, "cached", dev, (n,)), _ints(new, "new", dev, (n,)), _ints(free_pages, "free_pages", dev)
         s.cached, s.new_tokens = cached.data_ptr(), new.data_ptr()
+        _int32(("the number of free pages", free_pages.numel()))
         s.free_pages, s.free_count = free_pages.data_ptr(), free_pages.numel()
         _call(dev, _lib().cis2b_kv4_plan, self._ref)
 
@@ -185,6 +194,7 @@ class Cache:
 
     def __init__(self, pages: int, page_size: int, kv_heads: int, head_dim: int, pool=None, device="cuda"):
         self.device = _device_index(device if pool is None else pool.device)
+        _int32(("pages", pages), ("page_size", page_size), ("kv_heads", kv_heads), ("head_dim", head_dim))
         self._c = _Cache(self.device, pages, page_size, kv_heads, head_dim, 0, None, None)
         self._ref = ctypes.byref(self._c)
         size = _U64()
@@ -306,10 +316,11 @@ class Cache:
         if batch.page_size != self.page_size:
             raise ValueError(f"the batch was made for pages of {batch.page_size} tokens, not {self.page_size}")
         rows, heads = q.shape[0], q.shape[1]
+        _int32(("window", window), ("sinks", sinks))
         if max_new is None:
             max_new = 1 if rows <= batch.table.shape[0] else rows
         a = _Attn(_DTYPES[q.dtype], heads, batch.table.shape[0], rows, batch.table.shape[1],
-                  max(1, max_new), window, sinks,
+                  min(max(1, max_new), 2 ** 31 - 1), window, sinks,
                   self.head_dim ** -0.5 if scale is None else scale, int(whole), None, None, q.stride(0), q.stride(1),
                   out.stride(0), out.stride(1), None, None, None, None, 0)
         need = _U64()

@@ -521,3 +521,19 @@ def test_a_decode_batch_takes_the_one_row_kernel_by_itself(torch, kv4, dtype):
     q = w.queries(16, 64)
     w.check(q, w.cache.attention(q, w.batch))
     assert torch.equal(w.cache.attention(q, w.batch, max_new=0), w.cache.attention(q, w.batch, max_new=1))
+
+
+def test_numbers_past_32_bits_are_refused(torch, kv4):
+    w = World(torch, kv4, [100], [1], 1, 64, 16, "float32")
+    q = w.queries(2, 64)
+    want = w.cache.attention(q, w.batch)
+    for kw in [dict(window=2 ** 32 + 5), dict(window=2 ** 31), dict(window=5, sinks=2 ** 32), dict(sinks=-2 ** 40)]:
+        with pytest.raises(ValueError):
+            w.cache.attention(q, w.batch, **kw)
+    w.check(q, w.cache.attention(q, w.batch, max_new=2 ** 32 + 1))  # a bound may be anything
+    for args in [(2 ** 32 + 4, 16, 1, 64), (4, 2 ** 32 + 16, 1, 64), (4, 16, 2 ** 32 + 1, 64), (4, 16, 1, 2 ** 32 + 64)]:
+        with pytest.raises(ValueError):
+            kv4.Cache(*args)
+    with pytest.raises(ValueError):
+        kv4.Batch(1, 4, 4, 2 ** 32 + 16)
+    assert torch.equal(w.cache.attention(q, w.batch, window=0), want)

@@ -79,3 +79,10 @@ def test_bad_attention_calls_are_refused(kv4, field, value):
 def test_batches_live_on_the_gpu(kv4):
     with pytest.raises(ValueError):
         kv4.Batch(1, 1, 1, 16, device="cpu")
+
+
+def test_sizes_past_32_bits_are_refused(kv4):
+    """A field of 32 bits would take 2^32 + 4 for 4."""
+    for args in [(2 ** 32 + 4, 16, 1, 64), (4, 2 ** 32 + 16, 1, 64), (4, 16, 2 ** 32 + 1, 64), (4, 16, 1, 2 ** 32 + 64)]:
+        with pytest.raises(ValueError):
+            kv4.Cache(*args, device="cuda:0")
