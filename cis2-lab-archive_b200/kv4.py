@@ -174,6 +174,7 @@ class Batch:
 
     def errors(self) -> int:
         """PLAN_* bits of the last plan, 0 if all is well.  Waits for the GPU."""
+        torch.cuda.synchronize(self.device)  # on whichever stream it was
         return int(self.counts[2].item())
 
 
@@ -213,13 +214,13 @@ class Cache:
 
     def errors(self) -> int:
         """BAD_* and STUCK bits that calls have left since the last time, 0 if all is well.  Waits for the GPU."""
+        torch.cuda.synchronize(self.device)  # calls may be on any stream, and those that follow too
         bits = int(self.status.item())
         if bits:
             self.status.zero_()
-        if bits & STUCK:  # counters may have been left in the middle, on any stream
-            torch.cuda.synchronize(self.device)
-            for work in list(self._work.values()):
-                work[:_WORK_ZERO].zero_()
+            if bits & STUCK:  # counters may have been left in the middle
+                for work in list(self._work.values()):
+                    work[:_WORK_ZERO].zero_()
             torch.cuda.synchronize(self.device)
         return bits
 

@@ -537,3 +537,29 @@ def test_numbers_past_32_bits_are_refused(torch, kv4):
     with pytest.raises(ValueError):
         kv4.Batch(1, 4, 4, 2 ** 32 + 16)
     assert torch.equal(w.cache.attention(q, w.batch, window=0), want)
+
+
+def test_errors_waits_for_every_stream(torch, kv4):
+    """errors() of calls that still run on another stream, and of one that follows it there."""
+    cache = kv4.Cache(2, 16, 1, 64)
+    x = torch.randn(1, 1, 64, device="cuda")
+    bad = torch.tensor([10 ** 6], dtype=torch.int32, device="cuda")
+    batch = kv4.Batch(1, 4, 1, 16)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    args = i32(0), i32(17), i32(0, 1)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(20_000_000)  # about 10 ms
+            cache.append(x, x, bad)
+            batch.plan(*args)
+        assert cache.errors() == kv4.BAD_SLOT
+        with torch.cuda.stream(side):
+            cache.append(x, x, bad)  # not wiped by the read before
+        assert cache.errors() == kv4.BAD_SLOT and cache.errors() == 0
+        with torch.cuda.stream(side):
+            batch.counts.fill_(0)
+            torch.cuda._sleep(20_000_000)
+            batch.plan(*args)
+        assert batch.errors() == kv4.PLAN_WIDTH | kv4.PLAN_ROWS
