@@ -52,7 +52,6 @@ struct PromptArgs {
   float *part;        // [units that are parts][128 rows][HD], then (M, l) [128]
   uint32_t *counter;  // [query tiles that may be cut][kv_heads]
   uint32_t *ticket;   // next unit; blocks that are done
-  int slots;          // parts that the workspace holds
 };
 
 __host__ __device__ constexpr int pr_smem_bytes(int hd, int limbs) {
