@@ -159,7 +159,7 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
   constexpr int KB = HD / 64;                  // 64-element column blocks of Q and K
   constexpr uint32_t QB = PR_ROWS * 128, VB = HD * 128;  // bytes of a block of Q or K; of V
   extern __shared__ uint8_t pr_smem[];
-  __shared__ __align__(8) uint64_t bars[6];
+  __shared__ __align__(8) uint64_t bars[7];
   __shared__ int scan_q[256], req_len[256], req_row[256], req_n[256];
   __shared__ int64_t warp_sum[8];
   __shared__ unsigned long long tile_sum;
@@ -175,14 +175,14 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
   uint8_t *sq = base, *sk = sq + LIMBS * KB * QB, *sv = sk + KB * QB;
   float4 *sp = reinterpret_cast<float4 *>(sv + 2 * VB);  // [2][64 key pairs][2]: (ks, ks, kz, kz), (vs, vs, vz, vz)
   const uint32_t b_v = smem_of(&bars[1]), b_s = smem_of(&bars[2]), b_p = smem_of(&bars[3]),
-                 b_o = smem_of(&bars[4]);
+                 b_o = smem_of(&bars[4]), b_end = smem_of(&bars[6]);
   // Keys and parameters have a barrier for each parity of the tile: the code
   // warps may be through with the next tile's before a row warp has seen this
   // one's.  They are not through with those of the tile after: that waits for
   // the next tile's scores, which wait for every row warp's weights of this one.
   auto b_k = [&](uint32_t now) { return smem_of(&bars[now & 1 ? 5 : 0]); };
   if (tid == 0) {
-    bar_init(b_k(0), 128), bar_init(b_k(1), 128), bar_init(b_v, 128), bar_init(b_s, 1), bar_init(b_p, 128), bar_init(b_o, 1);
+    bar_init(b_k(0), 128), bar_init(b_k(1), 128), bar_init(b_v, 128), bar_init(b_s, 1), bar_init(b_p, 128), bar_init(b_o, 1), bar_init(b_end, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     dead = 0;
   }
@@ -793,6 +793,12 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
   }
 
   // ---- the last block out leaves the tickets as it found them
+  __syncthreads();
+  if (dead && warp == 0) {  // products may be under way: tensor memory is theirs until they are done
+    if (lane == 0) tc_commit(b_end);
+    __syncwarp();
+    for (int i = 0; i < PR_WAIT && !__all_sync(0xffffffffu, bar_poll(b_end, 0)); ++i) {}
+  }
   __syncthreads();
   if (tid == 0) {
     if (dead && a.status) atomicOr(a.status, CIS2B_KV4_STUCK);
