@@ -27,6 +27,9 @@ constexpr int ATT_LEAST = 8;   // least records (of 16 keys) that a warp is give
 constexpr int ATT_SETUP = 6;   // what an item's fixed costs come to, in records
 constexpr int ATT_MEET = 8;    // what joining the parts of several blocks comes to, in records
 
+// log2 of the most that p = exp(score - M) may be: 2^27 of them stay in fp32, and
+// the least steps of the format, 2^-100, still make weights of 2^-6 and more.
+constexpr float P_MOST = 100.0f;
 constexpr float LOWEST = -FLT_MAX;  // a maximum before anything is seen: below every finite score
 
 struct AttArgs {
@@ -289,7 +292,7 @@ __host__ __device__ constexpr int att_parts(int hd, int nt) { return ATT_WARPS +
 // to the second's operand layout by an 8 x 8 register transpose.
 //
 // M is a lazy maximum per column: it moves only when a weight p * vs (the
-// number that is rounded to half precision) passes 2^14, or p 2^60, or p |vz|
+// number that is rounded to half precision) passes 2^14, or p 2^100, or p |vz|
 // 2^94 (whose sum stays in fp32: of groups of one large number, with step 0),
 // and then to 2^8 below the top.  Whether one might is asked per lane, unseen
 // keys' parameters included; the move goes by the keys that the column sees.  Weights keep 11 bits down to 2^-22 of the
@@ -645,7 +648,7 @@ __global__ __launch_bounds__(ATT_THREADS, NT == 1 ? 2 : 1) void k_kv4_attention(
       float z_most = 0.0f;
 #pragma unroll
       for (int i = 0; i < 2 * RP; ++i) z_most = fmaxf(z_most, fabsf(vz[i]));
-      const float p_bound = fmaxf(0x1p-46f, z_most * OF_BASE);
+      const float p_bound = fmaxf(0x1p-86f, z_most * OF_BASE);  // 2^14 over 2^P_MOST
       uint32_t bw[RP][NT][LIMBS][2];
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
@@ -695,9 +698,9 @@ __global__ __launch_bounds__(ATT_THREADS, NT == 1 ? 2 : 1) void k_kv4_attention(
               w_top = fmaxf(w_top, __shfl_xor_sync(0xffffffffu, w_top, d));
               t_top = fmaxf(t_top, __shfl_xor_sync(0xffffffffu, t_top, d));
             }
-            if (!(fmaxf(w_top - 14.0f, t_top - 60.0f) > m)) return 1.0f;
+            if (!(fmaxf(w_top - 14.0f, t_top - P_MOST) > m)) return 1.0f;
             const float before = m;
-            m = fmaxf(w_top - 8.0f, t_top - 54.0f);
+            m = fmaxf(w_top - 8.0f, t_top - (P_MOST - 6.0f));
             return ex2(before - m);
           };
           const float2 f = make_float2(raise(M[j].x, tw.x, ts.x), raise(M[j].y, tw.y, ts.y));

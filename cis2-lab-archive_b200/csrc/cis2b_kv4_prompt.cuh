@@ -22,7 +22,7 @@
 // row's top, polling without suspension.
 //
 // M is an integer (a power of two scales exactly) and moves only when a weight
-// passes 2^14, p 2^60 or p |vz_j| 2^94 (whose sum stays in fp32); then the row's weights already written, its sums and
+// passes 2^14, p 2^100 or p |vz_j| 2^94 (whose sum stays in fp32); then the row's weights already written, its sums and
 // its O are scaled.  Whether one might is asked per 32 keys, by the row's top
 // score and the largest step or base, of tokens that it does not see too; whether and
 // how far M moves goes by the weights of the keys that it sees.
@@ -598,8 +598,8 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
 #pragma unroll
           for (int i = 0; i < 16; i += 2) top = fmaxf(top, fmaxf(fmaxf(u[i].x, u[i].y), fmaxf(u[i + 1].x, u[i + 1].y)));
           top *= factor;
-          // Weights stay below 2^14, p below 2^60; if not, M rises to 2^8 below the top.
-          bool raise = fmaxf(top + lv_top - 14.0f, top - 60.0f) > M;  // might it have to
+          // Weights stay below 2^14, p below 2^100; if not, M rises to 2^8 below the top.
+          bool raise = fmaxf(top + lv_top - 14.0f, top - P_MOST) > M;  // might it have to
           float w_top = -INFINITY;
           if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
@@ -609,12 +609,12 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
               const float2 y0 = add2(mul2(u[i], fact), make_float2(lv.x, lv.y)), y1 = add2(mul2(u[i + 1], fact), make_float2(lv.z, lv.w));
               w_top = fmaxf(fmaxf(w_top, fmaxf(y0.x, y0.y)), fmaxf(y1.x, y1.y));
             }
-            raise = fmaxf(w_top - 14.0f, top - 60.0f) > M;
+            raise = fmaxf(w_top - 14.0f, top - P_MOST) > M;
           }
           if (__any_sync(0xffffffffu, raise)) {
             float f = 1.0f;
             if (raise) {
-              const float m = ceilf(fmaxf(w_top - 8.0f, top - 54.0f));
+              const float m = ceilf(fmaxf(w_top - 8.0f, top - (P_MOST - 6.0f)));
               f = ex2(M - m);
               M = m, l *= f, z *= f;
             }

@@ -563,3 +563,15 @@ def test_errors_waits_for_every_stream(torch, kv4):
             torch.cuda._sleep(20_000_000)
             batch.plan(*args)
         assert batch.errors() == kv4.PLAN_WIDTH | kv4.PLAN_ROWS
+
+
+# ---------------------------------------------------------------- small values
+
+@pytest.mark.parametrize("new", [1, 5, 60])
+@pytest.mark.parametrize("gain", [1e-12, 1e-16, 1e-20, 1e-24, 1e-27, 3e-29])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_values_of_any_small_size(torch, kv4, dtype, gain, new):
+    """Values down to the format's least steps (2^-96 here) keep their codes."""
+    w = World(torch, kv4, [300, 90], [new, 1], 1, 64, 16, dtype, gain=gain)
+    q = w.queries(4, 64)
+    w.check(q, w.cache.attention(q, w.batch, max_new=new))
