@@ -27,6 +27,9 @@ constexpr int ATT_LEAST = 8;   // least records (of 16 keys) that a warp is give
 constexpr int ATT_SETUP = 6;   // what an item's fixed costs come to, in records
 constexpr int ATT_MEET = 8;    // what joining the parts of several blocks comes to, in records
 
+// log2 of the most that a query is scaled up by: its inverse times a usual scale
+// is still a normal number.
+constexpr int Q_UP = 116;
 // log2 of the most that p = exp(score - M) may be: 2^27 of them stay in fp32, and
 // the least steps of the format, 2^-100, still make weights of 2^-6 and more.
 constexpr float P_MOST = 100.0f;
@@ -532,7 +535,7 @@ __global__ __launch_bounds__(ATT_THREADS, NT == 1 ? 2 : 1) void k_kv4_attention(
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
         const int e = (int)(__float_as_uint(top[j]) >> 23);  // biased exponent
-        const int up = e == 0 || e == 255 ? 0 : min(13 - (e - 127), 100);
+        const int up = e == 0 || e == 255 ? 0 : min(13 - (e - 127), Q_UP);
         const float f = __uint_as_float((uint32_t)(127 + up) << 23);
         const float own = sl * OF_Q * __uint_as_float((uint32_t)(127 - up) << 23);
         code_scale[j] = make_float2(__shfl_sync(0xffffffffu, own, 8 * t), __shfl_sync(0xffffffffu, own, 8 * t + 4));

@@ -351,7 +351,7 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
         for (int i = 0; i < 32; ++i) top = fmaxf(top, fabsf(e[i])), sum_s += e[i];
       }
       const int e2 = (int)(__float_as_uint(top) >> 23);
-      const int up = e2 == 0 || e2 == 255 ? 0 : min(13 - (e2 - 127), 100);
+      const int up = e2 == 0 || e2 == 255 ? 0 : min(13 - (e2 - 127), Q_UP);
       float f = __uint_as_float((uint32_t)(127 + up) << 23);
       // (codes' operands are 16 times as large)
       factor = __uint_as_float(sl_bits & 0x7f800000u) * __uint_as_float((uint32_t)(127 - up) << 23) * (0.0625f / PR_K);

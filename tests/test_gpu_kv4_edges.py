@@ -575,3 +575,16 @@ def test_values_of_any_small_size(torch, kv4, dtype, gain, new):
     w = World(torch, kv4, [300, 90], [new, 1], 1, 64, 16, dtype, gain=gain)
     q = w.queries(4, 64)
     w.check(q, w.cache.attention(q, w.batch, max_new=new))
+
+
+@pytest.mark.parametrize("new", [1, 5, 60])
+@pytest.mark.parametrize("power", [-117, -108, -90, 90, 95])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_queries_and_keys_at_the_ends_of_the_range(torch, kv4, dtype, power, new):
+    """Queries of 2^power over keys that bring their scores back (steps below 2^-100 are 0 in the format)."""
+    d = 64
+    w = World(torch, kv4, [200, 90], [new, 1], 1, d, 16, dtype)
+    for r in range(2):
+        write(torch, w, w.x[r] * np.float32(2.0 ** -power), w.y[r], r)
+    q = (w.queries(4, d).float() * 2.0 ** power).to(w.dtype)
+    w.check(q, w.cache.attention(q, w.batch, max_new=new))
