@@ -103,6 +103,39 @@ __device__ __forceinline__ int tiles_bound(const AttArgs &a, int len) {
   const int some = records(min((uint32_t)a.sinks, keys)) + (int)((min((uint32_t)a.window, keys) + a.qt - 2) >> 4) + 2;
   return min(all, some);
 }
+// How a query row of largest element `top` becomes an operand: times f, a power
+// of two that brings it to 2^13 .. 2^14 (with the scale's sign), so that 16-bit
+// elements down to 2^-24 of it stay exact.  The scores are then
+//   factor (raw * step_factor * unit * ks + kz * sum_of(sum(q)))
+// where raw is the product of the operands in units of the codes' operands.
+// With the scale's mantissa in the second factors, factor is a positive power
+// of two: a score times it is the same number wherever it is formed, and
+// -infinity stays that.
+struct QueryScale {
+  float f, factor, of_sum;
+  // A row with an infinity has NaN for every key that it sees (an infinite sum
+  // could make -infinity of each, which is a mask's).
+  __device__ __forceinline__ float sum_of(float sum) const { return sum * f * of_sum; }
+};
+constexpr float SCORE_UNIT = 16384.0f;  // of factor; in the middle of the range of what products can be
+__device__ __forceinline__ float mantissa_of(float sl) {
+  const uint32_t bits = __float_as_uint(sl) & 0x7fffffffu;
+  return bits >> 23 ? __uint_as_float((bits & 0x7fffffu) | 0x3f800000u) : 1.0f;
+}
+__device__ __forceinline__ float step_factor(float scale) { return mantissa_of(scale * 1.4426950408889634f) / SCORE_UNIT; }
+__device__ __forceinline__ QueryScale query_scale(float scale, float top) {
+  const float sl = scale * 1.4426950408889634f;
+  const int e = (int)(__float_as_uint(top) >> 23);  // biased exponent
+  const int up = e == 0 || e == 255 ? 0 : min(13 - (e - 127), Q_UP);
+  const float f = __uint_as_float((uint32_t)(127 + up) << 23);
+  const float back = __uint_as_float(__float_as_uint(sl) & 0x7f800000u) * __uint_as_float((uint32_t)(127 - up) << 23) * SCORE_UNIT;
+  QueryScale s;
+  s.f = sl > 0.0f ? f : sl < 0.0f ? -f : 0.0f;
+  s.factor = sl == 0.0f ? 1.0f : fminf(fmaxf(back, 0x1p-126f), 0x1p126f);
+  s.of_sum = top == INFINITY ? __int_as_float(0x7fffffff) : mantissa_of(sl) / SCORE_UNIT;
+  return s;
+}
+
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                          uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -316,9 +349,10 @@ __global__ __launch_bounds__(ATT_THREADS, NT == 1 ? 2 : 1) void k_kv4_attention(
   constexpr int PARTS = att_parts(HD, NT);
   // A code's operand is the code over this, of even and odd elements.
   constexpr float EVEN = EXACT ? 1.0f / 16.0f : 16777216.0f, ODD = EXACT ? 1.0f / 16.0f : 1048576.0f;
-  // Of the scores, it goes to the queries' factors and the keys' steps in equal
-  // shares where it is large, so that neither leaves fp32's range before the other.
-  constexpr float OF_Q = EXACT ? EVEN : 4096.0f, OF_K = EXACT ? 1.0f : 4096.0f;
+  // Sums and factors of the query columns, where registers are short (measured 7
+  // to 10 percent slower with them in registers, which spill).
+  constexpr bool COLUMNS_SHARED = NT == 4;
+  __shared__ float4 column_of[COLUMNS_SHARED ? ATT_WARPS : 1][NT][4];
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int scan_t[ATT_THREADS], scan_q[ATT_THREADS], warp_t[ATT_WARPS], warp_top[ATT_WARPS];
   __shared__ int64_t warp_q[ATT_WARPS];
@@ -487,12 +521,12 @@ __global__ __launch_bounds__(ATT_THREADS, NT == 1 ? 2 : 1) void k_kv4_attention(
     };
     // ---- query operands: lane (g, t) holds elements t HD/4 .. of column g
     uint32_t bq[NT == 1 ? LIMBS : 1][NT == 1 ? KS : 1][2];
-    float2 sum_s[NT];  // sum(q) * scale * log2 e of this lane's two columns
-    float2 code_scale[NT];  // of the same columns
+    // Of this lane's two columns: a score is factor (raw * ks + kz * sum_s), see QueryScale.
+    float2 sum_s[COLUMNS_SHARED ? 1 : NT], factor[COLUMNS_SHARED ? 1 : NT];
+    const float of_step = step_factor(a.scale) * EVEN;
     int pos[NT][2];
     {
-      float x[NT][4 * W][2], top[NT];
-      const float sl = a.scale * 1.4426950408889634f;
+      float x[NT][4 * W][2], f[NT];
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
         const int col = 8 * j + g, tok = col / a.group;
@@ -510,41 +544,37 @@ __global__ __launch_bounds__(ATT_THREADS, NT == 1 ? 2 : 1) void k_kv4_attention(
             cp_async_commit();
           }
         }
-        top[j] = 0.0f;
+        float top = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8 * W; ++i) top[j] = fmaxf(top[j], fabsf(e[i])), sum += e[i];
+        for (int i = 0; i < 8 * W; ++i) top = fmaxf(top, fabsf(e[i])), sum += e[i];
         // Word w's `and`s give the code pairs (0,4) (1,5) (2,6) (3,7).
 #pragma unroll
         for (int i = 0; i < 4 * W; ++i) x[j][i][0] = e[(i & ~3) * 2 + (i & 3)], x[j][i][1] = e[(i & ~3) * 2 + (i & 3) + 4];
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], 1));
-        top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], 2));
-        // A column with an infinity has NaN for every key that it sees (an
-        // infinite sum could be -infinity for each, which is a mask's).
-        sum = top[j] == INFINITY ? __int_as_float(0x7fffffff) : sum * sl;
-        sum_s[j] = make_float2(__shfl_sync(0xffffffffu, sum, 8 * t), __shfl_sync(0xffffffffu, sum, 8 * t + 4));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const QueryScale own = query_scale(a.scale, top);
+        f[j] = own.f;
+        sum = own.sum_of(sum);
+        const int to = COLUMNS_SHARED ? 0 : j;
+        sum_s[to] = make_float2(__shfl_sync(0xffffffffu, sum, 8 * t), __shfl_sync(0xffffffffu, sum, 8 * t + 4));
+        factor[to] = make_float2(__shfl_sync(0xffffffffu, own.factor, 8 * t), __shfl_sync(0xffffffffu, own.factor, 8 * t + 4));
+        if (COLUMNS_SHARED && g == 0) column_of[warp][j][t] = make_float4(sum_s[0].x, sum_s[0].y, factor[0].x, factor[0].y);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           const int cc = 8 * j + 2 * t + c;
           pos[j][c] = cc < ncol ? s.p0 + cc / a.group : -1;
         }
       }
-      // A power of two per column brings its largest element to 2^13 .. 2^14:
-      // 16-bit elements down to 2^-24 of it stay exact.
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
-        const int e = (int)(__float_as_uint(top[j]) >> 23);  // biased exponent
-        const int up = e == 0 || e == 255 ? 0 : min(13 - (e - 127), Q_UP);
-        const float f = __uint_as_float((uint32_t)(127 + up) << 23);
-        const float own = sl * OF_Q * __uint_as_float((uint32_t)(127 - up) << 23);
-        code_scale[j] = make_float2(__shfl_sync(0xffffffffu, own, 8 * t), __shfl_sync(0xffffffffu, own, 8 * t + 4));
 #pragma unroll
         for (int w = 0; w < W; ++w) {
           uint32_t v[LIMBS][4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float k = (i & 1) && !EXACT ? f * 0.0625f : f;
+            const float k = (i & 1) && !EXACT ? f[j] * 0.0625f : f[j];
             const float y0 = x[j][4 * w + i][0] * k, y1 = x[j][4 * w + i][1] * k;
             v[0][i] = pack_half(y0, y1);
             if constexpr (LIMBS == 2) {
@@ -644,7 +674,7 @@ __global__ __launch_bounds__(ATT_THREADS, NT == 1 ? 2 : 1) void k_kv4_attention(
       for (int i = 0; i < 2 * RP; ++i) {
         const uint8_t *rec = ring + (stage * RP + (i >> 1)) * REC;
         const uint2 p = *reinterpret_cast<const uint2 *>(rec + 16 * HD + (g + 8 * (i & 1)) * 8);
-        ks[i] = bf16_lo(p.x) * OF_K;
+        ks[i] = bf16_lo(p.x) * of_step;
         kz[i] = EXACT ? fmaf(7.5f, bf16_lo(p.x), bf16_hi(p.x)) : bf16_hi(p.x);
         vs[i] = bf16_lo(p.y), vz[i] = fmaf(7.5f, vs[i], bf16_hi(p.y));
       }
@@ -657,10 +687,17 @@ __global__ __launch_bounds__(ATT_THREADS, NT == 1 ? 2 : 1) void k_kv4_attention(
       for (int j = 0; j < NT; ++j) {
         constexpr int E = 2 * RP;  // pair i: key g + 8 (i & 1) of record i >> 1, columns 2t and 2t + 1
         float2 tt[E], p[E], w[E], vse[E], vze[E];
+        float2 sum_j, factor_j;
+        if constexpr (COLUMNS_SHARED) {
+          const float4 c = column_of[warp][j][t];
+          sum_j = make_float2(c.x, c.y), factor_j = make_float2(c.z, c.w);
+        } else {
+          sum_j = sum_s[j], factor_j = factor[j];
+        }
 #pragma unroll
         for (int i = 0; i < E; ++i) {
           const float2 raw = make_float2(sc[i >> 1][j][2 * (i & 1)], sc[i >> 1][j][2 * (i & 1) + 1]);
-          tt[i] = fma2(mul2(raw, code_scale[j]), make_float2(ks[i], ks[i]), mul2(make_float2(kz[i], kz[i]), sum_s[j]));
+          tt[i] = fma2(raw, make_float2(ks[i], ks[i]), mul2(make_float2(kz[i], kz[i]), sum_j));
           vse[i] = make_float2(vs[i], vs[i]), vze[i] = make_float2(vz[i], vz[i]);
         }
         if (!unmasked) {
@@ -677,7 +714,7 @@ __global__ __launch_bounds__(ATT_THREADS, NT == 1 ? 2 : 1) void k_kv4_attention(
         const float2 minus_m = make_float2(-M[j].x, -M[j].y);
 #pragma unroll
         for (int i = 0; i < E; ++i) {
-          const float2 u = add2(tt[i], minus_m);
+          const float2 u = fma2(tt[i], factor_j, minus_m);
           p[i] = make_float2(ex2(u.x), ex2(u.y));
           w[i] = mul2(p[i], vse[i]);
         }
@@ -690,6 +727,8 @@ __global__ __launch_bounds__(ATT_THREADS, NT == 1 ? 2 : 1) void k_kv4_attention(
         chk.x = fmaxf(chk.x, big.x * p_bound), chk.y = fmaxf(chk.y, big.y * p_bound);
         if (__any_sync(0xffffffffu, fmaxf(chk.x, chk.y) > 0x1p14f)) {
           float2 tw = make_float2(-INFINITY, -INFINITY), ts = tw;
+#pragma unroll
+          for (int i = 0; i < E; ++i) tt[i] = mul2(tt[i], factor_j);
 #pragma unroll
           for (int i = 0; i < E; ++i) {
             tw.x = fmaxf(tw.x, tt[i].x + lg2(size_of(vse[i].x, vze[i].x))), tw.y = fmaxf(tw.y, tt[i].y + lg2(size_of(vse[i].y, vze[i].y)));

@@ -45,7 +45,6 @@ constexpr int PR_THREADS = 256;      // warps 0-3 rows, 4-7 codes; warp 0 also i
 constexpr int PR_MAX_SORT = 512;     // query tiles whose order is chosen (longest first)
 constexpr int PR_LEAST = 16;         // least key tiles of a part
 constexpr int PR_WAIT = 1 << 20;     // polls of a barrier before the kernel gives up
-constexpr float PR_K = 0x1p-14f;     // of the keys' parameters: products with queries' operands (2^28 at most) stay in range
 
 struct PromptArgs {
   AttArgs a;
@@ -326,16 +325,9 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
     auto key_rec = [&](int rec) { return rec < s.sink ? rec : rec - s.sink + s.lo; };
 
     // ---- queries: row = token x group + head of the group
-    // A power of two per row brings its largest element to 2^13 .. 2^14.  It is
-    // divided out in the exponent: a row's scores are `factor` times S * ks +
-    // kz * sum_s.  With the scale's sign in the query and its mantissa in the keys'
-    // parameters, factor is a positive power of two, so that a score times it is
-    // the same number wherever it is formed, and -infinity stays that.
-    float sum_s = 0.0f, factor = 1.0f;
+    float sum_s = 0.0f, factor = 1.0f;  // a row's scores are factor (S * ks + kz * sum_s), see QueryScale
     int pos = -1;
-    const float sl = a.scale * 1.4426950408889634f;
-    const uint32_t sl_bits = __float_as_uint(fabsf(sl));
-    const float key_factor = PR_K * (sl_bits >> 23 ? __uint_as_float((sl_bits & 0x7fffffu) | 0x3f800000u) : 1.0f);
+    const float of_step = step_factor(a.scale) * 0.0625f;  // codes' operands are 16 times as large
     if (warp < 4) {
       const int tok = tid / a.group;
       const int64_t row = (int64_t)row0 + tok;
@@ -350,16 +342,9 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
 #pragma unroll
         for (int i = 0; i < 32; ++i) top = fmaxf(top, fabsf(e[i])), sum_s += e[i];
       }
-      const int e2 = (int)(__float_as_uint(top) >> 23);
-      const int up = e2 == 0 || e2 == 255 ? 0 : min(13 - (e2 - 127), Q_UP);
-      float f = __uint_as_float((uint32_t)(127 + up) << 23);
-      // (codes' operands are 16 times as large)
-      factor = __uint_as_float(sl_bits & 0x7f800000u) * __uint_as_float((uint32_t)(127 - up) << 23) * (0.0625f / PR_K);
-      factor = sl == 0.0f ? 1.0f : fminf(fmaxf(factor, 0x1p-126f), 0x1p126f);
-      f = sl > 0.0f ? f : sl < 0.0f ? -f : 0.0f;
-      // A row with an infinity has NaN for every key that it sees (an infinite
-      // sum could be -infinity for each, which is a mask's).
-      sum_s = top == INFINITY ? __int_as_float(0x7fffffff) : sum_s * f * 16.0f;
+      const QueryScale own = query_scale(a.scale, top);
+      const float f = own.f;
+      factor = own.factor, sum_s = own.sum_of(sum_s);
 #pragma unroll 1
       for (int d0 = 0; d0 < HD; d0 += 32) {
         float e[32];
@@ -445,7 +430,7 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
         if (pw == 0 && lane < PR_RECS) held[now & 1][lane] = ids != NONE;
         float *dst = reinterpret_cast<float *>(sp + (now & 1) * 128 + (pt >> 1) * 2) + (pt & 1);
         const float ks = bf16_lo(par.x), vs = bf16_lo(par.y), vz = fmaf(7.5f, vs, bf16_hi(par.y));
-        dst[0] = ks * key_factor, dst[2] = fmaf(7.5f, ks, bf16_hi(par.x)) * key_factor;
+        dst[0] = ks * of_step, dst[2] = fmaf(7.5f, ks, bf16_hi(par.x));
         dst[4] = vs, dst[6] = vz;
         // The largest logarithm, not that of the largest, bounds what the row
         // warps add for each key.
