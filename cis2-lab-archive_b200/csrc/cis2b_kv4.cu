@@ -270,7 +270,8 @@ __device__ __forceinline__ uint32_t kv4_codes(const float (&x)[8], uint32_t para
 // elements each, so one warp instruction reads whole 128-byte lines and a
 // group's range is log2(D / 8) shuffles away.  Half of the lanes then find the
 // key's parameters and half the value's.  Each element is read once and each
-// code written once; instructions bound it (fp16, 40,009 rows of 8 x 128).
+// code written once; instructions bound it: 18 per element, issued in 84 percent
+// of the cycles (fp16, 40,009 rows of 8 x 128 in 54 us; its bytes need 32).
 template <int HD, int DT>
 __global__ __launch_bounds__(ROW_THREADS) void k_kv4_append(RowArgs a, const void *k, const void *v, bool wide) {
   constexpr int LANES = HD / 8;
@@ -333,8 +334,9 @@ __device__ __forceinline__ void kv4_values(uint32_t word, uint32_t params, float
   for (int i = 0; i < 8; ++i) x[i] = fmaf(step, __uint_as_float(((word >> (4 * i)) & 15) | 0x4b000000u) - 8388608.0f, base);
 }
 
-// Codes to rows, the same split, two rows per lane: what bounds it is the wait
-// for the slot and then for the codes.
+// Codes to rows, the same split, two rows per lane: 12 instructions per element,
+// issued in 74 percent of the cycles, and the wait for the slot and then for the
+// codes bound it (fp16, 40,009 rows of 8 x 128 in 42 us; its bytes need 32).
 template <int HD>
 __global__ __launch_bounds__(ROW_THREADS) void k_kv4_gather(RowArgs a, void *k, void *v, int dt, bool wide) {
   constexpr int LANES = HD / 8, PER = ROW_THREADS / LANES;

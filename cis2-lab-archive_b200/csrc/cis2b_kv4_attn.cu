@@ -308,15 +308,20 @@ __host__ __device__ constexpr int att_parts(int hd, int nt) { return ATT_WARPS +
 // subnormal), and in bits 4-7 c * 2^-20, so `and` makes two operands out of a
 // 32-bit word, and the factor of 16 is divided out of every other query
 // element (keys) or output row (values).  The tensor pipe lines subnormal
-// products up by their exponent field, so its sums keep about 15 bits
-// (measured: 4e-5 of fp32 rows' results, 2.4 times plain fp16's error at
-// 130,051 keys), enough for 8-bit results; fp16 and fp32 rows (EXACT) pay
-// one or two more operations for the normal numbers 16 (c - 7.5).
+// products up by their exponent field and drops what falls below its sums (in
+// fp32), so a sum keeps about 15 bits (measured: 4e-5 of fp32 rows' results,
+// 2.4 times plain fp16's error at 130,051 keys), enough for 8-bit results: the
+// error of bf16 rows is 1.66e-3 there, 1.56e-3 of which is the results' own
+// rounding, and exact codes would take 134 us in place of 102 over a ragged
+// batch of 64.  fp16 and fp32 rows (EXACT) pay one or two more operations for
+// the normal numbers 16 (c - 7.5).
 //
-// The cache's bytes bound it: at 16 warps per SM a record of head_dim 128 takes
-// 101 cycles per SM (bf16; HBM's 93 at its measured rate), 345 instructions with
-// exact codes, which issue bounds at about 125.  Around that a call spends about
-// 10,000 cycles until the first record is there and 10,000 to 20,000 joining
+// The cache's bytes bound bf16 rows, instructions the others: HBM at its measured
+// rate gives an SM a record of head_dim 128 every 93 cycles, and the 280 (bf16),
+// 437 (fp16) and 483 (fp32) warp instructions per record, all included, are 70,
+// 109 and 121 cycles of issue; a call over 206,616 records takes 109, 136 and 174
+// us, 8 rows per request 334, 316 and 412.  Around the records a call spends
+// about 10,000 cycles until the first one is there and 10,000 to 20,000 joining
 // parts.  Measured on the way: a block per 512 keys with tickets 184 us for the
 // ragged batch of 64 (a unit's fixed costs are 12,000 cycles), even stretches
 // per block 132, per warp 119 to 105.

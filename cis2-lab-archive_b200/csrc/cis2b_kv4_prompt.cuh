@@ -13,19 +13,21 @@
 //   the same thread issues O += W V^T (128 x head_dim fp32 in TMEM).
 // The two blocks of an SM fill each other's waits.  Per tile of head_dim 128
 // the tensor cores need 1,024 cycles, the exponentials 1,024 and the warps'
-// 7,300 instructions 1,825; measured (bf16, 100 GFLOP) are 3,650, i.e. 7,300
-// per block: 4,100 for the row warps' work, whose registers leave no room to
-// load ahead, and 3,100 for the products and the hand-offs around them, which
-// cannot overlap it since the weights take the scores' place in TMEM.
+// 9,400 instructions 2,350; measured (bf16, 100 GFLOP in 250 us) are 5,200, all
+// included.  The row warps' registers leave no room to load ahead, and the
+// products cannot overlap their work, since the weights take the scores' place
+// in TMEM.  fp32 rows of head_dim 64 need 13,000 instructions a tile (8 x 1,024
+// rows in 93 us).
 // Measured slower: the products issued by a code warp (it stalls while they
 // are queued) or by a ninth warp (96 registers), a pass of its own for the
 // row's top, polling without suspension.
 //
 // M is an integer (a power of two scales exactly) and moves only when a weight
-// passes 2^14, p 2^100 or p |vz_j| 2^94 (whose sum stays in fp32); then the row's weights already written, its sums and
-// its O are scaled.  Whether one might is asked per 32 keys, by the row's top
-// score and the largest step or base, of tokens that it does not see too; whether and
-// how far M moves goes by the weights of the keys that it sees.
+// passes 2^14, p 2^100 or p |vz_j| 2^94 (whose sum stays in fp32); then the row's
+// weights already written, its sums and its O are scaled.  Whether one might is
+// asked per 32 keys, by the row's top score and the largest step or base, of
+// tokens that it does not see too; whether and how far M moves goes by the
+// weights of the keys that it sees.
 // LIMBS = 2 (fp32 rows): two half-precision limbs of the query and of the
 // weights, twice the products.
 // The tensor cores cut off what falls below their sums, so the small limbs have

@@ -368,8 +368,13 @@ int cis2b_kv4_gather(const cis2b_kv4_cache *c, int32_t dtype, void *k, void *v, 
  *              it too, but calls that may overlap on the GPU (replays of
  *              captured ones among them) need one each.
  *              Zero it again after CIS2B_KV4_STUCK
- * Softmax statistics and sums are held in fp32; fp32 rows keep 22 bits of
- * every product's operands, 16-bit rows at least 11. */
+ * Softmax statistics and sums are held in fp32 (of bf16 rows in the kernel for
+ * one or few tokens, the tensor cores' sums keep about 15 bits).  Codes are
+ * exact; a row's query elements and its weights are rounded to 22 bits (fp32
+ * rows) or 11 (16-bit rows), those below 2^-10 (22 bits) or 2^-21 (11 bits) of
+ * the row's largest to 2^-32 of it.  What a row does not see, whatever finite
+ * or other number stands there, changes no bit of its result; a query row with
+ * an infinity or a NaN is NaN where it sees anything. */
 #define CIS2B_KV4_WHOLE 1
 #define CIS2B_KV4_WORK_ZERO 266240
 typedef struct {
