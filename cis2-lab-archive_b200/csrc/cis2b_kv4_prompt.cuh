@@ -46,7 +46,7 @@ constexpr int PR_ROWS = 128, PR_KEYS = 128, PR_RECS = PR_KEYS / KV4_REC;
 constexpr int PR_THREADS = 256;      // warps 0-3 rows, 4-7 codes; warp 0 also issues the products
 constexpr int PR_MAX_SORT = 512;     // query tiles whose order is chosen (longest first)
 constexpr int PR_LEAST = 16;         // least key tiles of a part
-constexpr int PR_WAIT = 1 << 20;     // polls of a barrier before the kernel gives up
+constexpr int PR_WAIT = 1 << 18;     // polls of a barrier, of about 4 us each, before the kernel gives up
 
 struct PromptArgs {
   AttArgs a;
