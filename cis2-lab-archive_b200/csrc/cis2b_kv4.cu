@@ -1,5 +1,6 @@
 // cis2b_kv4.cu -- step planning, append and read-back of the 4-bit key/value
-// cache (include/cis2b.h).  Attention over it is in cis2b_kv4_attn.cu.
+// cache (include/cis2b.h).  Attention over it is in
+// cis2b_kv4_attn.cuh, drafted trees in cis2b_kv4_tree.cu.
 #include "../../include/cis2b.h"
 #include "cis2b_kv4.h"
 #include "cis2b_kv4.cuh"
@@ -25,7 +26,7 @@ int kv4_cuda(cudaError_t e) noexcept {
   return e == cudaSuccess ? CIS2B_OK : kv4_fail(CIS2B_ERR_CUDA, cudaGetErrorString(e));
 }
 
-static int page_shift(int page_size) {
+int kv4_page_shift(int page_size) noexcept {
   for (int s = 4; s <= 8; ++s)
     if (page_size == 1 << s) return s;
   return -1;
@@ -35,7 +36,7 @@ int kv4_check_cache(const cis2b_kv4_cache *c, bool pool) noexcept {
   if (!c) return kv4_fail(CIS2B_ERR_ARG, "cache is NULL");
   if (c->reserved) return kv4_fail(CIS2B_ERR_ARG, "cache: reserved must be zero");
   if (c->head_dim != 64 && c->head_dim != 128) return kv4_fail(CIS2B_ERR_ARG, "cache: head_dim must be 64 or 128");
-  if (page_shift(c->page_size) < 0)
+  if (kv4_page_shift(c->page_size) < 0)
     return kv4_fail(CIS2B_ERR_ARG, "cache: page_size must be 16, 32, 64, 128 or 256");
   if (c->kv_heads < 1 || c->kv_heads > 65535) return kv4_fail(CIS2B_ERR_ARG, "cache: kv_heads must be in 1..65535");
   if (c->pages < 1 || (int64_t)c->pages * c->page_size > INT_MAX)
@@ -399,7 +400,7 @@ static int row_args(const cis2b_kv4_cache *c, int32_t dtype, const void *k, cons
   if ((int64_t)rows * c->kv_heads > INT_MAX || blocks > INT_MAX)
     return kv4_fail(CIS2B_ERR_ARG, "rows * kv_heads must be < 2^31");
   *grid = (int)blocks;
-  *a = RowArgs{static_cast<const uint8_t *>(c->pool), c->status, slot, rows, c->kv_heads, page_shift(c->page_size),
+  *a = RowArgs{static_cast<const uint8_t *>(c->pool), c->status, slot, rows, c->kv_heads, kv4_page_shift(c->page_size),
                c->pages * c->page_size, 0, 0, 0, 0};
   return CIS2B_OK;
 }
@@ -419,7 +420,7 @@ extern "C" int cis2b_kv4_plan(const cis2b_kv4_step *s, void *stream) {
   if (!s) return kv4_fail(CIS2B_ERR_ARG, "step is NULL");
   if (s->requests < 1 || s->requests > PLAN_MAX_REQUESTS)
     return kv4_fail(CIS2B_ERR_ARG, "step: requests must be in 1..16384");
-  const int shift = page_shift(s->page_size);
+  const int shift = kv4_page_shift(s->page_size);
   if (shift < 0) return kv4_fail(CIS2B_ERR_ARG, "step: page_size must be 16, 32, 64, 128 or 256");
   if (s->rows < 0 || s->width < 1 || s->free_count < 0)
     return kv4_fail(CIS2B_ERR_ARG, "step: rows and free_count must be >= 0 and width >= 1");

@@ -1,6 +1,6 @@
 // cis2b_kv4_prompt.cuh -- attention of many new rows per request over the
 // 4-bit cache, on the fifth-generation tensor cores.  Included by
-// cis2b_kv4_attn.cu, whose argument and span types it shares.
+// cis2b_kv4_attn.cuh, whose argument and span types it shares.
 //
 // A unit is 128 query rows (tokens x the group of one KV head) of one request
 // against a stretch of its keys.  Per tile of 128 keys:
@@ -152,7 +152,7 @@ __device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, ui
                "r"(a), "l"(b), "r"(idesc), "r"((int)add) : "memory");
 }
 
-template <int HD, int LIMBS>
+template <int HD, int LIMBS, Rows SEE>
 __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k_kv4_prompt(PromptArgs pa) {
   const AttArgs &a = pa.a;
   constexpr int REC = kv4_rec_bytes(HD);
@@ -252,7 +252,7 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
     t.qi = q - before;
     return t;
   };
-  auto key_tiles = [&](const Tile &t) { return (span_of(a, t.len, t.n, t.rows, t.qi).tiles + PR_RECS - 1) / PR_RECS; };
+  auto key_tiles = [&](const Tile &t) { return (span_of<SEE>(a, t.len, t.n, t.rows, t.qi).tiles + PR_RECS - 1) / PR_RECS; };
 
   // Up to PR_MAX_SORT query tiles are taken longest first, and the longest are
   // cut into parts of `each` key tiles where there are too few to go round.
@@ -320,7 +320,7 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
       q = all_q - 1 - ui;
     }
     const Tile t = find(q);
-    const Span s = span_of(a, t.len, t.n, t.rows, t.qi);
+    const Span s = span_of<SEE>(a, t.len, t.n, t.rows, t.qi);
     const int all_tiles = (s.tiles + PR_RECS - 1) / PR_RECS, share = (all_tiles + parts - 1) / parts;
     const int j0 = min(part * share, all_tiles), j1 = min(j0 + share, all_tiles);
     const int row0 = t.row0 + t.qi * a.qt, nrow = min(a.qt, t.rows - t.qi * a.qt) * a.group;
@@ -335,7 +335,7 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
       const int64_t row = (int64_t)row0 + tok;
       const bool on = tid < nrow && row >= 0 && row < a.rows;
       const int64_t from = row * a.q_row + (int64_t)(head * a.group + tid - tok * a.group) * a.q_head;
-      if (tid < nrow) pos = s.p0 + tok;
+      if (tid < nrow) pos = SEE == Rows::CAUSAL ? s.p0 + tok : SEE == Rows::CROSS ? s.p1 : tree_position(a, row, s.p0 + 1, t.n);
       float top = 0.0f;
 #pragma unroll 1
       for (int d = 0; d < HD; d += 32) {
@@ -572,6 +572,12 @@ __global__ __launch_bounds__(PR_THREADS, HD == 128 && LIMBS == 2 ? 1 : 2) void k
                 const uint32_t late = first_i <= 0 ? 0xffffu : first_i > 15 ? 0u : 0xffffu & ~((1u << first_i) - 1);
                 const uint32_t sink = sink_i <= 0 ? 0u : sink_i > 15 ? 0xffffu : (1u << sink_i) - 1;
                 bits &= late | sink;
+              }
+              if (SEE == Rows::TREE && key0 + 15 > s.p0) {  // new tokens among them: bit 0 of the mask is key p0 + 1
+                const int old = max(0, min(s.p0 + 1 - key0, 16)), end = max(0, min(s.p1 + 1 - key0, 16));
+                const uint32_t before = (1u << old) - 1;
+                const uint32_t named = pos < 0 ? 0u : tree_bits(a, (int64_t)row0 + tid / a.group, key0 - s.p0 - 1);
+                bits = (bits & before) | (named & ~before & ((1u << end) - 1));
               }
               see |= bits << (16 * h);
             }

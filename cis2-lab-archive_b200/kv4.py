@@ -15,6 +15,18 @@ share; each call captured in a CUDA graph has its own, so graphs may be
 replayed on any streams, and beside other calls (not one graph beside itself).
 Nothing here has a gradient.  This module needs torch for its tensors; the
 rest of the package does not.
+
+A step that verifies a tree of drafted tokens, and attention to an encoder's
+states, whose keys and values another cache holds:
+
+    batch = kv4.Batch(requests=64, tokens=64 * 16, width=256, page_size=64, tree=16)
+    batch.plan(cached, new, free_pages)
+    batch.plan_tree(parent)                    # batch.mask, batch.position
+    cache.append(k, v, batch.slot)             # in every layer
+    out = cache.tree_attention(q, batch, max_new=16)
+    out = encoder.cross_attention(q, encoder_batch, max_new=16)
+    batch.accept(token, parent, target)        # batch.accepted, .path, .next_token, .kept
+    batch.keep(caches)                         # the accepted rows, in all layers at once
 """
 from __future__ import annotations
 
@@ -29,9 +41,11 @@ Cis2Error = _pkg.Cis2Error
 
 _I32, _I64, _U64, _P = ctypes.c_int32, ctypes.c_int64, ctypes.c_uint64, ctypes.c_void_p
 
-BAD_SLOT, BAD_PAGE, STUCK = 1, 2, 4  # CIS2B_KV4_*
+BAD_SLOT, BAD_PAGE, STUCK, BAD_PATH = 1, 2, 4, 8  # CIS2B_KV4_*
 _WORK_ZERO = 266240  # CIS2B_KV4_WORK_ZERO
 PLAN_FREE, PLAN_WIDTH, PLAN_ROWS, PLAN_NEGATIVE = 1, 2, 4, 8  # CIS2B_KV4_PLAN_*
+TREE_PARENT, TREE_ROWS = 1, 2  # CIS2B_KV4_TREE_*
+TREE_MOST = 1024  # CIS2B_KV4_TREE_MOST
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # CIS2B_F32, _F16, _BF16
 
 
@@ -54,6 +68,22 @@ class _Attn(ctypes.Structure):
                 ("work_bytes", _U64)]
 
 
+class _Tree(ctypes.Structure):
+    _fields_ = [("device", _I32), ("requests", _I32), ("rows", _I32), ("words", _I32), ("length", _P), ("row_start", _P),
+                ("parent", _P), ("mask", _P), ("position", _P), ("status", _P)]
+
+
+class _Draft(ctypes.Structure):
+    _fields_ = [("device", _I32), ("requests", _I32), ("rows", _I32), ("reserved", _I32), ("length", _P), ("row_start", _P),
+                ("token", _P), ("parent", _P), ("target", _P), ("accepted", _P), ("path", _P), ("next_token", _P),
+                ("kept", _P), ("status", _P)]
+
+
+class _Kept(ctypes.Structure):
+    _fields_ = [("device", _I32), ("requests", _I32), ("rows", _I32), ("reserved", _I32), ("row_start", _P),
+                ("accepted", _P), ("path", _P), ("slot", _P)]
+
+
 _funcs = None
 
 
@@ -67,6 +97,12 @@ def _lib():
         L.cis2b_kv4_gather.argtypes = [_P, _I32, _P, _P, _P, _I32, _P]
         L.cis2b_kv4_workspace.argtypes = [_P, _P, _P]
         L.cis2b_kv4_attention.argtypes = [_P, _P, _P]
+        L.cis2b_kv4_plan_tree.argtypes = [_P, _P]
+        L.cis2b_kv4_accept.argtypes = [_P, _P]
+        L.cis2b_kv4_keep.argtypes = [_P, _I32, _P, _P]
+        L.cis2b_kv4_tree_workspace.argtypes = [_P, _P, _P]
+        L.cis2b_kv4_tree_attention.argtypes = [_P, _P, _P, _I32, _P, _P]
+        L.cis2b_kv4_cross_attention.argtypes = [_P, _P, _P]
         _funcs = L
     return _funcs
 
@@ -121,9 +157,16 @@ class Batch:
     table [requests, width], length [requests], row_start [requests + 1],
     slot, position and request [tokens], counts [4]: int32 on the device.
     `plan` fills them; a batch made by `of` takes a table, lengths and row
-    starts that the caller has built."""
+    starts that the caller has built.
 
-    def __init__(self, requests: int, tokens: int, width: int, page_size: int, table=None, device="cuda"):
+    Of drafted trees: mask [tokens, ceil(tree / 32)], which `plan_tree` fills
+    (and position with it), if `tree`, the most rows of one request, is given;
+    accepted, next_token and kept [requests] and path [tokens], which `accept`
+    fills and which are None before."""
+
+    mask = accepted = path = next_token = kept = None
+
+    def __init__(self, requests: int, tokens: int, width: int, page_size: int, table=None, device="cuda", tree: int = 0):
         if requests < 1 or tokens < 0 or width < 1:
             raise ValueError("requests and width must be >= 1 and tokens >= 0")
         _int32(("requests", requests), ("tokens", tokens), ("width", width), ("page_size", page_size))
@@ -142,10 +185,24 @@ class Batch:
                            self.slot.data_ptr(), self.position.data_ptr(), self.request.data_ptr(),
                            self.counts.data_ptr())
         self._ref = ctypes.byref(self._step)
+        self._trees(tree, tokens)
+
+    def _trees(self, tree: int, rows: int) -> None:
+        if not 0 <= tree <= TREE_MOST:
+            raise ValueError(f"tree must be in 0..{TREE_MOST}")
+        self._tree = self._draft = self._kept = None
+        self._tree_bits = torch.zeros(1, dtype=torch.int32, device=f"cuda:{self.device}")
+        if tree:
+            words = (tree + 31) // 32
+            self.mask = torch.zeros((rows, words), dtype=torch.int32, device=f"cuda:{self.device}")
+            self._tree = _Tree(self.device, self.length.numel(), rows, words, None, None, None, None, None,
+                               self._tree_bits.data_ptr())
 
     @classmethod
-    def of(cls, table, length, row_start, page_size: int) -> "Batch":
-        """A batch over the caller's own table, lengths and row starts."""
+    def of(cls, table, length, row_start, page_size: int, slot=None, rows: int | None = None, tree: int = 0) -> "Batch":
+        """A batch over the caller's own table, lengths and row starts.  `keep`
+        needs slot [rows], plan_tree `tree` and the number of rows (slot's, if
+        that is given)."""
         self = cls.__new__(cls)
         self.device = _device_index(table.device)
         self.page_size = page_size
@@ -156,6 +213,16 @@ class Batch:
         self.length = _ints(length, "length", self.device, (n,))
         self.row_start = _ints(row_start, "row_start", self.device, (n + 1,))
         self.slot = self.position = self.request = self.counts = self._step = None
+        if slot is not None:
+            if slot.dim() != 1 or rows not in (None, slot.shape[0]):
+                raise ValueError("slot must be [rows]")
+            self.slot, rows = _ints(slot, "slot", self.device), slot.shape[0]
+        if tree:
+            if rows is None or rows < 0:
+                raise ValueError("a batch with trees needs the number of its rows")
+            _int32(("rows", rows))
+            self.position = torch.full((rows,), -1, dtype=torch.int32, device=f"cuda:{self.device}")
+        self._trees(tree, rows or 0)
         return self
 
     def plan(self, cached, new, free_pages) -> None:
@@ -176,6 +243,74 @@ class Batch:
         """PLAN_* bits of the last plan, 0 if all is well.  Waits for the GPU."""
         torch.cuda.synchronize(self.device)  # on whichever stream it was
         return int(self.counts[2].item())
+
+    def plan_tree(self, parent) -> None:
+        """Masks and positions of drafted trees (cis2b_kv4_plan_tree): parent
+        [rows], int32, the row of the same request that each row continues, -1
+        for the cached tokens.  Fills mask and position.  `tree_errors` reads
+        what went wrong, if anything."""
+        t = self._tree
+        if t is None:
+            raise ValueError("this batch was made without trees; give it `tree`, the most rows of one request")
+        _ints(parent, "parent", self.device, (t.rows,))
+        t.length, t.row_start, t.parent = self.length.data_ptr(), self.row_start.data_ptr(), parent.data_ptr()
+        t.mask, t.position = self.mask.data_ptr(), self.position.data_ptr()
+        _call(self.device, _lib().cis2b_kv4_plan_tree, ctypes.byref(t))
+
+    def accept(self, token, parent, target) -> None:
+        """The longest path of drafted tokens that the model agrees with
+        (cis2b_kv4_accept): token, parent and target [rows], int32; target is
+        the model's next token after each row.  Fills accepted, path, next_token
+        and kept, the tokens that the request has cached from now on."""
+        dev = self.device
+        if token.dim() != 1:
+            raise ValueError("token must be [rows]")
+        rows, n = token.shape[0], self.length.numel()
+        for t, name in ((token, "token"), (parent, "parent"), (target, "target")):
+            _ints(t, name, dev, (rows,))
+        d = self._draft
+        if d is None or d.rows != rows:
+            _int32(("rows", rows))
+            self.accepted, self.next_token, self.kept, self.path = (
+                torch.full((m,), -1, dtype=torch.int32, device=f"cuda:{dev}") for m in (n, n, n, rows))
+            d = self._draft = _Draft(dev, n, rows, 0, None, None, None, None, None, self.accepted.data_ptr(),
+                                     self.path.data_ptr(), self.next_token.data_ptr(), self.kept.data_ptr(),
+                                     self._tree_bits.data_ptr())
+        d.length, d.row_start = self.length.data_ptr(), self.row_start.data_ptr()
+        d.token, d.parent, d.target = token.data_ptr(), parent.data_ptr(), target.data_ptr()
+        _call(dev, _lib().cis2b_kv4_accept, ctypes.byref(d))
+
+    def keep(self, caches) -> None:
+        """Moves the accepted rows of every request to the places that follow
+        its cached tokens, in each of `caches` (cis2b_kv4_keep), one launch for
+        up to 64 layers.  They are cached from then on: kept[r] tokens.  What
+        stands in the other rows' places is left as it is."""
+        caches = list(caches)
+        if self._draft is None or self.slot is None:
+            raise ValueError("keep follows accept, and needs the batch's slots")
+        if not caches or any(c.device != self.device or c.page_size != self.page_size for c in caches):
+            raise ValueError(f"the caches must be on cuda:{self.device}, with pages of {self.page_size} tokens")
+        if len({c.pool.data_ptr() for c in caches}) != len(caches):
+            raise ValueError("a cache may be given once")
+        rows = self.path.shape[0]
+        if self.slot.shape[0] < rows:
+            raise ValueError(f"the batch has slots for {self.slot.shape[0]} rows, not {rows}")
+        every = self._kept
+        if every is None or every[0] != caches:
+            every = self._kept = (caches, (_Cache * len(caches))(*(c._c for c in caches)))
+        k = _Kept(self.device, self.length.numel(), rows, 0, self.row_start.data_ptr(), self.accepted.data_ptr(),
+                  self.path.data_ptr(), self.slot.data_ptr())
+        _call(self.device, _lib().cis2b_kv4_keep, every[1], len(caches), ctypes.byref(k))
+
+    def tree_errors(self) -> int:
+        """TREE_* bits that plan_tree and accept have left since the last time,
+        0 if all is well.  Waits for the GPU."""
+        torch.cuda.synchronize(self.device)
+        bits = int(self._tree_bits.item())
+        if bits:
+            self._tree_bits.zero_()
+            torch.cuda.synchronize(self.device)
+        return bits
 
 
 class _Workspaces(dict):
@@ -267,15 +402,56 @@ class Cache:
         rows in one request.  whole: a request's result does not depend on the
         rest of the batch, given the same max_new (slower over long requests).
         Returns out (made if None)."""
+        ref, out = self._arguments("attention", q, batch, out, scale, window, sinks, max_new, whole)
+        _call(self.device, _lib().cis2b_kv4_attention, self._ref, ref)
+        return out
+
+    def tree_attention(self, q, batch: Batch, mask=None, position=None, scale: float | None = None, window: int = 0,
+                       sinks: int = 0, max_new: int | None = None, out=None, whole: bool = False):
+        """Attention of drafted tokens q [rows, heads, head_dim], whose own
+        keys and values are appended before.  A row sees the request's cached
+        tokens (with window > 0 those less than `window` before its position,
+        and the first `sinks`), and of its new ones those whose bits mask
+        [rows, words] has: bit b % 32 of word b // 32 for row b of the request.
+        mask and position [rows] are the batch's own (plan_tree) if None; any
+        mask may be given; position is read with a window only.  The rest is as
+        in `attention`."""
+        mask = batch.mask if mask is None else mask
+        position = batch.position if position is None else position
+        if mask is None or mask.dim() != 2 or mask.shape[0] < q.shape[0] or not mask.shape[1]:
+            raise ValueError("mask must be [rows, words], with a row for each of q; plan_tree makes the batch's own")
+        _ints(mask, "mask", self.device)
+        at = None
+        if window:
+            if position is None or position.dim() != 1 or position.shape[0] < q.shape[0]:
+                raise ValueError("with a window, position must be [rows], with one for each row of q")
+            at = _ints(position, "position", self.device).data_ptr()
+        ref, out = self._arguments("tree_attention", q, batch, out, scale, window, sinks, max_new, whole)
+        _call(self.device, _lib().cis2b_kv4_tree_attention, self._ref, ref, mask.data_ptr(), mask.shape[1], at)
+        return out
+
+    def cross_attention(self, q, batch: Batch, scale: float | None = None, max_new: int | None = None, out=None,
+                        whole: bool = False):
+        """Attention of rows q [rows, heads, head_dim] to the states of an
+        encoder that this cache holds: batch.length[r] of them, 0 or more, on
+        the pages of batch.table[r], all seen by every row of request r
+        (batch.row_start), however many rows that are.  Requests may share
+        pages, as beams do.  The rest is as in `attention`."""
+        ref, out = self._arguments("cross_attention", q, batch, out, scale, 0, 0, max_new, whole)
+        _call(self.device, _lib().cis2b_kv4_cross_attention, self._ref, ref)
+        return out
+
+    def _arguments(self, kind, q, batch, out, scale, window, sinks, max_new, whole):
+        """The filled-in arguments of a call, and its output."""
         if q.requires_grad and torch.is_grad_enabled():
             raise ValueError("attention over the 4-bit cache has no gradient")
         if out is None:
             out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        key = (q.dtype, q.shape, q.stride(), out.dtype, out.shape, out.stride(), batch.table.shape, batch.page_size,
+        key = (kind, q.dtype, q.shape, q.stride(), out.dtype, out.shape, out.stride(), batch.table.shape, batch.page_size,
                scale, window, sinks, max_new, whole)
         call = self._calls.get(key)
         if call is None:
-            call = self._prepare(q, out, batch, scale, window, sinks, max_new, whole)
+            call = self._prepare(kind, q, out, batch, scale, window, sinks, max_new, whole)
             if len(self._calls) >= 64:
                 self._calls.clear()
             self._calls[key] = call
@@ -286,8 +462,7 @@ class Cache:
         work = self._workspace(need)
         a.q, a.out, a.work, a.work_bytes = q.data_ptr(), out.data_ptr(), work.data_ptr(), work.numel()
         a.table, a.length, a.row_start = batch.table.data_ptr(), batch.length.data_ptr(), batch.row_start.data_ptr()
-        _call(dev, _lib().cis2b_kv4_attention, self._ref, ref)
-        return out
+        return ref, out
 
     def _workspace(self, need: int):
         """The current stream's workspace.  A call that is captured gets one of
@@ -305,7 +480,7 @@ class Cache:
                 self._work[stream] = work  # an outgrown one is free for what follows on this stream
         return work
 
-    def _prepare(self, q, out, batch, scale, window, sinks, max_new, whole):
+    def _prepare(self, kind, q, out, batch, scale, window, sinks, max_new, whole):
         if q.dim() != 3 or q.shape[2] != self.head_dim:
             raise ValueError(f"q must be [rows, heads, {self.head_dim}]")
         if q.dtype not in _DTYPES:
@@ -325,5 +500,6 @@ class Cache:
                   self.head_dim ** -0.5 if scale is None else scale, int(whole), None, None, q.stride(0), q.stride(1),
                   out.stride(0), out.stride(1), None, None, None, None, 0)
         need = _U64()
-        _check(_lib().cis2b_kv4_workspace(self._ref, ctypes.byref(a), ctypes.byref(need)))
+        size = _lib().cis2b_kv4_workspace if kind == "attention" else _lib().cis2b_kv4_tree_workspace
+        _check(size(self._ref, ctypes.byref(a), ctypes.byref(need)))
         return a, ctypes.byref(a), need.value

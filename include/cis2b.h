@@ -398,6 +398,96 @@ typedef struct {
 int cis2b_kv4_workspace(const cis2b_kv4_cache *c, const cis2b_kv4_attn *a, uint64_t *out_bytes);
 int cis2b_kv4_attention(const cis2b_kv4_cache *c, const cis2b_kv4_attn *a, void *stream);
 
+/* ---- drafted trees and encoders over the 4-bit cache ---------------------
+ * Rows that do not see by their place alone: the tokens of a tree that a
+ * smaller model has drafted, and rows that attend to an encoder's states.
+ *
+ * A step of drafted tokens.  cis2b_kv4_plan gives request r's n = row_start[r+1]
+ * - row_start[r] new tokens the places that follow its cached = length[r] - n
+ * tokens, in row order.  Row 0 of a request is the token that the model has
+ * settled on last; parent[row] is the number, within the request, of the row
+ * that a row continues, or -1 for one that continues the cached tokens.  A
+ * parent stands before its children.  Then: cis2b_kv4_plan_tree for masks and
+ * positions; per layer cis2b_kv4_append and cis2b_kv4_tree_attention; when the
+ * model's own next token after every row is known, cis2b_kv4_accept, and
+ * cis2b_kv4_keep on the caches of all layers.  Next step's `cached` is kept[].
+ * All entry points follow the rules above: device pointers, asynchronous,
+ * nothing allocated, capturable, deterministic. */
+#define CIS2B_KV4_TREE_MOST 1024 /* rows of one request's tree; those past it are no part of it */
+#define CIS2B_KV4_TREE_PARENT 1  /* a parent < -1 or not before its child; taken as -1 */
+#define CIS2B_KV4_TREE_ROWS 2    /* a request with more rows than the masks (or CIS2B_KV4_TREE_MOST) hold */
+
+/* Masks and positions of drafted tokens.  Bit b % 32 of mask[row][b / 32] is
+ * set for row b of the request being the row itself or one of its ancestors;
+ * position[row] = cached + number of its ancestors.  Rows past 32 * words of
+ * their request, and rows past row_start[requests], get an empty mask and
+ * position -1. */
+typedef struct {
+  int32_t device;
+  int32_t requests; /* >= 1 */
+  int32_t rows;     /* of parent, mask and position */
+  int32_t words;    /* of a row of mask: 1 .. 32 */
+  const int32_t *length, *row_start, *parent;
+  int32_t *mask;     /* [rows][words] */
+  int32_t *position; /* [rows] */
+  int32_t *status;   /* one word or NULL: CIS2B_KV4_TREE_* bits OR-ed in */
+} cis2b_kv4_tree;
+int cis2b_kv4_plan_tree(const cis2b_kv4_tree *t, void *stream);
+
+/* The longest path of drafted tokens that the model agrees with.  target[row]
+ * is the model's next token after that row (greedy, or drawn by a sampler
+ * whose randomness goes by seed and position).  The path begins at row 0 and
+ * goes on, from row i, to the lowest row whose parent is i and whose token is
+ * target[i], as long as there is one.
+ *   accepted   [requests]  rows of the path: >= 1, or 0 for a request without rows
+ *   path       [rows]      path[row_start + k] is its k-th row within the
+ *              request; -1 from accepted on, and past row_start[requests]
+ *   next_token [requests]  target of its last row; -1 for a request without rows
+ *   kept       [requests]  cached + accepted */
+typedef struct {
+  int32_t device;
+  int32_t requests; /* >= 1 */
+  int32_t rows;
+  int32_t reserved; /* must be zero */
+  const int32_t *length, *row_start, *token, *parent, *target;
+  int32_t *accepted, *path, *next_token, *kept;
+  int32_t *status; /* as above */
+} cis2b_kv4_draft;
+int cis2b_kv4_accept(const cis2b_kv4_draft *d, void *stream);
+
+/* Moves, in each of n caches (of one device, page_size, kv_heads and
+ * head_dim), what slot[row_start + path[k]] holds to slot[row_start + k], for
+ * every request and k < accepted: bit for bit, all moves at once.  path[k] >=
+ * k; the slots of one call differ.  Entries with a slot < 0 are skipped, as
+ * are, with CIS2B_KV4_BAD_SLOT or CIS2B_KV4_BAD_PATH in the caches' status,
+ * those out of range. */
+#define CIS2B_KV4_BAD_PATH 8 /* path[k] < k, or not a row of the request */
+typedef struct {
+  int32_t device;
+  int32_t requests; /* >= 1 */
+  int32_t rows;
+  int32_t reserved; /* must be zero */
+  const int32_t *row_start, *accepted, *path, *slot;
+} cis2b_kv4_kept;
+int cis2b_kv4_keep(const cis2b_kv4_cache *caches, int32_t n, const cis2b_kv4_kept *k, void *stream);
+
+/* Attention of drafted tokens.  Row i of request r sees of its cached tokens
+ * (j < cached) all, or with window > 0 those with j > position[i] - window or
+ * j < sinks, and of its new ones those whose bit is set in mask[i] (no more
+ * than 32 * words, none at or past length[r]), whatever the window.  position
+ * is read with window > 0 only; one outside cached .. cached + n - 1 counts as
+ * the nearest inside.  Any bits may be set: a tree's, or another order of the
+ * new tokens among themselves.  Everything else as cis2b_kv4_attention. */
+int cis2b_kv4_tree_attention(const cis2b_kv4_cache *c, const cis2b_kv4_attn *a, const int32_t *mask, int32_t words,
+                             const int32_t *position, void *stream);
+/* Attention to an encoder's states: every row of request r sees the first
+ * length[r] tokens of its table, 0 or more, however many rows it has; nothing
+ * is causal.  window must be 0.  Requests may share pages.  Everything else as
+ * cis2b_kv4_attention. */
+int cis2b_kv4_cross_attention(const cis2b_kv4_cache *c, const cis2b_kv4_attn *a, void *stream);
+/* Bytes of `work` for either of the two. */
+int cis2b_kv4_tree_workspace(const cis2b_kv4_cache *c, const cis2b_kv4_attn *a, uint64_t *out_bytes);
+
 #ifdef __cplusplus
 }
 #endif
