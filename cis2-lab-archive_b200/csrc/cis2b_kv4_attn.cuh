@@ -1113,8 +1113,12 @@ int dispatch(const Shape &s, const AttArgs &args, const cis2b_kv4_cache *c, uint
       return !one ? launch<HD, 2, 2, true, SEE>(args, c, most, sms, st)
                   : bf16 ? launch<HD, 2, 1, false, SEE>(args, c, most, sms, st) : launch<HD, 2, 1, true, SEE>(args, c, most, sms, st);
     default:
-      return !one ? launch<HD, 4, 2, true, SEE>(args, c, most, sms, st)
-                  : bf16 ? launch<HD, 4, 1, false, SEE>(args, c, most, sms, st) : launch<HD, 4, 1, true, SEE>(args, c, most, sms, st);
+      // bfloat16 rows of a tree or over an encoder have another kernel from 17 columns on.
+      if constexpr (SEE != Rows::CAUSAL)
+        return !one ? launch<HD, 4, 2, true, SEE>(args, c, most, sms, st) : launch<HD, 4, 1, true, SEE>(args, c, most, sms, st);
+      else
+        return !one ? launch<HD, 4, 2, true, SEE>(args, c, most, sms, st)
+                    : bf16 ? launch<HD, 4, 1, false, SEE>(args, c, most, sms, st) : launch<HD, 4, 1, true, SEE>(args, c, most, sms, st);
   }
 }
 

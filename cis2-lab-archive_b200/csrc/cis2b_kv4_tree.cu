@@ -6,6 +6,8 @@
 namespace cis2b {
 namespace {
 
+#include "cis2b_kv4_columns.cuh"
+
 // A request's first row and its rows, as tokens_of() and rows_of(); `fresh`
 // counts new tokens that have no row, too.
 struct Request {
@@ -184,6 +186,78 @@ int check_rows(int32_t requests, int32_t rows) {
 
 constexpr int TREE_BLOCKS = 65536;  // at most; more requests take turns
 
+// ---------------------------------------------------------------- attention
+
+// bfloat16 rows of 17 to 64 query columns a request take k_kv4_columns, with 32
+// or 64 columns an item, and so do up to 128 columns of a batch of so few items
+// that most are cut, where its parts cost less.  Fewer columns take
+// k_kv4_attention, more k_kv4_prompt, and so do rows of other types.  Measured both
+// ways, us a call, columns first (64 requests, 413K keys, 32 over 8 heads of 128,
+// bf16): 16 columns 206 and 160, 32 columns 226 and 335, 64 columns 313 and 534,
+// 128 columns 598 and 493; one request of 130,051 keys with 128 columns, 8 KV
+// heads: 181 and 258; 8 prompts of 1,000 rows to encoders: 612 and 462.
+struct Columns {
+  bool on;
+  int nc, qt;
+  uint64_t items, bytes;
+};
+Columns columns_of(const cis2b_kv4_cache *c, const cis2b_kv4_attn *a) {
+  Columns s{};
+  const int group = a->heads / c->kv_heads;
+  const int64_t cols = (int64_t)group * a->max_new;
+  s.on = a->dtype == CIS2B_BF16 && cols > 16 && (cols <= 64 || (cols <= 128 && (int64_t)a->requests * c->kv_heads <= 2 * CO_BLOCKS));
+  s.nc = cols <= 32 ? 32 : 64;
+  s.qt = s.nc / group;
+  s.items = ((uint64_t)a->requests + (uint64_t)a->rows / s.qt) * c->kv_heads;  // at most
+  s.bytes = WORK_PARTS + (uint64_t)CO_BLOCKS * 2 * co_part(c->head_dim, s.nc) * 4;
+  return s;
+}
+static_assert(CO_BLOCKS <= WORK_ITEMS, "a counter per block");
+
+template <int HD, int NC, Rows SEE>
+int launch_columns(const AttArgs &args, const cis2b_kv4_cache *c, uint64_t most, int sms, cudaStream_t stream) {
+  static std::atomic<bool> ready[64];  // by device: the attribute is set
+  const int smem = co_smem_bytes(HD, NC);
+  if (!ready[c->device].load(std::memory_order_relaxed)) {
+    if (int rc = kv4_cuda(cudaFuncSetAttribute(k_kv4_columns<HD, NC, SEE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)))
+      return rc;
+    ready[c->device].store(true, std::memory_order_relaxed);
+  }
+  const int grid = (int)std::max<uint64_t>(1, std::min<uint64_t>(most, std::min(sms, CO_BLOCKS)));
+  k_kv4_columns<HD, NC, SEE><<<grid, co_threads(NC), smem, stream>>>(args);
+  return kv4_cuda(cudaGetLastError());
+}
+
+template <Rows SEE> int run_rows(const cis2b_kv4_cache *c, const cis2b_kv4_attn *a, const AttArgs &more, void *stream) {
+  if (int rc = kv4_check_cache(c, true)) return rc;
+  if (int rc = check_attn(c, a)) return rc;
+  const Columns s = columns_of(c, a);
+  if (!s.on) return run_attention<SEE>(c, a, more, stream);
+  if (s.items > ITEMS_MOST) return kv4_fail(CIS2B_ERR_ARG, "attention: (requests + rows) * kv_heads must be at most 2^30");
+  if (!a->table || !a->length || !a->row_start || (a->rows && (!a->q || !a->out)))
+    return kv4_fail(CIS2B_ERR_ARG, "attention: a device pointer is NULL");
+  if (a->work_bytes < s.bytes || !a->work || (reinterpret_cast<uintptr_t>(a->work) & 15))
+    return kv4_fail(CIS2B_ERR_ARG, "attention: work must be 16-byte aligned and hold cis2b_kv4_tree_workspace() bytes");
+  int sms = 0;
+  if (int rc = kv4_sm_count(c->device, &sms)) return rc;
+  if (int rc = kv4_cuda(cudaSetDevice(c->device))) return rc;
+  if (!a->rows) return CIS2B_OK;
+  AttArgs k = more;
+  Shape as{};
+  as.qt = s.qt, as.items = s.items;
+  fill(k, c, a, as);
+  k.counter = reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(a->work) + WORK_PROMPT);
+  k.part = reinterpret_cast<float *>(static_cast<uint8_t *>(a->work) + WORK_PARTS);
+  const uint64_t tiles = ((uint64_t)a->width * c->page_size / 16 + 1 + CO_RECS - 1) / CO_RECS;  // as tiles_bound()
+  // The row of tiles is counted in 32 bits; a batch that could pass that has items enough to take them whole.
+  k.whole = (a->flags & CIS2B_KV4_WHOLE) || s.items * (tiles + CO_SETUP) > INT_MAX;
+  const uint64_t most = k.whole ? s.items : s.items * ((tiles + CO_SETUP + CO_LEAST - 1) / CO_LEAST);
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (c->head_dim == 64)
+    return s.nc == 32 ? launch_columns<64, 32, SEE>(k, c, most, sms, st) : launch_columns<64, 64, SEE>(k, c, most, sms, st);
+  return s.nc == 32 ? launch_columns<128, 32, SEE>(k, c, most, sms, st) : launch_columns<128, 64, SEE>(k, c, most, sms, st);
+}
+
 }  // namespace
 }  // namespace cis2b
 
@@ -256,7 +330,8 @@ extern "C" int cis2b_kv4_tree_workspace(const cis2b_kv4_cache *c, const cis2b_kv
   if (int rc = kv4_check_cache(c, false)) return rc;
   if (int rc = check_attn(c, a)) return rc;
   if (!out_bytes) return kv4_fail(CIS2B_ERR_ARG, "out_bytes is NULL");
-  *out_bytes = shape_of(c, a).bytes;
+  const Columns s = columns_of(c, a);
+  *out_bytes = s.on ? s.bytes : shape_of(c, a).bytes;
   return CIS2B_OK;
 }
 
@@ -267,10 +342,10 @@ extern "C" int cis2b_kv4_tree_attention(const cis2b_kv4_cache *c, const cis2b_kv
     return kv4_fail(CIS2B_ERR_ARG, "tree attention: mask, or position with a window, is NULL");
   AttArgs more{};
   more.mask = mask, more.position = position, more.words = words;
-  return run_attention<Rows::TREE>(c, a, more, stream);
+  return run_rows<Rows::TREE>(c, a, more, stream);
 }
 
 extern "C" int cis2b_kv4_cross_attention(const cis2b_kv4_cache *c, const cis2b_kv4_attn *a, void *stream) {
   if (a && (a->window || a->sinks)) return kv4_fail(CIS2B_ERR_ARG, "cross attention: window and sinks must be 0");
-  return run_attention<Rows::CROSS>(c, a, AttArgs{}, stream);
+  return run_rows<Rows::CROSS>(c, a, AttArgs{}, stream);
 }

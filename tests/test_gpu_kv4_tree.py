@@ -287,7 +287,7 @@ def everyone(w):
     return lambda r, i: np.ones(w.lengths[r], bool)
 
 
-NEW = [1, 5, 14, 60]  # of 4 heads of one KV head: 4, 20, 56 and 240 query columns
+NEW = [1, 3, 5, 14, 30, 60]  # of 4 heads of one KV head: 4, 12, 20, 56, 120 and 240 query columns
 
 
 @pytest.mark.parametrize("new", NEW)
