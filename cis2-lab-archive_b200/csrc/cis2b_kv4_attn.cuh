@@ -391,6 +391,12 @@ __global__ __launch_bounds__(ATT_THREADS, NT == 1 ? 2 : 1) void k_kv4_attention(
   constexpr int PARTS = att_parts(HD, NT);
   // A code's operand is the code over this, of even and odd elements.
   constexpr float EVEN = EXACT ? 1.0f / 16.0f : 16777216.0f, ODD = EXACT ? 1.0f / 16.0f : 1048576.0f;
+  // The tensor cores cut their sums off where fp32 would round: 80 records lose
+  // 3e-6 of fp32 rows' results, 400 in k_kv4_prompt's chains 4e-6; plain fp32 has an
+  // error of 1e-6 to 2e-6.  Of rows that are no causal ones, whose bits stay as they
+  // are, each record's product is added up outside (0.9e-6 to 1.5e-6; 39,361 keys a
+  // request, 16 requests, 12 heads of 64: 100 us in place of 89).
+  constexpr bool OWN_SUMS = LIMBS == 2 && SEE != Rows::CAUSAL;
   // Sums and factors of the query columns, where registers are short (measured 7
   // to 10 percent slower with them in registers, which spill).
   constexpr bool COLUMNS_SHARED = NT == 4;
@@ -841,10 +847,21 @@ __global__ __launch_bounds__(ATT_THREADS, NT == 1 ? 2 : 1) void k_kv4_attention(
           for (int q = 0; q < 2; ++q) {
             const int m = 2 * w + q;  // rows of elements 32 w + 4 g + 2 q and the next
 #pragma unroll
-            for (int j = 0; j < NT; ++j)
+            for (int j = 0; j < NT; ++j) {
+              if constexpr (OWN_SUMS) {
+                float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-              for (int lm = 0; lm < LIMBS; ++lm)
-                mma16816(o[j][m], x[2 * q], x[2 * q + 1], y[2 * q], y[2 * q + 1], bw[k][j][lm][0], bw[k][j][lm][1]);
+                for (int lm = LIMBS - 1; lm >= 0; --lm)  // the small limb first
+                  mma16816(d, x[2 * q], x[2 * q + 1], y[2 * q], y[2 * q + 1], bw[k][j][lm][0], bw[k][j][lm][1]);
+                const float2 a0 = add2(make_float2(o[j][m][0], o[j][m][1]), make_float2(d[0], d[1])),
+                             a1 = add2(make_float2(o[j][m][2], o[j][m][3]), make_float2(d[2], d[3]));
+                o[j][m][0] = a0.x, o[j][m][1] = a0.y, o[j][m][2] = a1.x, o[j][m][3] = a1.y;
+              } else {
+#pragma unroll
+                for (int lm = 0; lm < LIMBS; ++lm)
+                  mma16816(o[j][m], x[2 * q], x[2 * q + 1], y[2 * q], y[2 * q + 1], bw[k][j][lm][0], bw[k][j][lm][1]);
+              }
+            }
           }
         }
 #pragma unroll
@@ -1036,13 +1053,15 @@ static_assert(8 + 4 * 2 * PR_BLOCKS <= WORK_PROMPT, "tickets and counters of k_k
 // Query columns per item: the fewest groups of 8 that hold one request's rows,
 // up to 32.
 constexpr uint64_t ITEMS_MOST = 1u << 30;  // a block's next item, its number plus the grid's, stays in 32 bits
-Shape shape_of(const cis2b_kv4_cache *c, const cis2b_kv4_attn *a) {
+// `own_sums`: fp32 rows that are no causal ones stay with k_kv4_attention, whatever
+// their number, see OWN_SUMS.
+Shape shape_of(const cis2b_kv4_cache *c, const cis2b_kv4_attn *a, bool own_sums = false) {
   Shape s;
   const int group = a->heads / c->kv_heads;
   const int64_t cols = (int64_t)group * a->max_new;
   s.nt = cols <= 8 ? 1 : cols <= 16 ? 2 : 4;
   s.limbs = a->dtype == CIS2B_F32 ? 2 : 1;
-  s.prompt = cols > 32;
+  s.prompt = cols > 32 && !own_sums;
   s.slots = 0;
   if (s.prompt) {
     s.cols = PR_ROWS;
@@ -1161,7 +1180,8 @@ template <Rows SEE> int run_attention(const cis2b_kv4_cache *c, const cis2b_kv4_
   if (int rc = check_attn(c, a)) return rc;
   if (!a->table || !a->length || !a->row_start || (a->rows && (!a->q || !a->out)))
     return kv4_fail(CIS2B_ERR_ARG, "attention: a device pointer is NULL");
-  const Shape s = shape_of(c, a);
+  const Shape s = shape_of(c, a, SEE != Rows::CAUSAL && a->dtype == CIS2B_F32);
+  if (s.items > ITEMS_MOST) return kv4_fail(CIS2B_ERR_ARG, "attention: (requests + rows) * kv_heads must be at most 2^30");
   if (a->work_bytes < s.bytes || !a->work || (reinterpret_cast<uintptr_t>(a->work) & 15))
     return kv4_fail(CIS2B_ERR_ARG, "attention: work must be 16-byte aligned and hold cis2b_kv4_workspace() bytes");
   int sms = 0;
@@ -1180,8 +1200,9 @@ template <Rows SEE> int run_attention(const cis2b_kv4_cache *c, const cis2b_kv4_
     const uint64_t tiles = ((uint64_t)a->width * c->page_size + PR_KEYS - 1) / PR_KEYS;
     const uint64_t most = s.items * ((tiles + PR_LEAST - 1) / PR_LEAST);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (a->dtype == CIS2B_F32)
-      return c->head_dim == 64 ? launch_prompt<64, 2, SEE>(p, c, most, sms, st) : launch_prompt<128, 2, SEE>(p, c, most, sms, st);
+    if constexpr (SEE == Rows::CAUSAL)
+      if (a->dtype == CIS2B_F32)
+        return c->head_dim == 64 ? launch_prompt<64, 2, SEE>(p, c, most, sms, st) : launch_prompt<128, 2, SEE>(p, c, most, sms, st);
     return c->head_dim == 64 ? launch_prompt<64, 1, SEE>(p, c, most, sms, st) : launch_prompt<128, 1, SEE>(p, c, most, sms, st);
   }
   k.counter = reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(a->work) + WORK_PROMPT);

@@ -39,15 +39,15 @@
 //
 // What bounds it.  Per tile of head_dim 128 HBM needs 760 cycles, 64 columns' two
 // products 512 each and its exponentials 512; measured (64 requests, 413K keys, 8
-// KV heads, bf16) are 2,100 with 32 columns (227 us a call) and 2,900 with 64 (313 us),
+// KV heads, bf16) are 2,100 with 32 columns (225 us a call) and 2,700 with 64 (292 us),
 // the softmax's warps working all the time and the others waiting for them.
 // Measured on the way (64 columns): 830 us with every warp walking the requests
 // itself (245 KB of code, instruction fetch), 580 with a scout, 412 with the seldom
 // run parts in loops (code runs the first time at 10 cycles an instruction), 322
 // with codes copied to shared memory in place of loads per key, 311 with operands
-// made by `and` and one multiply-add, 313 evenly shared and with one elected lane
-// issuing the products (120 cycles a product before), which narrower items gain
-// from: 32 columns 272 to 227.  Named barriers between the softmax's warps take 50
+// made by `and` and one multiply-add, 292 evenly shared, with a warp for queries
+// and one elected lane issuing the products (120 cycles a product before), which
+// narrower items gain from: 32 columns 272 to 225.  Named barriers between the softmax's warps take 50
 // cycles, memory barriers 500.
 #pragma once
 
@@ -64,6 +64,7 @@ constexpr float CO_UNIT = 16384.0f;  // of a row's factor; in the middle of the 
 // product, the scout and one for the queries.
 __host__ __device__ constexpr int co_sets(int nc) { return nc / 16; }
 __host__ __device__ constexpr int co_threads(int nc) { return 32 * (4 * co_sets(nc) + 2 * CO_CODES + 4); }
+__host__ __device__ constexpr int co_registers(int nc) { return nc == 64 ? 72 : 96; }  // a thread's at the launch, see below
 // Workspace: a counter per block, and two parts of an item per block.
 __host__ __device__ constexpr int co_part(int hd, int nc) { return nc * (hd + 2); }
 __host__ __device__ constexpr int co_smem_bytes(int hd, int nc) {
@@ -99,6 +100,8 @@ template <int ROW> __device__ __forceinline__ int line_piece(int k, int p) {
   static_assert(ROW == 128 || ROW == 64, "lines of 64 or 32 elements");
   return ROW == 128 ? p ^ (k & 7) : p ^ ((k >> 1) & 3);
 }
+constexpr int CO_WAIT = 1 << 20;  // polls of a barrier, of 0.1 us or more, before the kernel gives up
+
 // Shared memory by its 32-bit address, which stays in a register: the address of
 // a __shared__ variable is made anew for every access, from the block's number in
 // its cluster, whose reading takes 20 cycles.
@@ -131,7 +134,7 @@ __device__ __forceinline__ void co_wait_one(uint32_t b, uint32_t parity, uint32_
     int i = 0;
 #pragma unroll 1
     while (!bar_poll(b, parity) && !lds1(dead))
-      if (++i == PR_WAIT) sts1(dead, 1);
+      if (++i == CO_WAIT) sts1(dead, 1);
   }
 }
 __device__ __forceinline__ void co_wait(uint32_t b, uint32_t parity, uint32_t dead) {
@@ -322,7 +325,7 @@ __global__ __launch_bounds__(co_threads(NC), 1) void k_kv4_columns(AttArgs a) {
   // Registers go to the softmax's warps from the codes', out of what the launch
   // gives (a scheduler's warps share 512 a lane): 72 for each of 28 warps, or 96
   // for each of 20.
-  constexpr int AT_LAUNCH = NC == 64 ? 72 : 96, R_SOFT = NC == 64 ? 80 : 128, R_CODES = NC == 64 ? 56 : 64;
+  constexpr int AT_LAUNCH = co_registers(NC), R_SOFT = NC == 64 ? 80 : 128, R_CODES = NC == 64 ? 56 : 64;
   static_assert(SOFT * R_SOFT + 2 * CO_CODES * R_CODES + 4 * AT_LAUNCH <= THREADS / 32 * AT_LAUNCH, "what is taken is what is given");
   if (warp >= WARP_CODES && warp < WARP_S) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R_CODES));
@@ -868,7 +871,7 @@ __global__ __launch_bounds__(co_threads(NC), 1) void k_kv4_columns(AttArgs a) {
     if (elected()) tc_commit(b_end);
     __syncwarp();
 #pragma unroll 1
-    for (int i = 0; i < PR_WAIT && !__all_sync(0xffffffffu, bar_poll(b_end, 0)); ++i) {}
+    for (int i = 0; i < CO_WAIT && !__all_sync(0xffffffffu, bar_poll(b_end, 0)); ++i) {}
   }
   __syncthreads();
   if (tid == 0 && lds1(dead) && a.status) atomicOr(a.status, CIS2B_KV4_STUCK);

@@ -188,14 +188,14 @@ constexpr int TREE_BLOCKS = 65536;  // at most; more requests take turns
 
 // ---------------------------------------------------------------- attention
 
-// bfloat16 rows of 17 to 64 query columns a request take k_kv4_columns, with 32
-// or 64 columns an item, and so do up to 128 columns of a batch of so few items
-// that most are cut, where its parts cost less.  Fewer columns take
-// k_kv4_attention, more k_kv4_prompt, and so do rows of other types.  Measured both
-// ways, us a call, columns first (64 requests, 413K keys, 32 over 8 heads of 128,
-// bf16): 16 columns 206 and 160, 32 columns 226 and 335, 64 columns 313 and 534,
-// 128 columns 598 and 493; one request of 130,051 keys with 128 columns, 8 KV
-// heads: 181 and 258; 8 prompts of 1,000 rows to encoders: 612 and 462.
+// bfloat16 rows of 17 to 64 query columns a request take k_kv4_columns, with 32 or
+// 64 columns an item, and so do up to 128 columns of a batch of so few items that
+// most are cut, where its parts cost less.  Fewer columns take k_kv4_attention, more
+// k_kv4_prompt, and so do fp16 rows; fp32 rows always take k_kv4_attention.
+// Measured both ways, us a call, columns first (64 requests, 413K keys, 32 over 8
+// heads of 128): 16 columns 206 and 161, 32 columns 225 and 335, 64 columns 292
+// and 534, 128 columns 542 and 491; one request of 130,051 keys with 128 columns, 8
+// KV heads: 181 and 258; 8 prompts of 1,000 rows to encoders: 612 and 462.
 struct Columns {
   bool on;
   int nc, qt;
@@ -221,6 +221,10 @@ int launch_columns(const AttArgs &args, const cis2b_kv4_cache *c, uint64_t most,
   if (!ready[c->device].load(std::memory_order_relaxed)) {
     if (int rc = kv4_cuda(cudaFuncSetAttribute(k_kv4_columns<HD, NC, SEE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)))
       return rc;
+    // The kernel hands registers from warp to warp, out of what it is launched with.
+    cudaFuncAttributes made;
+    if (int rc = kv4_cuda(cudaFuncGetAttributes(&made, k_kv4_columns<HD, NC, SEE>))) return rc;
+    if (made.numRegs != co_registers(NC)) return kv4_fail(CIS2B_ERR_CUDA, "k_kv4_columns was built with other registers than it counts with");
     ready[c->device].store(true, std::memory_order_relaxed);
   }
   const int grid = (int)std::max<uint64_t>(1, std::min<uint64_t>(most, std::min(sms, CO_BLOCKS)));
@@ -331,7 +335,7 @@ extern "C" int cis2b_kv4_tree_workspace(const cis2b_kv4_cache *c, const cis2b_kv
   if (int rc = check_attn(c, a)) return rc;
   if (!out_bytes) return kv4_fail(CIS2B_ERR_ARG, "out_bytes is NULL");
   const Columns s = columns_of(c, a);
-  *out_bytes = s.on ? s.bytes : shape_of(c, a).bytes;
+  *out_bytes = s.on ? s.bytes : shape_of(c, a, a->dtype == CIS2B_F32).bytes;
   return CIS2B_OK;
 }
 
