@@ -477,13 +477,18 @@ int cis2b_kv4_keep(const cis2b_kv4_cache *caches, int32_t n, const cis2b_kv4_kep
  * than 32 * words, none at or past length[r]), whatever the window.  position
  * is read with window > 0 only; one outside cached .. cached + n - 1 counts as
  * the nearest inside.  Any bits may be set: a tree's, or another order of the
- * new tokens among themselves.  Everything else as cis2b_kv4_attention. */
+ * new tokens among themselves.  Everything else as cis2b_kv4_attention, but for
+ * the precision of two kinds of rows.  bfloat16 rows, where a request has 17 query
+ * columns (rows x heads / kv_heads) or more: every key and value is taken times a
+ * power of two of its own and rounded to 11 bits, no token's size mattering to
+ * another's; weights below 2^-18 of the row's largest are rounded to 2^-28 of it.
+ * fp32 rows: sums over keys are rounded to fp32, nothing is cut off. */
 int cis2b_kv4_tree_attention(const cis2b_kv4_cache *c, const cis2b_kv4_attn *a, const int32_t *mask, int32_t words,
                              const int32_t *position, void *stream);
 /* Attention to an encoder's states: every row of request r sees the first
  * length[r] tokens of its table, 0 or more, however many rows it has; nothing
- * is causal.  window must be 0.  Requests may share pages.  Everything else as
- * cis2b_kv4_attention. */
+ * is causal.  window and sinks must be 0.  Requests may share pages.  Everything
+ * else as cis2b_kv4_tree_attention. */
 int cis2b_kv4_cross_attention(const cis2b_kv4_cache *c, const cis2b_kv4_attn *a, void *stream);
 /* Bytes of `work` for either of the two. */
 int cis2b_kv4_tree_workspace(const cis2b_kv4_cache *c, const cis2b_kv4_attn *a, uint64_t *out_bytes);
