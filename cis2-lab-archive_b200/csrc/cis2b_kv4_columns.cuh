@@ -254,7 +254,7 @@ __global__ __launch_bounds__(co_threads(NC), 1) void k_kv4_columns(AttArgs a) {
   auto b_qfree = [&](uint32_t g) { return b1 + 8 * (14 + (g & 1)); };
   const uint32_t b_end = b1 + 8 * 16;
   if (tid == 0) {
-    for (uint32_t i = 0; i < CO_AHEAD; ++i) bar_init(b_raw(i), 32), bar_init(b_rawfree(i), 2 * CO_CODES);
+    for (uint32_t i = 0; i < CO_AHEAD; ++i) bar_init(b_raw(i), 33), bar_init(b_rawfree(i), 2 * CO_CODES);
     for (uint32_t i = 0; i < CO_SEGMENTS; ++i) bar_init(b_seg(i), 1), bar_init(b_segfree(i), 2);
     for (uint32_t i = 0; i < 4; ++i) bar_init(b_k(i), CO_CODES);
     for (uint32_t i = 0; i < 2; ++i)
@@ -672,9 +672,11 @@ __global__ __launch_bounds__(co_threads(NC), 1) void k_kv4_columns(AttArgs a) {
       auto tile_place = [&]() {
         if (t >= CO_AHEAD) co_wait(b_rawfree(t), (t / CO_AHEAD - 1) & 1, dead);
       };
-      auto tile_done = [&](int kind) {  // its copies count when they are there
-        if (lane == 0) sts1(s_kind + 4 * (t % CO_AHEAD), kind);
+      // Every lane's copies count when they are there.  That arrival is of copies alone:
+      // what lane 0 writes itself is released by one of its own.
+      auto tile_done = [&](int kind) {
         asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(b_raw(t)) : "memory");
+        if (lane == 0) sts1(s_kind + 4 * (t % CO_AHEAD), kind), bar_arrive(b_raw(t));
       };
       Segment g;
       while (at < end) {

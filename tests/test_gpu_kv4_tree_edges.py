@@ -1,0 +1,51 @@
+"""Drafted trees and encoders over the 4-bit cache at their edges: hand-offs between warps, the ends of the
+number range, requests alone and in large batches, windows shorter than a path, what a batch allocates.
+
+Tolerances are those of test_gpu_kv4_tree.py; where a test needs another one its comment derives it."""
+from __future__ import annotations
+
+import importlib
+
+import numpy as np
+import pytest
+
+from test_gpu_kv4 import World
+from test_gpu_kv4_tree import check
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def torch():
+    return importlib.import_module("torch")
+
+
+@pytest.fixture(scope="module")
+def kv4():
+    return importlib.import_module("cis2-lab-archive_b200.kv4")
+
+
+# ---------------------------------------------------------------- hand-offs between warps
+
+@pytest.mark.parametrize("new", [5, 14])  # of 4 heads of one KV head: 20 and 56 query columns
+@pytest.mark.parametrize("head_dim", [64, 128])
+@pytest.mark.parametrize("whole", [False, True])
+def test_short_items_hand_over(torch, kv4, head_dim, new, whole):
+    """Many items of none to a few key tiles behind one another in each block, some with missing pages: what is
+    there, the last tile of an item and the end of the work are known in time, call after call."""
+    g = np.random.default_rng(5)
+    lengths = [int(n) for n in g.choice([0, 1, 15, 127, 128, 129, 300, 700], 350)]
+    w = World(torch, kv4, lengths, [new] * 350, 1, head_dim, 16, "bfloat16", seed=4)
+    gone = [r for r in range(350) if lengths[r] > 200 and r % 3 == 0]
+    for r in gone:
+        w.table[r, 3] = -1
+    q = w.queries(4, head_dim)
+
+    def see(r, i):
+        j = np.arange(lengths[r])
+        return (j // 16 != 3) | (r not in gone)
+    want = w.cache.cross_attention(q, w.batch, max_new=new, whole=whole)
+    check(w, q, want, see)
+    for _ in range(100):
+        assert torch.equal(w.cache.cross_attention(q, w.batch, max_new=new, whole=whole), want)
+    assert w.cache.errors() == kv4.BAD_PAGE
