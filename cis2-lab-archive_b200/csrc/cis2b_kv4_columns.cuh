@@ -433,7 +433,8 @@ __global__ __launch_bounds__(co_threads(NC), 1) void k_kv4_columns(AttArgs a) {
           const float4 y = *reinterpret_cast<const float4 *>(col_top[c]);
           const float den = (y.x + y.y) + (y.z + y.w);
           const int64_t row = (int64_t)g.row0 + tok;
-          col_scale[c] = g.parts > 1 ? 4096.0f : den > 0.0f || den != den ? 4096.0f / den : 0.0f;  // the powers of V and W do not cancel
+          // 1 / den alone: values of 2^126 leave p of 2^-116, and 2^12 over that is none that fp32 has.
+          col_scale[c] = g.parts > 1 ? 1.0f : den > 0.0f || den != den ? 1.0f / den : 0.0f;
           col_out[c] = c >= g.ncol || row < 0 || row >= a.rows ? NOWHERE : row * a.o_row + (int64_t)(g.head * a.group + c - tok * a.group) * a.o_head;
           if (g.parts > 1) *reinterpret_cast<float2 *>(part + NC * HD + 2 * c) = make_float2(col_m[c], den);
         }
@@ -452,7 +453,7 @@ __global__ __launch_bounds__(co_threads(NC), 1) void k_kv4_columns(AttArgs a) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
               const int64_t at = col_out[c + i];
-              const float x = __uint_as_float(o[i]) * col_scale[c + i];
+              const float x = __uint_as_float(o[i]) * 4096.0f * col_scale[c + i];  // the powers of V and W do not cancel
               if (at == NOWHERE) continue;
               if (g.parts > 1) part[(c + i) * HD + element] = x;
               else static_cast<__nv_bfloat16 *>(a.out)[at + element] = __float2bfloat16_rn(x);

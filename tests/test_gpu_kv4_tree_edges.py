@@ -10,7 +10,7 @@ import numpy as np
 import pytest
 
 from test_gpu_kv4 import World
-from test_gpu_kv4_tree import check
+from test_gpu_kv4_tree import NEW, check, everyone, write
 
 pytestmark = pytest.mark.gpu
 
@@ -49,3 +49,18 @@ def test_short_items_hand_over(torch, kv4, head_dim, new, whole):
     for _ in range(100):
         assert torch.equal(w.cache.cross_attention(q, w.batch, max_new=new, whole=whole), want)
     assert w.cache.errors() == kv4.BAD_PAGE
+
+
+# ---------------------------------------------------------------- the ends of the number range
+
+@pytest.mark.parametrize("new", NEW)
+@pytest.mark.parametrize("size", [2.0 ** 125, 2.0 ** 126, 2.0 ** 127])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_few_keys_of_the_largest_values(torch, kv4, dtype, size, new):
+    """One key, or a few, whose values are the largest that a cache holds: their mean is one that the type holds."""
+    g = np.random.default_rng(3)
+    w = World(torch, kv4, [1, 2, 40], [new] * 3, 1, 64, 16, dtype)
+    for r, n in enumerate(w.lengths):
+        write(torch, w, w.x[r], np.float32(size) * g.uniform(1, 1.8, (n, 1, 64)).astype(np.float32), r)
+    q = w.queries(4, 64)
+    check(w, q, w.cache.cross_attention(q, w.batch, max_new=new), everyone(w))
