@@ -190,7 +190,8 @@ constexpr int TREE_BLOCKS = 65536;  // at most; more requests take turns
 
 // bfloat16 rows of 17 to 64 query columns a request take k_kv4_columns, with 32 or
 // 64 columns an item, and so do up to 128 columns of a batch of so few items that
-// most are cut, where its parts cost less.  Fewer columns take k_kv4_attention, more
+// most are cut, where its parts cost less; not with CIS2B_KV4_WHOLE, whose rows
+// must not go by the number of requests.  Fewer columns take k_kv4_attention, more
 // k_kv4_prompt, and so do fp16 rows; fp32 rows always take k_kv4_attention.
 // Measured both ways, us a call, columns first (64 requests, 413K keys, 32 over 8
 // heads of 128): 16 columns 206 and 161, 32 columns 225 and 335, 64 columns 292
@@ -205,7 +206,8 @@ Columns columns_of(const cis2b_kv4_cache *c, const cis2b_kv4_attn *a) {
   Columns s{};
   const int group = a->heads / c->kv_heads;
   const int64_t cols = (int64_t)group * a->max_new;
-  s.on = a->dtype == CIS2B_BF16 && cols > 16 && (cols <= 64 || (cols <= 128 && (int64_t)a->requests * c->kv_heads <= 2 * CO_BLOCKS));
+  const bool few = !(a->flags & CIS2B_KV4_WHOLE) && (int64_t)a->requests * c->kv_heads <= 2 * CO_BLOCKS;
+  s.on = a->dtype == CIS2B_BF16 && cols > 16 && cols <= (few ? 128 : 64);
   s.nc = cols <= 32 ? 32 : 64;
   s.qt = s.nc / group;
   s.items = ((uint64_t)a->requests + (uint64_t)a->rows / s.qt) * c->kv_heads;  // at most

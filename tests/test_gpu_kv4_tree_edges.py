@@ -10,7 +10,7 @@ import numpy as np
 import pytest
 
 from test_gpu_kv4 import World
-from test_gpu_kv4_tree import NEW, check, everyone, write
+from test_gpu_kv4_tree import DTYPES, NEW, Trees, check, everyone, i32, write
 
 pytestmark = pytest.mark.gpu
 
@@ -64,3 +64,21 @@ def test_few_keys_of_the_largest_values(torch, kv4, dtype, size, new):
         write(torch, w, w.x[r], np.float32(size) * g.uniform(1, 1.8, (n, 1, 64)).astype(np.float32), r)
     q = w.queries(4, 64)
     check(w, q, w.cache.cross_attention(q, w.batch, max_new=new), everyone(w))
+
+
+# ---------------------------------------------------------------- alone and in a batch
+
+@pytest.mark.parametrize("heads,new", [(8, 17), (64, 8), (8, 65), (64, 9), (64, 16), (8, 129)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_request_alone_gives_the_bits_it_gives_in_a_large_batch(torch, kv4, dtype, heads, new):
+    """17, 64, 65, 72, 128 and 129 query columns a KV head, 8 KV heads, alone and with 47 other requests."""
+    n, g = 48, np.random.default_rng(9)
+    t = Trees(torch, kv4, [int(x) for x in g.integers(new, 400, n)], [new] * n, 8, 64, 16, dtype, seed=81)
+    w, q = t.w, t.w.queries(heads, 64)
+    more = dict(max_new=new, whole=True)
+    tree, cross = w.cache.tree_attention(q, w.batch, **t.args, **more), w.cache.cross_attention(q, w.batch, **more)
+    for r in (0, 41):
+        rows = slice(r * new, (r + 1) * new)
+        one = kv4.Batch.of(w.table[r:r + 1], w.batch.length[r:r + 1].clone(), i32(torch, [0, new]), 16)
+        assert torch.equal(w.cache.tree_attention(q[rows], one, mask=t.args["mask"][rows], **more), tree[rows])
+        assert torch.equal(w.cache.cross_attention(q[rows], one, **more), cross[rows])

@@ -1,0 +1,21 @@
+"""CPU checks of what the forms of attention over the 4-bit cache ask for: the workspace's size shows which
+kernel a call takes."""
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+
+from test_kv4_tree_abi import attention, cache, kv4  # noqa: F401
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("new", [1, 2, 4, 5, 8, 16, 17, 32, 33, 64, 128, 129, 1000])
+def test_a_whole_request_takes_the_same_kernel_in_any_batch(kv4, dtype, new):  # noqa: F811
+    sizes = set()
+    for requests in (1, 2, 40, 81, 160, 161, 1000):
+        a = attention(kv4, dtype=dtype, max_new=new, requests=requests, rows=requests * new, flags=1)
+        n = ctypes.c_uint64()
+        assert kv4._lib().cis2b_kv4_tree_workspace(ctypes.byref(cache(kv4)), ctypes.byref(a), ctypes.byref(n)) == 0
+        sizes.add(n.value)
+    assert len(sizes) == 1
