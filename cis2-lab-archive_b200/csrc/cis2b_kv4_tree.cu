@@ -30,10 +30,11 @@ constexpr int TREE_THREADS = 128;
 // through the parents in shared memory and fills its words from the top down
 // (a parent stands before its child, so the walk only goes to lower words and
 // ends).  A walk is as long as the row is deep, about 30 cycles a step; that
-// and the launch bound the call.
-__global__ __launch_bounds__(TREE_THREADS) void k_kv4_plan_tree(cis2b_kv4_tree a) {
+// and the launch bound the call.  With a window a first walk finds the depth: the
+// ancestor `up` steps above a row is one that the window or the sinks hold.
+__global__ __launch_bounds__(TREE_THREADS) void k_kv4_plan_tree(cis2b_kv4_tree a, int window, int sinks) {
   __shared__ int16_t parent[CIS2B_KV4_TREE_MOST];
-  const int tid = threadIdx.x, most = 32 * a.words;
+  const int tid = threadIdx.x, most = 32 * a.words, near = window ? window : INT_MAX;
   int bad = 0;
   for (int r = blockIdx.x; r < a.requests; r += gridDim.x) {
     const Request q = request_of(a.row_start, r, a.rows);
@@ -48,13 +49,19 @@ __global__ __launch_bounds__(TREE_THREADS) void k_kv4_plan_tree(cis2b_kv4_tree a
     __syncthreads();
     for (int i = tid; i < q.on; i += TREE_THREADS) {
       int32_t *mask = a.mask + (int64_t)(q.row0 + i) * a.words;
-      int depth = -1, at = i < n ? i : -1;
+      int depth = -1, at = i < n ? i : -1, up = 0;
+      int64_t first = INT64_MAX;  // steps up to the last of the sinks
+      if (window) {
+        for (int x = at; x >= 0; x = parent[x]) ++depth;
+        first = (int64_t)cached + depth - sinks + 1;
+      }
       for (int w = a.words - 1; w >= 0; --w) {
         uint32_t bits = 0;
-        for (; at >= 32 * w; at = parent[at]) bits |= 1u << (at & 31), ++depth;
+        for (; at >= 32 * w; at = parent[at], ++up)
+          if (up < near || up >= first) bits |= 1u << (at & 31);
         mask[w] = (int32_t)bits;
       }
-      a.position[q.row0 + i] = i < n ? cached + depth : -1;
+      a.position[q.row0 + i] = i < n ? cached + up - 1 : -1;
     }
   }
   // Rows past the last request.
@@ -269,17 +276,20 @@ template <Rows SEE> int run_rows(const cis2b_kv4_cache *c, const cis2b_kv4_attn 
 
 using namespace cis2b;
 
-extern "C" int cis2b_kv4_plan_tree(const cis2b_kv4_tree *t, void *stream) {
+extern "C" int cis2b_kv4_plan_tree(const cis2b_kv4_tree *t, void *stream) { return cis2b_kv4_plan_tree_window(t, 0, 0, stream); }
+
+extern "C" int cis2b_kv4_plan_tree_window(const cis2b_kv4_tree *t, int32_t window, int32_t sinks, void *stream) {
   if (!t) return kv4_fail(CIS2B_ERR_ARG, "tree is NULL");
   if (int rc = check_rows(t->requests, t->rows)) return rc;
   if (t->words < 1 || 32 * t->words > CIS2B_KV4_TREE_MOST) return kv4_fail(CIS2B_ERR_ARG, "tree: words must be in 1..32");
+  if (window < 0 || sinks < 0) return kv4_fail(CIS2B_ERR_ARG, "tree: window and sinks must be >= 0");
   if (!t->length || !t->row_start || (t->rows && (!t->parent || !t->mask || !t->position)))
     return kv4_fail(CIS2B_ERR_ARG, "tree: a device pointer is NULL");
   int sms = 0;
   if (int rc = kv4_sm_count(t->device, &sms)) return rc;
   if (int rc = kv4_cuda(cudaSetDevice(t->device))) return rc;
   if (!t->rows) return CIS2B_OK;
-  k_kv4_plan_tree<<<std::min(t->requests, TREE_BLOCKS), TREE_THREADS, 0, static_cast<cudaStream_t>(stream)>>>(*t);
+  k_kv4_plan_tree<<<std::min(t->requests, TREE_BLOCKS), TREE_THREADS, 0, static_cast<cudaStream_t>(stream)>>>(*t, window, sinks);
   return kv4_cuda(cudaGetLastError());
 }
 

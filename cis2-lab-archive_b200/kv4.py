@@ -21,7 +21,7 @@ states, whose keys and values another cache holds:
 
     batch = kv4.Batch(requests=64, tokens=64 * 16, width=256, page_size=64, tree=16)
     batch.plan(cached, new, free_pages)
-    batch.plan_tree(parent)                    # batch.mask, batch.position
+    batch.plan_tree(parent)                    # batch.mask, batch.position; with a window: plan_tree(parent, window, sinks)
     cache.append(k, v, batch.slot)             # in every layer
     out = cache.tree_attention(q, batch, max_new=16)
     out = encoder.cross_attention(q, encoder_batch, max_new=16)
@@ -97,6 +97,7 @@ def _lib():
         L.cis2b_kv4_gather.argtypes = [_P, _I32, _P, _P, _P, _I32, _P]
         L.cis2b_kv4_workspace.argtypes = [_P, _P, _P]
         L.cis2b_kv4_attention.argtypes = [_P, _P, _P]
+        L.cis2b_kv4_plan_tree_window.argtypes = [_P, _I32, _I32, _P]
         L.cis2b_kv4_plan_tree.argtypes = [_P, _P]
         L.cis2b_kv4_accept.argtypes = [_P, _P]
         L.cis2b_kv4_keep.argtypes = [_P, _I32, _P, _P]
@@ -244,18 +245,25 @@ class Batch:
         torch.cuda.synchronize(self.device)  # on whichever stream it was
         return int(self.counts[2].item())
 
-    def plan_tree(self, parent) -> None:
-        """Masks and positions of drafted trees (cis2b_kv4_plan_tree): parent
-        [rows], int32, the row of the same request that each row continues, -1
-        for the cached tokens.  Fills mask and position.  `tree_errors` reads
-        what went wrong, if anything."""
+    def plan_tree(self, parent, window: int = 0, sinks: int = 0, mask=None) -> None:
+        """Masks and positions of drafted trees (cis2b_kv4_plan_tree_window):
+        parent [rows], int32, the row of the same request that each row
+        continues, -1 for the cached tokens.  Fills mask and position.  Give it
+        the window and sinks of the layers that the masks are for: a row does
+        not see ancestors outside them.  That matters only where a path is
+        longer than the window; then layers with other windows need masks of
+        their own: another call with `mask`, which is filled in place of the
+        batch's and passed to tree_attention.  `tree_errors` reads what went
+        wrong, if anything."""
         t = self._tree
         if t is None:
             raise ValueError("this batch was made without trees; give it `tree`, the most rows of one request")
         _ints(parent, "parent", self.device, (t.rows,))
         t.length, t.row_start, t.parent = self.length.data_ptr(), self.row_start.data_ptr(), parent.data_ptr()
-        t.mask, t.position = self.mask.data_ptr(), self.position.data_ptr()
-        _call(self.device, _lib().cis2b_kv4_plan_tree, ctypes.byref(t))
+        mask = self.mask if mask is None else _ints(mask, "mask", self.device, tuple(self.mask.shape))
+        _int32(("window", window), ("sinks", sinks))
+        t.mask, t.position = mask.data_ptr(), self.position.data_ptr()
+        _call(self.device, _lib().cis2b_kv4_plan_tree_window, ctypes.byref(t), window, sinks)
 
     def accept(self, token, parent, target) -> None:
         """The longest path of drafted tokens that the model agrees with
@@ -413,7 +421,8 @@ class Cache:
         tokens (with window > 0 those less than `window` before its position,
         and the first `sinks`), and of its new ones those whose bits mask
         [rows, words] has: bit b % 32 of word b // 32 for row b of the request.
-        mask and position [rows] are the batch's own (plan_tree) if None; any
+        The window hides no new token: where a path is longer than it, the mask
+        has to be one that plan_tree made for that window.  mask and position [rows] are the batch's own (plan_tree) if None; any
         mask may be given; position is read with a window only.  The rest is as
         in `attention`."""
         mask = batch.mask if mask is None else mask

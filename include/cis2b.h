@@ -407,8 +407,8 @@ int cis2b_kv4_attention(const cis2b_kv4_cache *c, const cis2b_kv4_attn *a, void 
  * tokens, in row order.  Row 0 of a request is the token that the model has
  * settled on last; parent[row] is the number, within the request, of the row
  * that a row continues, or -1 for one that continues the cached tokens.  A
- * parent stands before its children.  Then: cis2b_kv4_plan_tree for masks and
- * positions; per layer cis2b_kv4_append and cis2b_kv4_tree_attention; when the
+ * parent stands before its children.  Then: cis2b_kv4_plan_tree (of layers with a
+ * window cis2b_kv4_plan_tree_window) for masks and positions; per layer cis2b_kv4_append and cis2b_kv4_tree_attention; when the
  * model's own next token after every row is known, cis2b_kv4_accept, and
  * cis2b_kv4_keep on the caches of all layers.  Next step's `cached` is kept[].
  * All entry points follow the rules above: device pointers, asynchronous,
@@ -433,6 +433,13 @@ typedef struct {
   int32_t *status;   /* one word or NULL: CIS2B_KV4_TREE_* bits OR-ed in */
 } cis2b_kv4_tree;
 int cis2b_kv4_plan_tree(const cis2b_kv4_tree *t, void *stream);
+/* The same for layers with a sliding window: a row's mask leaves out the
+ * ancestors that stand `window` or more positions before it and are not among
+ * the first `sinks` positions, as causal attention of the text along the path
+ * would.  window 0: none.  Positions are the same.  Where no path is longer than
+ * the window the masks are cis2b_kv4_plan_tree's; where one is, layers with
+ * different windows need masks of their own. */
+int cis2b_kv4_plan_tree_window(const cis2b_kv4_tree *t, int32_t window, int32_t sinks, void *stream);
 
 /* The longest path of drafted tokens that the model agrees with.  target[row]
  * is the model's next token after that row (greedy, or drawn by a sampler
@@ -474,7 +481,8 @@ int cis2b_kv4_keep(const cis2b_kv4_cache *caches, int32_t n, const cis2b_kv4_kep
 /* Attention of drafted tokens.  Row i of request r sees of its cached tokens
  * (j < cached) all, or with window > 0 those with j > position[i] - window or
  * j < sinks, and of its new ones those whose bit is set in mask[i] (no more
- * than 32 * words, none at or past length[r]), whatever the window.  position
+ * than 32 * words, none at or past length[r]), whatever the window: which of its
+ * ancestors a window hides is in the mask (cis2b_kv4_plan_tree_window).  position
  * is read with window > 0 only; one outside cached .. cached + n - 1 counts as
  * the nearest inside.  Any bits may be set: a tree's, or another order of the
  * new tokens among themselves.  Everything else as cis2b_kv4_attention, but for

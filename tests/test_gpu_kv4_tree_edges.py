@@ -10,7 +10,7 @@ import numpy as np
 import pytest
 
 from test_gpu_kv4 import World
-from test_gpu_kv4_tree import DTYPES, NEW, Trees, check, everyone, i32, write
+from test_gpu_kv4_tree import DTYPES, NEW, Trees, bits, check, everyone, i32, plain_plan, random_parents, sees_tree, tolerance, write
 
 pytestmark = pytest.mark.gpu
 
@@ -82,3 +82,81 @@ def test_a_request_alone_gives_the_bits_it_gives_in_a_large_batch(torch, kv4, dt
         one = kv4.Batch.of(w.table[r:r + 1], w.batch.length[r:r + 1].clone(), i32(torch, [0, new]), 16)
         assert torch.equal(w.cache.tree_attention(q[rows], one, mask=t.args["mask"][rows], **more), tree[rows])
         assert torch.equal(w.cache.cross_attention(q[rows], one, **more), cross[rows])
+
+
+# ---------------------------------------------------------------- paths longer than the window
+
+WINDOWS = [(1, 0), (7, 0), (16, 2), (5, 43), (30, 300), (33, 0), (1000, 4)]
+
+
+def plain_window(parent, lengths, new, rows, words, window, sinks):
+    """plan_tree's masks and positions, less the ancestors that the window hides."""
+    mask, position = plain_plan(parent, lengths, new, rows, words)
+    start = np.concatenate([[0], np.cumsum(new)])
+    for r, n in enumerate(new):
+        for i in range(min(n, 32 * words)):
+            for b in range(i):
+                at = position[start[r] + b]
+                if at <= position[start[r] + i] - window and at >= sinks:
+                    mask[start[r] + i, b // 32] &= ~np.uint32(1 << (b % 32))
+    return mask, position
+
+
+@pytest.mark.parametrize("window,sinks", WINDOWS)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_chain_longer_than_the_window_is_causal_attention(torch, kv4, dtype, window, sinks):
+    """Tokens that each continue the last see what a layer with a sliding window shows them: the same rows as
+    attention()'s, within both kernels' tolerances."""
+    lengths, new, d = [300, 41, 5], [40, 33, 5], 64
+    w = World(torch, kv4, lengths, new, 2, d, 16, dtype, seed=9)
+    batch = kv4.Batch.of(w.table, w.batch.length, w.batch.row_start, 16, rows=78, tree=40)
+    batch.plan_tree(i32(torch, np.concatenate([np.arange(n) - 1 for n in new])), window, sinks)
+    q = w.queries(8, d)
+    more = dict(window=window, sinks=sinks, max_new=40)
+    a, b = w.cache.attention(q, w.batch, **more), w.cache.tree_attention(q, batch, **more)
+    top = max(np.abs(v).max() for v in w.v)
+    assert (a.double() - b.double()).abs().max().item() <= 2 * tolerance(w, q, d ** -0.5) * top
+    assert batch.tree_errors() == 0
+
+
+@pytest.mark.parametrize("window,sinks", WINDOWS)
+def test_plan_tree_with_a_window_matches_the_loops(torch, kv4, window, sinks):
+    g = np.random.default_rng(window)
+    for new, pad in (([1], 0), ([0, 5, 70], 3), ([31, 32, 33, 64, 65], 0), ([300, 3], 7)):
+        rows, tree, words = sum(new) + pad, max(new), (max(new) + 31) // 32
+        lengths = np.array(new) + g.integers(0, 60, len(new))
+        for parent in (random_parents(g, new, roots=True), random_parents(g, new, 1)):
+            given = i32(torch, np.concatenate([parent, np.zeros(pad, np.int64)]))
+            batch = kv4.Batch.of(i32(torch, np.zeros((len(new), 1))), i32(torch, lengths),
+                                 i32(torch, np.concatenate([[0], np.cumsum(new)])), 16, rows=rows, tree=tree)
+            own, other = plain_plan(parent, lengths, new, rows, words), torch.empty_like(batch.mask)
+            mask, position = plain_window(parent, lengths, new, rows, words, window, sinks)
+            batch.plan_tree(given)
+            batch.plan_tree(given, window, sinks, mask=other)  # the batch's own stays as it is
+            assert np.array_equal(other.cpu().numpy().view(np.uint32), mask)
+            assert np.array_equal(batch.mask.cpu().numpy().view(np.uint32), own[0])
+            assert np.array_equal(batch.position.cpu().numpy(), position)
+            batch.plan_tree(given, window, sinks)
+            assert torch.equal(batch.mask, other) and batch.tree_errors() == 0
+
+
+@pytest.mark.parametrize("heads", [2, 8, 24])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_trees_deeper_than_their_window(torch, kv4, dtype, heads):
+    lengths, new, window, sinks = [200, 44, 40], [40, 20, 40], 6, 3
+    t = Trees(torch, kv4, lengths, new, 2, 64, 16, dtype, seed=17)
+    w, q = t.w, t.w.queries(heads, 64)
+    mask, position = plain_window(t.parent, lengths, new, w.rows, 2, window, sinks)
+    assert not np.array_equal(mask, t.mask)
+    out = w.cache.tree_attention(q, w.batch, mask=bits(torch, mask), position=i32(torch, position), window=window,
+                                 sinks=sinks, max_new=40)
+    check(w, q, out, sees_tree(mask, position, lengths, new, window, sinks))
+
+
+def test_windows_of_plan_tree_are_checked(torch, kv4):
+    batch = kv4.Batch.of(i32(torch, [[0]]), i32(torch, [4]), i32(torch, [0, 4]), 16, rows=4, tree=4)
+    parent = i32(torch, [-1, 0, 1, 2])
+    for more in (dict(window=-1), dict(sinks=-1), dict(window=2 ** 31), dict(mask=batch.mask[:3]), dict(mask=batch.mask.long()),
+                 dict(mask=batch.mask.cpu())):
+        with pytest.raises((ValueError, kv4.Cis2Error)):
+            batch.plan_tree(parent, **more)

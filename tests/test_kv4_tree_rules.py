@@ -6,7 +6,7 @@ import ctypes
 
 import pytest
 
-from test_kv4_tree_abi import attention, cache, kv4  # noqa: F401
+from test_kv4_tree_abi import attention, cache, kv4, message  # noqa: F401
 
 
 @pytest.mark.parametrize("dtype", [0, 1, 2])
@@ -19,3 +19,10 @@ def test_a_whole_request_takes_the_same_kernel_in_any_batch(kv4, dtype, new):  #
         assert kv4._lib().cis2b_kv4_tree_workspace(ctypes.byref(cache(kv4)), ctypes.byref(a), ctypes.byref(n)) == 0
         sizes.add(n.value)
     assert len(sizes) == 1
+
+
+@pytest.mark.parametrize("window,sinks", [(-1, 0), (0, -1), (-2 ** 31, 3)])
+def test_bad_windows_of_a_tree_are_refused(kv4, window, sinks):  # noqa: F811
+    t = kv4._Tree(0, 2, 4, 1, *([256] * 5), None)
+    assert kv4._lib().cis2b_kv4_plan_tree_window(ctypes.byref(t), window, sinks, None) == 1 and "window" in message(kv4)
+    assert kv4._lib().cis2b_kv4_plan_tree_window(None, 0, 0, None) == 1
