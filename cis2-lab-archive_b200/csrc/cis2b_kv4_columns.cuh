@@ -24,7 +24,7 @@
 // Operands.  A group (a key, a value) is normalised by a power of two of its own,
 // a = the exponent of its largest possible element: its elements base + step c,
 // times 2^(-6 - a), are rounded ONCE to half precision (11 bits; the format's
-// parameters have 8).  So no token coarsens another.  Scores are S 2^(a - 8)
+// parameters have 8).  So no token coarsens another.  Scores are S 2^(a - 6)
 // factor, factor the row's own (see CO_UNIT), weights w = p 2^(a' - 6) with the
 // value's a' and p = 2^(score - M) in fp32, rounded to half precision; O stands
 // for 2^-12 of the result's numerator.  M is one integer per column, moves only
@@ -58,7 +58,13 @@ constexpr int CO_SEGMENTS = 4;   // and segments that it is ahead of the softmax
 constexpr int CO_LEAST = 2;      // least tiles that a block is given
 constexpr int CO_SETUP = 4;      // what an item's fixed costs come to, in tiles
 constexpr int CO_BLOCKS = 160;   // at most: one for each of 148 SMs, and some to spare
-constexpr float CO_UNIT = 16384.0f;  // of a row's factor; in the middle of the range of what products can be
+// A row's factor is the scale times CO_UNIT over the power of two that the row is an
+// operand with: 2^CO_UP if its largest element is 2^-11 .. 2^8 (those have one factor),
+// else one that brings that to 2^3, the largest of all to 2^15.  So factors are 2^-104 to
+// 2^124 times the scale and a key's part of a score 2^-112 to 2^122, and neither product
+// of the two passes fp32's range where the score does not.
+constexpr float CO_UNIT = 4096.0f;
+constexpr int CO_UP = 7;
 
 // Warps: the softmax first, four for each 16 columns, then K, V, then one for each
 // product, the scout and one for the queries.
@@ -358,7 +364,7 @@ __global__ __launch_bounds__(co_threads(NC), 1) void k_kv4_columns(AttArgs a) {
         // Of the score: 2^(a + 6) / CO_UNIT.  Of the weight: 2^(a - 6), log2 of it but
         // -86 at least, and the powers that go from one to the other and back to p.
         const int log = power_v - 6, most = max(log, -86);
-        sts4(s_scale + ((t & 3) * CO_KEYS + key) * 16, group_fine(p.x) && group_fine(p.y) ? __float_as_uint(power(power_k - 8)) : 0x7fffffffu,
+        sts4(s_scale + ((t & 3) * CO_KEYS + key) * 16, group_fine(p.x) && group_fine(p.y) ? __float_as_uint(power(power_k - 6)) : 0x7fffffffu,
              __float_as_uint(__int_as_float(0x4b400000 + most) - 12582912.0f), there ? __float_as_uint(power(log - most)) : 0u,
              __float_as_uint(power(-most)));
         tc_after();
@@ -399,7 +405,7 @@ __global__ __launch_bounds__(co_threads(NC), 1) void k_kv4_columns(AttArgs a) {
     // ---- weights: a key and a set of 16 columns per thread
     const int set = warp >> 2, key = tid & 127, col0 = set * CN;
     const uint32_t mine = tmem + ((uint32_t)(warp & 3) << 21);
-    const float common = a.scale * 1.4426950408889634f * CO_UNIT;
+    const float common = a.scale * (1.4426950408889634f * CO_UNIT) * power(-CO_UP);
     uint32_t seg = 0, qn = 0;  // segments; those with tiles
     Segment g;
     float2 minus[CN / 2], l[CN / 2];  // -M and the sums of p, pairs of columns
@@ -764,7 +770,7 @@ __global__ __launch_bounds__(co_threads(NC), 1) void k_kv4_columns(AttArgs a) {
       tile_done(4);
     } else if (warp == WARP_Q) {
       // ---- queries: eight lanes a column, four columns at a time, a segment ahead of the softmax
-      const float common = a.scale * 1.4426950408889634f * CO_UNIT;
+      const float unit = a.scale * (1.4426950408889634f * CO_UNIT);
       constexpr int PIECES = HD / 64;  // of 8 elements
       uint32_t qn = 0;  // segments with tiles
 #pragma unroll 1
@@ -776,7 +782,7 @@ __global__ __launch_bounds__(co_threads(NC), 1) void k_kv4_columns(AttArgs a) {
         if (to.first < 0 || lds1(dead)) break;
         if (to.j1 <= to.j0) continue;
         if (qn >= 2) co_wait(b_qfree(qn), (qn / 2 - 1) & 1, dead);
-        bool all = true;
+        bool all = fabsf(unit) < 2.0f * CO_UNIT;  // fp32 has the common factor's product with any key's part
         constexpr int AT_ONCE = 2;
 #pragma unroll 1
         for (int c0 = 0; c0 < NC; c0 += 4 * AT_ONCE) {
@@ -802,14 +808,13 @@ __global__ __launch_bounds__(co_threads(NC), 1) void k_kv4_columns(AttArgs a) {
               for (int i = 0; i < 4; ++i) top = fmaxf(top, fmaxf(fabsf(element(words[k][w][i], false)), fabsf(element(words[k][w][i], true))));
 #pragma unroll
             for (int d = 1; d < 8; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-            // A row whose largest element is 2^-4 .. 2^15 is an operand as it is: what
-            // half precision drops of it is below 2^-21 of that.  Others are brought to
-            // 2^13 by a power of two.
+            // What half precision drops of a row of 2^-11 .. 2^8 is below 2^-21 of its largest
+            // element, of others 2^-28.
             const int x = (int)(__float_as_uint(top) >> 23) - 127;
-            const bool alike = !on[k] || top == 0.0f || (x >= -4 && x < 15);
-            const int up = alike || x == 128 ? 0 : x == -127 ? Q_UP : min(13 - x, Q_UP);
+            const bool alike = !on[k] || top == 0.0f || (x >= -4 - CO_UP && x < 15 - CO_UP);
+            const int up = alike ? CO_UP : x == 128 ? 0 : x == -127 ? Q_UP : max(min(3 - x, Q_UP), -112);
             const float f = top == INFINITY ? __int_as_float(0x7fffffff) : power(up);  // an infinity makes the row NaN
-            if ((lane & 7) == 0) col_factor[qn & 1][col] = common * power(-up);
+            if ((lane & 7) == 0) col_factor[qn & 1][col] = unit * power(-up);
             all = all && alike;
 #pragma unroll
             for (int w = 0; w < PIECES; ++w) {

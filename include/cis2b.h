@@ -374,7 +374,9 @@ int cis2b_kv4_gather(const cis2b_kv4_cache *c, int32_t dtype, void *k, void *v, 
  * rows) or 11 (16-bit rows), those below 2^-10 (22 bits) or 2^-21 (11 bits) of
  * the row's largest to 2^-32 of it.  What a row does not see, whatever finite
  * or other number stands there, changes no bit of its result; a query row with
- * an infinity or a NaN is NaN where it sees anything. */
+ * an infinity or a NaN is NaN where it sees anything.  Queries of 2^120 and keys
+ * of 2^118 and more may make a NaN: sums on the way to their scores may pass
+ * fp32's range. */
 #define CIS2B_KV4_WHOLE 1
 #define CIS2B_KV4_WORK_ZERO 266240
 typedef struct {

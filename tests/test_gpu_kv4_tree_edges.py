@@ -10,7 +10,7 @@ import numpy as np
 import pytest
 
 from test_gpu_kv4 import World
-from test_gpu_kv4_tree import DTYPES, NEW, Trees, bits, check, everyone, i32, plain_plan, random_parents, sees_tree, tolerance, write
+from test_gpu_kv4_tree import DTYPES, NEW, Trees, bits, check, everyone, i32, plain_plan, plain_rows, random_parents, sees_tree, tolerance, write
 
 pytestmark = pytest.mark.gpu
 
@@ -64,6 +64,61 @@ def test_few_keys_of_the_largest_values(torch, kv4, dtype, size, new):
         write(torch, w, w.x[r], np.float32(size) * g.uniform(1, 1.8, (n, 1, 64)).astype(np.float32), r)
     q = w.queries(4, 64)
     check(w, q, w.cache.cross_attention(q, w.batch, max_new=new), everyone(w))
+
+
+@pytest.mark.parametrize("new", [5, 14, 30])  # of 4 heads: query columns that k_kv4_columns takes
+@pytest.mark.parametrize("q_power,k_power,scale,elements", [(0, 125, 1.0, 1), (-3, 126, 0.125, 1), (-100, 126, 0.125, 64),
+                                                            (-60, 120, 1.0, 64), (126, -100, 2.0, 64), (127, -110, 4.0, 64),
+                                                            (127, -5, 1.0, 1), (-110, 126, 16.0, 64), (-125, 120, 1.0, 64)])
+def test_scores_whose_factors_are_far_apart(torch, kv4, q_power, k_power, scale, elements, new):
+    """Queries and keys of the largest and smallest sizes, whose scores fp32 holds: the first is far above the
+    others, or all are near 0."""
+    d, n = 64, 300
+    g = np.random.default_rng(3)
+    w = World(torch, kv4, [n], [new], 1, d, 16, "bfloat16")
+    first = 77
+    t = np.where(np.arange(n) == first, 1.0, g.uniform(-1, 0.4, n))
+    write(torch, w, t[:, None, None] * g.uniform(1, 1.2, (n, 1, d)) * 2.0 ** k_power, w.y[0])
+    q = torch.zeros((new, 4, d), device="cuda")
+    q[:, :, :elements] = 2.0 ** q_power
+    q = q.to(w.dtype)
+    out = w.cache.cross_attention(q, w.batch, scale=scale, max_new=new)
+    want = plain_rows(q.double().cpu().numpy(), w.k, w.v, w.new, scale, everyone(w))
+    # Scores: a key's elements are rounded to 2^-11, and the largest score is 1.2 / (0.4 * 1.2) of the next: far apart,
+    # or (-125 + 120 + 6 bits) below 2^2, where tolerance() holds.  Values and weights: 11 bits, the result 8.
+    limit = 2 * (2.0 ** -11 * 4 + 2.0 ** -11) + 2.0 ** -11 + 2.0 ** -15 + 2.0 ** -8
+    assert np.abs(out.double().cpu().numpy() - want).max() <= limit * np.abs(w.v[0]).max()
+
+
+@pytest.mark.parametrize("new", NEW)
+@pytest.mark.parametrize("q_power,k_power", [(119, -100), (-100, 117), (0, 117), (119, 0)])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_scores_within_every_kernels_range(torch, kv4, dtype, q_power, k_power, new):
+    """Queries below 2^120 and keys below 2^118, all elements of one sign, in every kernel."""
+    d, n = 128, 300
+    g = np.random.default_rng(3)
+    w = World(torch, kv4, [n], [new], 1, d, 16, dtype)
+    t = np.where(np.arange(n) == 77, 1.0, g.uniform(0, 0.4, n))
+    write(torch, w, t[:, None, None] * g.uniform(1, 1.2, (n, 1, d)) * 2.0 ** k_power, w.y[0])
+    q = torch.full((new, 4, d), 2.0 ** q_power, device="cuda").to(w.dtype)
+    out = w.cache.cross_attention(q, w.batch, max_new=new).double().cpu().numpy()
+    # One key has all the weight: its value, in 22 or 11 bits, and the result's rounding.
+    assert np.abs(out - w.v[0][77]).max() <= {"float32": 2.0 ** -20, "bfloat16": 2.0 ** -10 + 2.0 ** -8}[dtype] * np.abs(w.v[0][77]).max()
+
+
+@pytest.mark.parametrize("new", [5, 14, 30])
+def test_unseen_keys_of_the_largest_size_change_no_bit(torch, kv4, new):
+    """Scores are formed in two ways, by the sizes of the keys beside them: with the same bits."""
+    d, n = 64, 300
+    w = World(torch, kv4, [n], [new], 1, d, 16, "bfloat16")
+    q = w.queries(4, d)
+    clean = w.cache.cross_attention(q, w.batch, max_new=new)
+    check(w, q, clean, everyone(w))
+    slot = i32(torch, [int(w.table[0, (n - 1) // 16]) * 16 + n % 16])  # behind the last key, in its tile and page
+    huge = torch.full((1, 1, d), 3e38, device="cuda")
+    huge[0, 0, ::2] = 1e30
+    w.cache.append(huge, huge, slot)
+    assert torch.equal(w.cache.cross_attention(q, w.batch, max_new=new), clean)
 
 
 # ---------------------------------------------------------------- alone and in a batch
