@@ -191,13 +191,17 @@ class Batch:
     def _trees(self, tree: int, rows: int) -> None:
         if not 0 <= tree <= TREE_MOST:
             raise ValueError(f"tree must be in 0..{TREE_MOST}")
-        self._tree = self._draft = self._kept = None
-        self._tree_bits = torch.zeros(1, dtype=torch.int32, device=f"cuda:{self.device}")
+        self._tree = self._draft = self._kept = self._bits = None
         if tree:
             words = (tree + 31) // 32
             self.mask = torch.zeros((rows, words), dtype=torch.int32, device=f"cuda:{self.device}")
-            self._tree = _Tree(self.device, self.length.numel(), rows, words, None, None, None, None, None,
-                               self._tree_bits.data_ptr())
+            self._tree = _Tree(self.device, self.length.numel(), rows, words, None, None, None, None, None, self._tree_bits())
+
+    def _tree_bits(self) -> int:
+        """The status word of plan_tree and accept, made by the first that needs it."""
+        if self._bits is None:
+            self._bits = torch.zeros(1, dtype=torch.int32, device=f"cuda:{self.device}")
+        return self._bits.data_ptr()
 
     @classmethod
     def of(cls, table, length, row_start, page_size: int, slot=None, rows: int | None = None, tree: int = 0) -> "Batch":
@@ -283,7 +287,7 @@ class Batch:
                 torch.full((m,), -1, dtype=torch.int32, device=f"cuda:{dev}") for m in (n, n, n, rows))
             d = self._draft = _Draft(dev, n, rows, 0, None, None, None, None, None, self.accepted.data_ptr(),
                                      self.path.data_ptr(), self.next_token.data_ptr(), self.kept.data_ptr(),
-                                     self._tree_bits.data_ptr())
+                                     self._tree_bits())
         d.length, d.row_start = self.length.data_ptr(), self.row_start.data_ptr()
         d.token, d.parent, d.target = token.data_ptr(), parent.data_ptr(), target.data_ptr()
         _call(dev, _lib().cis2b_kv4_accept, ctypes.byref(d))
@@ -312,11 +316,14 @@ class Batch:
 
     def tree_errors(self) -> int:
         """TREE_* bits that plan_tree and accept have left since the last time,
-        0 if all is well.  Waits for the GPU."""
+        0 if all is well.  Waits for the GPU.  (Of a batch without `tree`, if its
+        first accept was captured: those of the last replay.)"""
+        if self._bits is None:
+            return 0
         torch.cuda.synchronize(self.device)
-        bits = int(self._tree_bits.item())
+        bits = int(self._bits.item())
         if bits:
-            self._tree_bits.zero_()
+            self._bits.zero_()
             torch.cuda.synchronize(self.device)
         return bits
 

@@ -215,3 +215,18 @@ def test_windows_of_plan_tree_are_checked(torch, kv4):
                  dict(mask=batch.mask.cpu())):
         with pytest.raises((ValueError, kv4.Cis2Error)):
             batch.plan_tree(parent, **more)
+
+
+# ---------------------------------------------------------------- what a batch allocates
+
+def test_a_batch_over_the_callers_tensors_allocates_nothing(torch, kv4):
+    """Neither memory nor a kernel that would fill it: also inside a capture, where it would be a node."""
+    given = i32(torch, [[0]]), i32(torch, [4]), i32(torch, [0, 4])
+    slot = i32(torch, [0, 1, 2, 3])
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_stats()["allocation.all.allocated"]
+    kept = [kv4.Batch.of(*given, 16), kv4.Batch.of(*given, 16, slot=slot)]
+    assert torch.cuda.memory_stats()["allocation.all.allocated"] == before
+    assert [b.tree_errors() for b in kept] == [0, 0]
+    kept[0].accept(slot, slot, slot)  # row 0 is not before itself
+    assert kept[0].tree_errors() == kv4.TREE_PARENT and kept[0].tree_errors() == 0 and kept[1].tree_errors() == 0
