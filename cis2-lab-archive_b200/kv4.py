@@ -273,7 +273,9 @@ class Batch:
         """The longest path of drafted tokens that the model agrees with
         (cis2b_kv4_accept): token, parent and target [rows], int32; target is
         the model's next token after each row.  Fills accepted, path, next_token
-        and kept, the tokens that the request has cached from now on."""
+        and kept, the tokens that the request has cached from now on: the same
+        tensors each time (path: the first rows of one that is made larger when
+        it has to be; a captured call keeps the one it was captured with)."""
         dev = self.device
         if token.dim() != 1:
             raise ValueError("token must be [rows]")
@@ -283,8 +285,15 @@ class Batch:
         d = self._draft
         if d is None or d.rows != rows:
             _int32(("rows", rows))
-            self.accepted, self.next_token, self.kept, self.path = (
-                torch.full((m,), -1, dtype=torch.int32, device=f"cuda:{dev}") for m in (n, n, n, rows))
+            if self.accepted is None:
+                self.accepted, self.next_token, self.kept = (
+                    torch.full((n,), -1, dtype=torch.int32, device=f"cuda:{dev}") for _ in range(3))
+                self._paths = []  # all of them: captured calls may write to any
+            most = self._paths[-1].shape[0] if self._paths else -1
+            if rows > most:
+                size = max(rows, 2 * most, self.slot.shape[0] if self.slot is not None else 0)
+                self._paths.append(torch.full((size,), -1, dtype=torch.int32, device=f"cuda:{dev}"))
+            self.path = self._paths[-1][:rows]
             d = self._draft = _Draft(dev, n, rows, 0, None, None, None, None, None, self.accepted.data_ptr(),
                                      self.path.data_ptr(), self.next_token.data_ptr(), self.kept.data_ptr(),
                                      self._tree_bits())

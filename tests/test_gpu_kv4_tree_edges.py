@@ -230,3 +230,29 @@ def test_a_batch_over_the_callers_tensors_allocates_nothing(torch, kv4):
     assert [b.tree_errors() for b in kept] == [0, 0]
     kept[0].accept(slot, slot, slot)  # row 0 is not before itself
     assert kept[0].tree_errors() == kv4.TREE_PARENT and kept[0].tree_errors() == 0 and kept[1].tree_errors() == 0
+
+
+def test_accepts_of_any_number_of_rows_share_their_outputs(torch, kv4):
+    """What a captured call writes to stays the batch's, whatever calls come between."""
+    batch = kv4.Batch.of(i32(torch, [[0]]), i32(torch, [4]), i32(torch, [0, 4]), 16)
+    few, many = (torch.zeros(n, dtype=torch.int32, device="cuda") for n in (4, 900))
+    chain = i32(torch, [-1, 0, 1, 2])
+    batch.accept(few, chain, few)
+    first, outputs = batch.path, (batch.accepted, batch.next_token, batch.kept)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        batch.accept(few, chain, few)
+    assert batch.path.data_ptr() == first.data_ptr()
+    place = first.data_ptr()
+    del first
+    for rows in (900, 3, 0, 4, 700):
+        batch.accept(many[:rows], many[:rows] - 1, many[:rows])
+        assert all(a is b for a, b in zip(outputs, (batch.accepted, batch.next_token, batch.kept)))
+        assert batch.path.shape == (rows,)
+    others = [torch.full((n,), 77, dtype=torch.int32, device="cuda") for n in (1, 4, 900) for _ in range(20)]
+    assert all(x.data_ptr() != place for x in others)
+    graph.replay()
+    assert all((x == 77).all() for x in others)
+    assert batch.accepted.tolist() == [4] and batch.kept.tolist() == [4]
+    batch.accept(few, chain, few)
+    assert batch.path.tolist() == [0, 1, 2, 3]
