@@ -369,7 +369,11 @@ int cis2b_kv4_gather(const cis2b_kv4_cache *c, int32_t dtype, void *k, void *v, 
  *              captured ones among them) need one each.
  *              Zero it again after CIS2B_KV4_STUCK
  * Softmax statistics and sums are held in fp32 (of bf16 rows in the kernel for
- * one or few tokens, the tensor cores' sums keep about 15 bits).  Codes are
+ * one or few tokens, the tensor cores' sums keep about 15 bits).  The tensor cores
+ * cut off what falls below a sum's last bit, which adds up where values have one
+ * sign: fp32 rows over 32,768 (131,072) such keys are off by 2e-5 (1e-4) up to 32
+ * query columns and 2e-4 (9e-4) from there on with CIS2B_KV4_WHOLE, by 5e-7 and
+ * 6e-6 in parts.  Codes are
  * exact; a row's query elements and its weights are rounded to 22 bits (fp32
  * rows) or 11 (16-bit rows), those below 2^-10 (22 bits) or 2^-21 (11 bits) of
  * the row's largest to 2^-32 of it.  What a row does not see, whatever finite
@@ -494,7 +498,8 @@ int cis2b_kv4_keep(const cis2b_kv4_cache *caches, int32_t n, const cis2b_kv4_kep
  * another's; weights below 2^-18 of the row's largest are rounded to 2^-28 of it.
  * (Without CIS2B_KV4_WHOLE rows of 65 to 128 columns are such rows or not by the
  * number of requests, too.)
- * fp32 rows: sums over keys are rounded to fp32, nothing is cut off. */
+ * fp32 rows: the products of 16 keys are summed as the tensor cores do, which cut
+ * off what falls below fp32's last bit; the sums over those are rounded to fp32. */
 int cis2b_kv4_tree_attention(const cis2b_kv4_cache *c, const cis2b_kv4_attn *a, const int32_t *mask, int32_t words,
                              const int32_t *position, void *stream);
 /* Attention to an encoder's states: every row of request r sees the first

@@ -9,7 +9,7 @@ import importlib
 import numpy as np
 import pytest
 
-from test_gpu_kv4 import World
+from test_gpu_kv4 import World, stands_for
 from test_gpu_kv4_tree import DTYPES, NEW, Trees, bits, check, everyone, i32, plain_plan, plain_rows, random_parents, sees_tree, tolerance, write
 
 pytestmark = pytest.mark.gpu
@@ -119,6 +119,29 @@ def test_unseen_keys_of_the_largest_size_change_no_bit(torch, kv4, new):
     huge[0, 0, ::2] = 1e30
     w.cache.append(huge, huge, slot)
     assert torch.equal(w.cache.cross_attention(q, w.batch, max_new=new), clean)
+
+
+# ---------------------------------------------------------------- sums over many keys
+
+@pytest.mark.parametrize("new", [1, 4, 12, 20, 70])  # 4 to 280 query columns
+def test_fp32_sums_over_many_keys_are_rounded(torch, kv4, new):
+    """Every token has the same value, so that is the result, whatever the weights; what is off is sums.  Of 32,768
+    keys each of a block's eight warps adds up 256 records of 16.  Rounded to nearest, 256 adds are off by a standard
+    deviation of 2^-23 sqrt(256 / 36) (the sum so far grows evenly), the denominators' in eight lanes by less, and
+    eight warps' mean by 1 / sqrt(8) of that: 1.3e-7, eight of which are 1.1e-6.  Within a record two products of 16
+    addends and a sum cut off up to 2^-24 of the largest each, at most 2 * 17 * 2^-24 = 2.0e-6 of the whole.  Chains of
+    products over all records would cut off half of 2^-24 to 2^-23 of the sum so far, twice a record, always
+    towards zero: about 1.1e-5."""
+    n, d, page = 32768, 64, 64
+    cache = kv4.Cache(n // page, page, 1, d)
+    g = np.random.default_rng(0)
+    x = g.standard_normal((n, 1, d)).astype(np.float32)
+    y = np.where(np.arange(d) < d // 2, 1.0, -1.0).astype(np.float32)
+    cache.append(torch.from_numpy(x).cuda(), torch.from_numpy(y).cuda().expand(n, 1, d).contiguous(), i32(torch, np.arange(n)))
+    q = torch.from_numpy(g.standard_normal((new, 4, d)).astype(np.float32)).cuda()
+    batch = kv4.Batch.of(i32(torch, np.arange(n // page)[None]), i32(torch, [n]), i32(torch, [0, new]), page)
+    out = cache.cross_attention(q, batch, max_new=new, whole=True).double().cpu().numpy()
+    assert np.abs(out - stands_for(y[None])[0]).max() <= 3.2e-6
 
 
 # ---------------------------------------------------------------- alone and in a batch
