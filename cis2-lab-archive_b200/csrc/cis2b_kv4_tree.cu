@@ -196,14 +196,23 @@ constexpr int TREE_BLOCKS = 65536;  // at most; more requests take turns
 // ---------------------------------------------------------------- attention
 
 // bfloat16 rows of 17 to 64 query columns a request take k_kv4_columns, with 32 or
-// 64 columns an item, and so do up to 128 columns of a batch of so few items that
-// most are cut, where its parts cost less; not with CIS2B_KV4_WHOLE, whose rows
-// must not go by the number of requests.  Fewer columns take k_kv4_attention, more
-// k_kv4_prompt, and so do fp16 rows; fp32 rows always take k_kv4_attention.
-// Measured both ways, us a call, columns first (64 requests, 413K keys, 32 over 8
-// heads of 128): 16 columns 206 and 161, 32 columns 225 and 335, 64 columns 292
-// and 534, 128 columns 542 and 491; one request of 130,051 keys with 128 columns, 8
-// KV heads: 181 and 258; 8 prompts of 1,000 rows to encoders: 612 and 462.
+// 64 columns an item.  Fewer columns take k_kv4_attention, more k_kv4_prompt, and so do
+// fp16 rows; fp32 rows always take k_kv4_attention.  Measured both ways, us a call,
+// columns first (64 requests, 413K keys, 32 over 8 heads of 128): 16 columns 206 and
+// 161, 32 columns 226 and 335, 64 columns 295 and 534, 128 columns 547 and 491; 8
+// prompts of 1,000 rows to encoders: 612 and 462.
+// 65 to 128 columns take k_kv4_columns, twice, where a batch's items are few for the
+// keys that its tables hold: k_kv4_prompt cuts only long items and leaves SMs empty, and
+// its parts cost more.  Not with CIS2B_KV4_WHOLE, whose rows must not go by the batch.
+// Columns first, requests of half to all of these keys, 68 columns over heads of 128:
+//   keys     40 items      104          160          320         512
+//   500     28 and 32   40 and 33    50 and 34    78 and 52  113 and 64
+//   1,000   30 and 49   49 and 49    59 and 50    95 and 72
+//   2,000   40 and 79   60 and 79    77 and 85  129 and 113
+//   4,000                80 and 105              197 and 200  294 and 264
+//   8,000   62 and 89  119 and 182  173 and 219  313 and 359
+// 100 columns over heads of 64: 2,000 keys, 48 items 42 and 70, 96 items 61 and 73, 156
+// items 81 and 73; 8,000 keys, 156 items 159 and 179, 312 items 293 and 280.
 struct Columns {
   bool on;
   int nc, qt;
@@ -213,7 +222,10 @@ Columns columns_of(const cis2b_kv4_cache *c, const cis2b_kv4_attn *a) {
   Columns s{};
   const int group = a->heads / c->kv_heads;
   const int64_t cols = (int64_t)group * a->max_new;
-  const bool few = !(a->flags & CIS2B_KV4_WHOLE) && (int64_t)a->requests * c->kv_heads <= 2 * CO_BLOCKS;
+  int64_t keys = (int64_t)a->width * c->page_size;  // that a row may see
+  if (a->window) keys = std::min(keys, (int64_t)a->window + a->sinks + a->max_new);
+  const bool few = !(a->flags & CIS2B_KV4_WHOLE) &&
+                   (int64_t)a->requests * c->kv_heads <= std::max<int64_t>(40, std::min<int64_t>(2 * CO_BLOCKS, keys / (c->head_dim == 64 ? 16 : 10)));
   s.on = a->dtype == CIS2B_BF16 && cols > 16 && cols <= (few ? 128 : 64);
   s.nc = cols <= 32 ? 32 : 64;
   s.qt = s.nc / group;

@@ -497,7 +497,7 @@ int cis2b_kv4_keep(const cis2b_kv4_cache *caches, int32_t n, const cis2b_kv4_kep
  * power of two of its own and rounded to 11 bits, no token's size mattering to
  * another's; weights below 2^-18 of the row's largest are rounded to 2^-28 of it.
  * (Without CIS2B_KV4_WHOLE rows of 65 to 128 columns are such rows or not by the
- * number of requests, too.)
+ * number of requests and the tables' width, too.)
  * fp32 rows: the products of 16 keys are summed as the tensor cores do, which cut
  * off what falls below fp32's last bit; the sums over those are rounded to fp32. */
 int cis2b_kv4_tree_attention(const cis2b_kv4_cache *c, const cis2b_kv4_attn *a, const int32_t *mask, int32_t words,
