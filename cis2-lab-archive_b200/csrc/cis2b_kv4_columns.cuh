@@ -37,10 +37,13 @@
 // fp16 rows the error is 1.5 times that of exact ones, so they have the kernels
 // that work on the codes themselves.
 //
-// What bounds it.  Per tile of head_dim 128 HBM needs 760 cycles, 64 columns' two
-// products 512 each and its exponentials 512; measured (64 requests, 413K keys, 8
-// KV heads, bf16) are 2,100 with 32 columns (225 us a call) and 2,700 with 64 (292 us),
-// the softmax's warps working all the time and the others waiting for them.
+// What bounds it.  Per tile of head_dim 128 HBM needs 760 cycles and 64 columns'
+// exponentials 512.  Their two products hold the tensor pipe for 1,024 each, by its
+// counter (512 with 32 columns): four times as long as k_kv4_prompt's do for as much
+// work.  The softmax's warps take 1,900, one step after another.  Both overlap in
+// part: measured (64 requests, 413K keys, 8 KV heads, bf16), an item's fixed costs
+// included, are 3,200 with 64 columns (298 us a call, the pipe busy for 60 percent) and
+// 2,440 with 32 (226 us, 37 percent).
 // Measured on the way (64 columns): 830 us with every warp walking the requests
 // itself (245 KB of code, instruction fetch), 580 with a scout, 412 with the seldom
 // run parts in loops (code runs the first time at 10 cycles an instruction), 322

@@ -242,7 +242,8 @@ int launch_columns(const AttArgs &args, const cis2b_kv4_cache *c, uint64_t most,
   if (!ready[c->device].load(std::memory_order_relaxed)) {
     if (int rc = kv4_cuda(cudaFuncSetAttribute(k_kv4_columns<HD, NC, SEE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)))
       return rc;
-    // The kernel hands registers from warp to warp, out of what it is launched with.
+    // The kernel hands registers from warp to warp, out of what it is launched with.  That
+    // goes by its launch bounds, whatever its code needs; another count would make it wait.
     cudaFuncAttributes made;
     if (int rc = kv4_cuda(cudaFuncGetAttributes(&made, k_kv4_columns<HD, NC, SEE>))) return rc;
     if (made.numRegs != co_registers(NC)) return kv4_fail(CIS2B_ERR_CUDA, "k_kv4_columns was built with other registers than it counts with");
