@@ -196,6 +196,7 @@ class Batch:
             words = (tree + 31) // 32
             self.mask = torch.zeros((rows, words), dtype=torch.int32, device=f"cuda:{self.device}")
             self._tree = _Tree(self.device, self.length.numel(), rows, words, None, None, None, None, None, self._tree_bits())
+            self._tree_ref = ctypes.byref(self._tree)
 
     def _tree_bits(self) -> int:
         """The status word of plan_tree and accept, made by the first that needs it."""
@@ -265,9 +266,10 @@ class Batch:
         _ints(parent, "parent", self.device, (t.rows,))
         t.length, t.row_start, t.parent = self.length.data_ptr(), self.row_start.data_ptr(), parent.data_ptr()
         mask = self.mask if mask is None else _ints(mask, "mask", self.device, tuple(self.mask.shape))
-        _int32(("window", window), ("sinks", sinks))
+        if window or sinks:
+            _int32(("window", window), ("sinks", sinks))
         t.mask, t.position = mask.data_ptr(), self.position.data_ptr()
-        _call(self.device, _lib().cis2b_kv4_plan_tree_window, ctypes.byref(t), window, sinks)
+        _call(self.device, _lib().cis2b_kv4_plan_tree_window, self._tree_ref, window, sinks)
 
     def accept(self, token, parent, target) -> None:
         """The longest path of drafted tokens that the model agrees with
