@@ -440,9 +440,9 @@ class Cache:
         and the first `sinks`), and of its new ones those whose bits mask
         [rows, words] has: bit b % 32 of word b // 32 for row b of the request.
         The window hides no new token: where a path is longer than it, the mask
-        has to be one that plan_tree made for that window.  mask and position [rows] are the batch's own (plan_tree) if None; any
-        mask may be given; position is read with a window only.  The rest is as
-        in `attention`."""
+        has to be one that plan_tree made for that window.  mask and position
+        [rows] are the batch's own (plan_tree) if None; any mask may be given;
+        position is read with a window only.  The rest is as in `attention`."""
         mask = batch.mask if mask is None else mask
         position = batch.position if position is None else position
         if mask is None or mask.dim() != 2 or mask.shape[0] < q.shape[0] or not mask.shape[1]:
